@@ -225,6 +225,90 @@ int tans_scatter_payloads(const uint8_t* in, const int64_t* payload_offsets,
 int tans_cdf_fix_zero_freqs(int32_t* cdfs, int64_t rows, int64_t n, uint32_t* dev_status,
                             void* cuda_stream);
 
+/* ---- 4-bit key/value cache ------------------------------------------------------------------
+ * No counterpart in the reference.  A serving program that keeps its attention cache as small
+ * integers and codes them with this library needs the cache itself: rows quantised into pages,
+ * attention that reads them, and pages as symbol streams.  The cache of one layer is two arrays
+ * that the caller owns:
+ *   codes   uint8 [num_pages, 2, kv_heads, page_size, head_dim / 2]  4-bit codes, the even channel
+ *           in the low half of a byte; [:, 0] keys, [:, 1] values
+ *   params  bfloat16 [num_pages, 2, kv_heads, page_size, 2]          (scale, offset) of each row
+ * A code c stands for c * scale + offset.  A row x is stored with offset = bf16(min x),
+ * scale = bf16((max x - offset) / 15) (0 when that is under 2^-100) and
+ * c = round-half-even((x - offset) / scale) clamped to 0..15; a row that is not finite is stored
+ * with NaN parameters and reads back as NaN.  A slot numbers a token's place: page * page_size +
+ * place in the page.  head_dim is 64, 128 or 256, page_size a multiple of 16.  dtype (TANS_BF16 or
+ * TANS_FP16) is that of queries, keys, values and outputs; their rows (one token's head) are
+ * contiguous, strides are in elements. */
+#define TANS_BF16 0
+#define TANS_FP16 1
+
+/* Quantise tokens' keys and values into their slots, keys (and queries) with the position rotation
+ * applied on the way.
+ *   k, v      [tokens, kv_heads, head_dim]; q [tokens, q_heads, head_dim] or NULL
+ *   q_out     [tokens, q_heads, head_dim], packed: the rotated queries (NULL without q)
+ *   slots     int64[tokens]; a negative slot stores nothing, one past the pool is skipped and
+ *             flags TANS_DEV_BAD_INDEX.  Two tokens with the same slot leave either's row.
+ *   rotation  float [rotation_rows, rotary_dim]: cosines of the rotary_dim / 2 angles, then their
+ *             sines, one row per position; NULL = no rotation.  rotary_dim is a multiple of 16.
+ *   positions int64[tokens], rows of `rotation`; one outside is not rotated and flags
+ *             TANS_DEV_BAD_INDEX.
+ *   interleaved  0: channel i turns with i + rotary_dim / 2; 1: channel 2i with 2i + 1. */
+int tans_kv4_append(uint8_t* codes, void* params, int64_t num_pages, int kv_heads, int page_size, int head_dim,
+                    int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_token_stride, int64_t v_head_stride, const void* q, int64_t q_token_stride,
+                    int64_t q_head_stride, int q_heads, void* q_out, const int64_t* slots, int64_t tokens,
+                    const float* rotation, int64_t rotation_rows, int rotary_dim, const int64_t* positions,
+                    int interleaved, uint32_t* dev_status, void* cuda_stream);
+
+/* The values that the rows in `slots` stand for: k_out, v_out [tokens, kv_heads, head_dim], packed.
+ * Rows of a negative slot (or, flagging TANS_DEV_BAD_INDEX, of one past the pool) are zeros. */
+int tans_kv4_gather(const uint8_t* codes, const void* params, int64_t num_pages, int kv_heads, int page_size,
+                    int head_dim, int dtype, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
+                    uint32_t* dev_status, void* cuda_stream);
+
+/* Attention of packed queries over the cache: for sequence b, the queries q_starts[b] ..
+ * q_starts[b + 1] are the last of its lengths[b] tokens, query head h reads key/value head
+ * h / (q_heads / kv_heads), and
+ *   out = softmax(scale * q k^T) v  over the tokens up to and including the query's own (causal),
+ * or over all lengths[b] tokens (causal 0).  A query that sees no token gives zeros.  Statistics
+ * and sums are float.
+ *   q         [total_queries, q_heads, head_dim]; out the same shape, packed
+ *   pages     int32 [batch, max_pages]: the page that holds tokens i * page_size .. of a sequence.
+ *             Only the first ceil(lengths[b] / page_size) are read; one outside the pool hides its
+ *             tokens and flags TANS_DEV_BAD_INDEX.
+ *   lengths   int32 [batch]; outside 0 .. max_pages * page_size it is clamped and flags
+ *             TANS_DEV_BAD_VALUE.
+ *   q_starts  int32 [batch + 1], from 0 upwards; NULL: one query for each sequence.  Queries before
+ *             the first start and after the last give zeros.  A sequence whose two starts are out of
+ *             order or past the queries is skipped and flags TANS_DEV_BAD_VALUE.
+ *   max_queries  the caller's bound on one sequence's queries; it chooses the kernel only.
+ *   lse       float [total_queries, q_heads] or NULL: log of the softmax's sum (-inf for none).
+ *   workspace tans_kv4_attend_workspace_size() bytes, 256-byte aligned; NULL allocates it
+ *             stream-ordered. */
+size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim, int64_t batch,
+                                      int64_t max_pages, int page_size, int64_t max_queries);
+int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t total_queries, int q_heads,
+                    int dtype, const uint8_t* codes, const void* params, int64_t num_pages, int kv_heads,
+                    int page_size, int head_dim, const int32_t* pages, int64_t batch, int64_t max_pages,
+                    const int32_t* lengths, const int32_t* q_starts, int64_t max_queries, float scale, int causal,
+                    void* out, float* lse, void* workspace, size_t workspace_bytes, uint32_t* dev_status,
+                    void* cuda_stream);
+
+/* Pages as streams of the coder, one row for each page, side (keys, values) and head:
+ * symbols [n * 2 * kv_heads, page_size * head_dim] receives the codes of pages page_ids[0..n) in
+ * token order, indexes (same shape, or NULL) the table of each: side * kv_heads + head, or with
+ * by_channel (side * kv_heads + head) * head_dim + channel.  A page outside the pool gives zeros
+ * and flags TANS_DEV_BAD_INDEX. */
+int tans_kv4_to_symbols(const uint8_t* codes, int64_t num_pages, int kv_heads, int page_size, int head_dim,
+                        const int64_t* page_ids, int64_t n, int by_channel, int32_t* symbols, int32_t* indexes,
+                        uint32_t* dev_status, void* cuda_stream);
+
+/* Inverse of tans_kv4_to_symbols.  A symbol outside 0..15 is stored as its low four bits and flags
+ * TANS_DEV_BAD_VALUE; a page outside the pool is skipped and flags TANS_DEV_BAD_INDEX. */
+int tans_kv4_from_symbols(const int32_t* symbols, uint8_t* codes, int64_t num_pages, int kv_heads, int page_size,
+                          int head_dim, const int64_t* page_ids, int64_t n, uint32_t* dev_status, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,8 +20,9 @@ LOOKUP = {"search": LOOKUP_SEARCH, "invcdf": LOOKUP_INVCDF, "alias": LOOKUP_ALIA
 OK = 0
 DEV_BAD_INDEX, DEV_BAD_VALUE, DEV_OVERFLOW, DEV_UNDERFLOW, DEV_BAD_FREQ, DEV_BAD_ESCAPE = 1, 2, 4, 8, 16, 32
 DEV_STALLED = 64
+BF16, FP16 = 0, 1
 
-_P, _I64, _I, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+_P, _I64, _I, _SZ, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 _SIGS = {
     "tans_version": ([], _I),
     "tans_status_string": ([_I], ctypes.c_char_p),
@@ -42,6 +43,14 @@ _SIGS = {
     "tans_push_ragged": ([_I, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _P, _SZ, _P, _P],
                          _I),
     "tans_pop_ragged": ([_I, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _P, _P], _I),
+    "tans_kv4_append": ([_P, _P, _I64, _I, _I, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _I64,
+                         _P, _I64, _I, _P, _I, _P, _P], _I),
+    "tans_kv4_gather": ([_P, _P, _I64, _I, _I, _I, _I, _P, _I64, _P, _P, _P, _P], _I),
+    "tans_kv4_attend_workspace_size": ([_I64, _I, _I, _I, _I64, _I64, _I, _I64], _SZ),
+    "tans_kv4_attend": ([_P, _I64, _I64, _I64, _I, _I, _P, _P, _I64, _I, _I, _I, _P, _I64, _I64, _P, _P, _I64, _F, _I,
+                         _P, _P, _P, _SZ, _P, _P], _I),
+    "tans_kv4_to_symbols": ([_P, _I64, _I, _I, _I, _P, _I64, _I, _P, _P, _P, _P], _I),
+    "tans_kv4_from_symbols": ([_P, _P, _I64, _I, _I, _I, _P, _I64, _P, _P], _I),
     "tans_probe": ([_I, _I64, ctypes.POINTER(ctypes.c_double)], _I),
 }
 

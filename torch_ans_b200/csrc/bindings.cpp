@@ -13,6 +13,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <tuple>
 #include <mutex>
@@ -773,6 +774,199 @@ std::tuple<Tensor, Tensor> alias_build_table(const Tensor& cdfs, const Tensor& c
   return {remap, table};
 }
 
+// ------------------------------------------------------------------ 4-bit key/value cache
+// Argument checks and outputs of the kv4_* ops (include/torch_ans_b200.h has the layout and the
+// meaning of each array).  Nothing is copied or cast here: a tensor of another type, device or
+// layout raises.
+struct Kv4Pool {
+  at::Device dev;
+  int64_t num_pages, kv_heads, page_size, head_dim;
+};
+
+void kv4_codes_ok(const Tensor& codes) {
+  TORCH_CHECK(codes.is_cuda(), "torch_ans_b200: `codes` must be a CUDA tensor");
+  TORCH_CHECK(codes.scalar_type() == torch::kUInt8 && codes.dim() == 5 && codes.size(1) == 2 && codes.is_contiguous(),
+              "torch_ans_b200: `codes` must be a contiguous uint8 tensor (pages, 2, kv_heads, page_size, head_dim / 2)");
+  const int64_t dim = 2 * codes.size(4);
+  TORCH_CHECK(dim == 64 || dim == 128 || dim == 256, "torch_ans_b200: head_dim must be 64, 128 or 256, not ", dim);
+  TORCH_CHECK(codes.size(3) >= 16 && codes.size(3) % 16 == 0 && codes.size(3) <= (1 << 20) && codes.size(2) >= 1 &&
+                  codes.size(2) <= 65535,
+              "torch_ans_b200: page_size must be a multiple of 16 and kv_heads at least 1");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "torch_ans_b200: `codes` must be 16-byte aligned");
+}
+
+Kv4Pool kv4_pool(const Tensor& codes, const Tensor& params) {
+  kv4_codes_ok(codes);
+  TORCH_CHECK(params.scalar_type() == torch::kBFloat16 && params.dim() == 5 && params.is_contiguous() &&
+                  params.sizes().slice(0, 4) == codes.sizes().slice(0, 4) && params.size(4) == 2,
+              "torch_ans_b200: `params` must be a contiguous bfloat16 tensor (pages, 2, kv_heads, page_size, 2) beside `codes`");
+  TORCH_CHECK(params.device() == codes.device(), "torch_ans_b200: `params` must be on the device of `codes`");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(params.data_ptr()) % 16 == 0, "torch_ans_b200: `params` must be 16-byte aligned");
+  return {codes.device(), codes.size(0), codes.size(2), codes.size(3), 2 * codes.size(4)};
+}
+
+int kv4_dtype(at::ScalarType t, const char* name) {
+  TORCH_CHECK(t == torch::kBFloat16 || t == torch::kHalf, "torch_ans_b200: `", name, "` must be bfloat16 or float16");
+  return t == torch::kHalf ? TANS_FP16 : TANS_BF16;
+}
+
+void kv4_rows(const Tensor& t, const char* name, const Kv4Pool& p, int64_t tokens, at::ScalarType type) {
+  TORCH_CHECK(t.device() == p.dev, "torch_ans_b200: `", name, "` must be on the device of `codes`");
+  TORCH_CHECK(t.scalar_type() == type, "torch_ans_b200: `", name, "` has another dtype than the other rows");
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == tokens && t.size(2) == p.head_dim,
+              "torch_ans_b200: `", name, "` must be (", tokens, ", heads, ", p.head_dim, ")");
+  TORCH_CHECK(t.numel() == 0 || t.stride(2) == 1, "torch_ans_b200: a row (last dimension) of `", name, "` must be contiguous");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "torch_ans_b200: `", name,
+              "` requires a gradient, and the 4-bit cache has none");
+}
+
+void kv4_vector(const Tensor& t, const char* name, const at::Device& dev, int64_t n, at::ScalarType type) {
+  TORCH_CHECK(t.device() == dev, "torch_ans_b200: `", name, "` must be on the device of `codes`");
+  TORCH_CHECK(t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), "torch_ans_b200: `", name,
+              "` must be a contiguous ", at::toString(type), " tensor of ", n, " entries");
+}
+
+uint32_t* kv4_status(const at::Device& dev) { return reinterpret_cast<uint32_t*>(status_word(dev).data_ptr<int32_t>()); }
+
+std::optional<Tensor> kv4_append(const Tensor& codes, const Tensor& params, const Tensor& k, const Tensor& v,
+                                 const Tensor& slots, const std::optional<Tensor>& q,
+                                 const std::optional<Tensor>& positions, const std::optional<Tensor>& rotation,
+                                 bool interleaved) {
+  const Kv4Pool p = kv4_pool(codes, params);
+  c10::cuda::CUDAGuard guard(p.dev);
+  const int64_t n = slots.numel();
+  const int dtype = kv4_dtype(k.scalar_type(), "k");
+  kv4_vector(slots, "slots", p.dev, n, torch::kInt64);
+  kv4_rows(k, "k", p, n, k.scalar_type());
+  kv4_rows(v, "v", p, n, k.scalar_type());
+  TORCH_CHECK(k.size(1) == p.kv_heads && v.size(1) == p.kv_heads, "torch_ans_b200: `k` and `v` must have the cache's ",
+              p.kv_heads, " heads");
+  TORCH_CHECK(positions.has_value() == rotation.has_value(), "torch_ans_b200: `positions` and `rotation` go together");
+  int64_t rotary = 0, rows = 0;
+  if (rotation) {
+    kv4_vector(*positions, "positions", p.dev, n, torch::kInt64);
+    TORCH_CHECK(rotation->device() == p.dev && rotation->scalar_type() == torch::kFloat32 && rotation->dim() == 2 &&
+                    rotation->is_contiguous(),
+                "torch_ans_b200: `rotation` must be a contiguous float32 tensor (positions, rotary_dim) on the device of `codes`");
+    rows = rotation->size(0);
+    rotary = rotation->size(1);
+    TORCH_CHECK(rows >= 1 && rotary >= 16 && rotary <= p.head_dim && rotary % 16 == 0,
+                "torch_ans_b200: rotary_dim must be a multiple of 16 up to head_dim, not ", rotary);
+  }
+  std::optional<Tensor> out;
+  if (q) {
+    kv4_rows(*q, "q", p, n, k.scalar_type());
+    TORCH_CHECK(q->size(1) >= 1 && q->size(1) <= 65535, "torch_ans_b200: `q` must have at least one head");
+    out = torch::empty({n, q->size(1), p.head_dim}, q->options().memory_format(at::MemoryFormat::Contiguous));
+  }
+  check_rc(tans_kv4_append(codes.data_ptr<uint8_t>(), params.data_ptr(), p.num_pages, (int)p.kv_heads,
+                           (int)p.page_size, (int)p.head_dim, dtype, k.data_ptr(), k.stride(0), k.stride(1),
+                           v.data_ptr(), v.stride(0), v.stride(1), q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0,
+                           q ? q->stride(1) : 0, q ? (int)q->size(1) : 0, out ? out->data_ptr() : nullptr,
+                           slots.data_ptr<int64_t>(), n, rotation ? rotation->data_ptr<float>() : nullptr, rows,
+                           (int)rotary, positions ? positions->data_ptr<int64_t>() : nullptr, interleaved,
+                           kv4_status(p.dev), cur_stream()),
+           "kv4 append");
+  after_op(p.dev);
+  return out;
+}
+
+std::tuple<Tensor, Tensor> kv4_gather(const Tensor& codes, const Tensor& params, const Tensor& slots,
+                                      at::ScalarType dtype) {
+  const Kv4Pool p = kv4_pool(codes, params);
+  c10::cuda::CUDAGuard guard(p.dev);
+  const int64_t n = slots.numel();
+  kv4_vector(slots, "slots", p.dev, n, torch::kInt64);
+  const int t = kv4_dtype(dtype, "dtype");
+  auto opt = torch::TensorOptions().dtype(dtype).device(p.dev);
+  Tensor k = torch::empty({n, p.kv_heads, p.head_dim}, opt), v = torch::empty({n, p.kv_heads, p.head_dim}, opt);
+  check_rc(tans_kv4_gather(codes.data_ptr<uint8_t>(), params.data_ptr(), p.num_pages, (int)p.kv_heads, (int)p.page_size,
+                           (int)p.head_dim, t, slots.data_ptr<int64_t>(), n, k.data_ptr(), v.data_ptr(),
+                           kv4_status(p.dev), cur_stream()),
+           "kv4 gather");
+  after_op(p.dev);
+  return {k, v};
+}
+
+Tensor kv4_attend(const Tensor& q, const Tensor& codes, const Tensor& params, const Tensor& pages, const Tensor& lengths,
+                  const std::optional<Tensor>& q_starts, std::optional<int64_t> max_queries, std::optional<double> scale,
+                  bool causal, const std::optional<Tensor>& lse) {
+  const Kv4Pool p = kv4_pool(codes, params);
+  c10::cuda::CUDAGuard guard(p.dev);
+  const int dtype = kv4_dtype(q.scalar_type(), "q");
+  TORCH_CHECK(q.dim() == 3, "torch_ans_b200: `q` must be (queries, heads, head_dim)");
+  const int64_t n = q.size(0), heads = q.size(1), batch = lengths.numel();
+  kv4_rows(q, "q", p, n, q.scalar_type());
+  TORCH_CHECK(heads >= 1 && heads <= 65535 && heads % p.kv_heads == 0, "torch_ans_b200: ", heads,
+              " query heads do not share ", p.kv_heads, " key/value heads");
+  kv4_vector(lengths, "lengths", p.dev, batch, torch::kInt32);
+  TORCH_CHECK(pages.device() == p.dev && pages.scalar_type() == torch::kInt32 && pages.dim() == 2 &&
+                  pages.size(0) == batch && pages.is_contiguous(),
+              "torch_ans_b200: `pages` must be a contiguous int32 tensor (", batch, ", max_pages) on the device of `codes`");
+  if (q_starts) {
+    kv4_vector(*q_starts, "q_starts", p.dev, batch + 1, torch::kInt32);
+  } else {
+    TORCH_CHECK(n == batch, "torch_ans_b200: without `q_starts` there is one query for each sequence (", batch, "), not ", n);
+  }
+  TORCH_CHECK(!max_queries || *max_queries >= 0, "torch_ans_b200: max_queries must not be negative");
+  if (lse)
+    TORCH_CHECK(lse->device() == p.dev && lse->scalar_type() == torch::kFloat32 && lse->dim() == 2 &&
+                    lse->size(0) == n && lse->size(1) == heads && lse->is_contiguous(),
+                "torch_ans_b200: `lse` must be a contiguous float32 tensor (", n, ", ", heads, ") on the device of `codes`");
+  Tensor out = torch::empty({n, heads, p.head_dim}, q.options().memory_format(at::MemoryFormat::Contiguous));
+  const int64_t most = max_queries ? *max_queries : (q_starts ? n : 1);
+  const size_t need = tans_kv4_attend_workspace_size(n, (int)heads, (int)p.kv_heads, (int)p.head_dim, batch,
+                                                     pages.size(1), (int)p.page_size, most);
+  Tensor ws;
+  if (need) ws = torch::empty({(int64_t)need}, torch::TensorOptions().dtype(torch::kUInt8).device(p.dev));
+  check_rc(tans_kv4_attend(q.data_ptr(), q.stride(0), q.stride(1), n, (int)heads, dtype, codes.data_ptr<uint8_t>(),
+                           params.data_ptr(), p.num_pages, (int)p.kv_heads, (int)p.page_size, (int)p.head_dim,
+                           pages.data_ptr<int32_t>(), batch, pages.size(1), lengths.data_ptr<int32_t>(),
+                           q_starts ? q_starts->data_ptr<int32_t>() : nullptr, most,
+                           scale ? (float)*scale : 1.0f / std::sqrt((float)p.head_dim), causal, out.data_ptr(),
+                           lse ? lse->data_ptr<float>() : nullptr, need ? ws.data_ptr() : nullptr, need,
+                           kv4_status(p.dev), cur_stream()),
+           "kv4 attend");
+  after_op(p.dev);
+  return out;
+}
+
+std::tuple<Tensor, Tensor> kv4_to_symbols(const Tensor& codes, const Tensor& page_ids, bool by_channel) {
+  kv4_codes_ok(codes);
+  const at::Device dev = codes.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t n = page_ids.numel();
+  kv4_vector(page_ids, "page_ids", dev, n, torch::kInt64);
+  const int64_t rows = n * 2 * codes.size(2), width = codes.size(3) * codes.size(4) * 2;
+  auto i32 = torch::TensorOptions().dtype(torch::kInt32).device(dev);
+  Tensor symbols = torch::empty({rows, width}, i32), indexes = torch::empty({rows, width}, i32);
+  check_rc(tans_kv4_to_symbols(codes.data_ptr<uint8_t>(), codes.size(0), (int)codes.size(2), (int)codes.size(3),
+                               (int)codes.size(4) * 2, page_ids.data_ptr<int64_t>(), n, by_channel,
+                               symbols.data_ptr<int32_t>(), indexes.data_ptr<int32_t>(), kv4_status(dev), cur_stream()),
+           "kv4 to symbols");
+  after_op(dev);
+  return {symbols, indexes};
+}
+
+void kv4_from_symbols(const Tensor& symbols, const Tensor& codes, const Tensor& page_ids) {
+  kv4_codes_ok(codes);
+  const at::Device dev = codes.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t n = page_ids.numel();
+  kv4_vector(page_ids, "page_ids", dev, n, torch::kInt64);
+  const int64_t rows = n * 2 * codes.size(2), width = codes.size(3) * codes.size(4) * 2;
+  TORCH_CHECK(symbols.device() == dev && symbols.scalar_type() == torch::kInt32 && symbols.dim() == 2 &&
+                  symbols.size(0) == rows && symbols.size(1) == width && symbols.is_contiguous() &&
+                  reinterpret_cast<uintptr_t>(symbols.data_ptr()) % 16 == 0,
+              "torch_ans_b200: `symbols` must be a contiguous int32 tensor (", rows, ", ", width,
+              "), 16-byte aligned, on the device of `codes`");
+  check_rc(tans_kv4_from_symbols(symbols.data_ptr<int32_t>(), codes.data_ptr<uint8_t>(), codes.size(0),
+                                 (int)codes.size(2), (int)codes.size(3), (int)codes.size(4) * 2,
+                                 page_ids.data_ptr<int64_t>(), n, kv4_status(dev), cur_stream()),
+           "kv4 from symbols");
+  after_op(dev);
+}
+
 int64_t device_status(std::optional<int64_t> device, bool reset) {
   const int64_t d = device.has_value() ? *device : (int64_t)c10::cuda::current_device();
   Tensor& w = status_word(at::Device(at::kCUDA, (c10::DeviceIndex)d));
@@ -864,6 +1058,21 @@ PYBIND11_MODULE(_C, m) {
         "Pop streams of different lengths; returns the flat int32 symbols (row_starts[-1] of them).");
   m.def("rans32_pop_ragged", &rans_pop_ragged<1>, TANS_RAGGED_POP_ARGS);
   m.def("rans32_16_pop_ragged", &rans_pop_ragged<2>, TANS_RAGGED_POP_ARGS);
+  m.def("kv4_append", &kv4_append, py::arg("codes"), py::arg("params"), py::arg("k"), py::arg("v"), py::arg("slots"),
+        py::arg("q") = py::none(), py::arg("positions") = py::none(), py::arg("rotation") = py::none(),
+        py::arg("interleaved") = false,
+        "Quantise keys and values (tokens, kv_heads, head_dim) to 4 bits into their cache slots, keys rotated to their "
+        "positions first; returns the rotated queries when `q` is given.");
+  m.def("kv4_gather", &kv4_gather, py::arg("codes"), py::arg("params"), py::arg("slots"), py::arg("dtype"),
+        "The keys and values that the cache rows in `slots` stand for (zeros for negative slots).");
+  m.def("kv4_attend", &kv4_attend, py::arg("q"), py::arg("codes"), py::arg("params"), py::arg("pages"),
+        py::arg("lengths"), py::arg("q_starts") = py::none(), py::arg("max_queries") = py::none(),
+        py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("lse") = py::none(),
+        "Attention of packed queries over a 4-bit paged cache: one token, a few or whole prompts for each sequence.");
+  m.def("kv4_to_symbols", &kv4_to_symbols, py::arg("codes"), py::arg("page_ids"), py::arg("by_channel") = false,
+        "Cache pages as coder streams: (symbols, indexes), one row for each page, side and head.");
+  m.def("kv4_from_symbols", &kv4_from_symbols, py::arg("symbols"), py::arg("codes"), py::arg("page_ids"),
+        "Write decoded symbols back into cache pages.");
   m.def("copy_columns", &copy_columns, py::arg("dst"), py::arg("dst_col"), py::arg("src"), py::arg("src_col"),
         py::arg("ncols"), py::arg("cuda_stream"),
         "Pitched asynchronous copy of a column block between 2-D tensors (pinned host and/or device).");

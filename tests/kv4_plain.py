@@ -48,11 +48,12 @@ def values(codes, params):
 
 
 def attend(q, codes, params, pages, lengths, q_starts, scale, causal=True):
-    """(out, lse, bound) in 64 bits; lengths and q_starts are lists.  bound: see attend_bound."""
+    """(out, lse, bound, score_bound) in 64 bits; lengths and q_starts are lists.  The bounds: see attend_bounds."""
     heads, dim, kv, page = q.shape[1], q.shape[2], codes.shape[2], codes.shape[3]
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     lse = torch.full(q.shape[:2], float("-inf"), dtype=torch.float64, device=q.device)
     bound = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    score_bound = torch.zeros(q.shape[:2], dtype=torch.float64, device=q.device)
     for b, m in enumerate(lengths):
         lo, hi = q_starts[b], q_starts[b + 1]
         n = hi - lo
@@ -72,20 +73,23 @@ def attend(q, codes, params, pages, lengths, q_starts, scale, causal=True):
         s = s.masked_fill(~seen[:, None, None], float("-inf"))
         out[lo:hi] = torch.einsum("ikgj,kjd->ikgd", torch.nan_to_num(torch.softmax(s, -1)), held[1]).flatten(1, 2)
         lse[lo:hi] = torch.logsumexp(s, -1).flatten(1, 2)
-        bound[lo:hi] = attend_bound(qb, held, scale).flatten(1, 2)[..., None]
-    return out, lse, bound
+        of_out, of_score = attend_bounds(qb, held, scale)
+        bound[lo:hi], score_bound[lo:hi] = of_out.flatten(1, 2)[..., None], of_score.flatten(1, 2)
+    return out, lse, bound, score_bound
 
 
-def attend_bound(qb, held, scale):
-    """How far an output may be from the 64-bit one before its own rounding, for each query and head.
+def attend_bounds(qb, held, scale):
+    """How far an output and a score may be from the 64-bit ones before the output's own rounding, for each query and head.
 
     A weight may carry half a unit of float16 (2^-11 relative at most) and a value too (2^-11 of the largest): 2^-10 of
     the largest value together.  A score may be off by the rounding of its factors to float16 (2^-11 of the sum of
-    |q||k| that it adds up) and by the float sums and the hardware's 2^x (2^-18 of it, plus 2^-20); an error e of the scores changes weights
-    by a factor of at most exp(2 e), the result by about 2 e of the largest value."""
+    |q||k| that it adds up) and by the float sums and the hardware's 2^x (2^-18 of it, plus 2^-20); an error e of the
+    scores changes the log of their sum by e, weights by a factor of at most exp(2 e), the result by about 2 e of the
+    largest value."""
     top = held[1].abs().amax((1, 2))  # [kv]
     size = torch.einsum("ikgd,kd->ikg", qb.abs(), held[0].abs().amax(1)) * abs(scale)
-    return top[:, None] * (2.0 ** -10 + 2 * (size * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -20))
+    score = size * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -20
+    return top[:, None] * (2.0 ** -10 + 2 * score), score
 
 
 def pool(pages, kv, page, dim, seed=0, device="cuda"):

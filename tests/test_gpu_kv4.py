@@ -3,7 +3,7 @@
 Tolerances.  A stored row: scale and offset are bfloat16 roundings of values computed in float, so they are within one
 bfloat16 unit (2^-7 relative) of the 64-bit ones; a value is then within half a step of the row, plus what the two
 roundings cut off at the ends (15 steps x 2^-8 and 2^-8 of the smallest value), plus the float rounding of the rotation
-(2^-22 of the row's largest).  Attention: kv4_plain.attend_bound, plus the output's own rounding."""
+(2^-22 of the row's largest).  Attention: kv4_plain.attend_bounds, plus the output's own rounding."""
 import pytest
 import torch
 
@@ -134,15 +134,15 @@ def run_attend(C, lengths, counts, heads, kv, dim, page, dtype, causal=True, see
     out = C.kv4_attend(q, codes, params, pages, torch.tensor(lengths, **i32),
                        q_starts=None if counts == [1] * len(counts) and how == "packed" else torch.tensor(starts, **i32),
                        max_queries=max_queries, causal=causal, scale=scale, lse=lse)
-    ref, ref_lse, bound = P.attend(q, codes, params, pages, lengths, starts, dim ** -0.5 if scale is None else scale, causal)
+    ref, ref_lse, bound, score_bound = P.attend(q, codes, params, pages, lengths, starts, dim ** -0.5 if scale is None else scale, causal)
     assert out.shape == q.shape and out.dtype == dtype
     err = (out.double() - ref).abs()
-    assert (err <= bound + ref.abs() * P.U[dtype] * 1.01 + 2.0 ** -24).all(), (err / bound.clamp(min=1e-30)).max()
+    least = 2.0 ** -24 if dtype == FP else 0.0  # float16's smallest step
+    assert (err <= bound + ref.abs() * P.U[dtype] * 1.01 + least).all(), (err / bound.clamp(min=1e-30)).max()
     none = torch.isinf(ref_lse)
     assert torch.equal(torch.isinf(lse) & (lse < 0), none)
     if (~none).any():
-        # the scores' own part of the bound: bound / top / 2
-        assert ((lse.double() - ref_lse)[~none].abs() <= (bound[..., 0] * 64 + ref_lse.abs() * 2.0 ** -20)[~none]).all()
+        assert ((lse.double() - ref_lse)[~none].abs() <= (score_bound + ref_lse.abs() * 2.0 ** -20)[~none]).all()
     assert out[none].eq(0).all()
     assert C.device_status() == 0
     return out
@@ -257,7 +257,7 @@ def test_attend_flags_bad_pages_lengths_and_starts(C, count):
     bad[1, 2], bad[1, 5] = total, -7  # hidden, and flagged
     out = C.kv4_attend(q, codes, params, bad, ln, q_starts=st)
     assert C.device_status() == 1
-    ref, _, bound = P.attend(q, codes, params, bad, lengths, starts, 128 ** -0.5)
+    ref, _, bound, _ = P.attend(q, codes, params, bad, lengths, starts, 128 ** -0.5)
     assert ((out.double() - ref).abs() <= bound + ref.abs() * P.U[BF] * 1.01).all()
     assert torch.equal(out[:count], good[:count])
     out = C.kv4_attend(q, codes, params, pages, torch.tensor([100, -5], **i32), q_starts=st)

@@ -1,0 +1,117 @@
+// kv4_attend.cuh -- what the attention kernels over the 4-bit cache share.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "kv4.cuh"
+
+namespace tans {
+namespace kv4 {
+
+struct AttendArgs {
+  Pool pool;
+  const void* q;
+  int64_t q_ts, q_hs;  // strides of a token and a head, in elements
+  int64_t total_queries;
+  int q_heads, group;  // query heads; those that share a key/value head
+  const int32_t* pages;
+  int64_t batch, max_pages;
+  const int32_t* lengths;
+  const int32_t* q_starts;
+  float scale_log2;  // the score's factor times log2(e): softmax is taken in powers of two
+  int causal;
+  int vec;  // rows of q start on 16 bytes
+  void* out;
+  float* lse;
+  uint32_t* status;
+};
+
+// One sequence: its tokens, its queries (first and number).
+struct Sequence {
+  int length, start, count;
+};
+
+__device__ __forceinline__ void flag(uint32_t* status, uint32_t bit) {
+  if (status) atomicOr(status, bit);
+}
+
+__device__ __forceinline__ Sequence sequence(const AttendArgs& a, int64_t b, bool report) {
+  Sequence s;
+  if (a.q_starts) {
+    const int lo = a.q_starts[b], hi = a.q_starts[b + 1];
+    const bool ok = lo >= 0 && hi >= lo && hi <= a.total_queries;
+    if (!ok && report) flag(a.status, TANS_DEV_BAD_VALUE);
+    s.start = ok ? lo : 0;
+    s.count = ok ? hi - lo : 0;
+  } else {
+    s.start = (int)b;
+    s.count = 1;
+  }
+  const int length = a.lengths[b];
+  const int64_t most = a.max_pages * a.pool.page_size;
+  s.length = length < 0 ? 0 : (length > most ? (int)most : length);
+  if (s.length != length && report) flag(a.status, TANS_DEV_BAD_VALUE);
+  return s;
+}
+
+// Queries before the first start and after the last belong to no sequence: zeros, shared by all
+// threads of the grid.
+template <typename T>
+__device__ __forceinline__ void zero_unowned(const AttendArgs& a, int dim, int64_t thread, int64_t threads) {
+  if (!a.q_starts) return;
+  const int64_t first = max(0, min((int)a.total_queries, a.q_starts[0]));
+  const int64_t last = max((int)first, min((int)a.total_queries, a.q_starts[a.batch]));
+  const int64_t heads = a.q_heads, unowned = (first + a.total_queries - last) * heads;
+  if (unowned == 0) return;
+  for (int64_t e = thread; e < unowned * dim; e += threads) {
+    const int64_t row = e / dim, at = row < first * heads ? row : row + (last - first) * heads;
+    static_cast<T*>(a.out)[at * dim + e % dim] = Half2<T>::round(0.0f);
+    if (a.lse && e % dim == 0) a.lse[at] = -INFINITY;
+  }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 2^x for a whole number x in -126 .. 127
+__device__ __forceinline__ float pow2(int x) { return __int_as_float((x + 127) << 23); }
+
+// Where the parts of a row tile that several blocks share are joined.  Blocks take equal, contiguous
+// shares of all (sequence, row tile, head, token) work, so a tile's blocks are neighbours c0 .. c1.
+// Each leaves its sums in one of its two places (1: the tile starts in this block, 0: it started
+// before), and the last of them to arrive joins them, in the order of the blocks whatever the order
+// of arrival, so results repeat.  Over kFan blocks join in two levels.
+//
+// A place of arrival is a 64-bit word: the launch's number above 16 bits of count.  A word of another
+// launch (or of memory that was never written) counts as none, and the last arrival leaves 0, which
+// is no launch's number: the workspace needs no clearing, and a captured launch can be replayed.
+constexpr int kFan = 24;
+
+struct Join {
+  float* parts;       // [blocks][2][rows][dim]
+  float2* stats;      // [blocks][2][rows]: maximum (a power of two's exponent) and sum
+  unsigned long long* arrivals;  // [2 levels][blocks][2]
+  unsigned long long launch;     // the launch's number << 16
+  int blocks;
+};
+
+__device__ __forceinline__ bool arrive(unsigned long long* word, unsigned long long launch, int expected) {
+  unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
+  for (;;) {  // each failed try means that another block's arrival went in: at most `expected` rounds
+    unsigned long long next = (seen >> 16) == (launch >> 16) ? seen + 1 : launch + 1;
+    const bool last = (int)(next & 0xffff) == expected;
+    if (last) next = 0;
+    const unsigned long long was = atomicCAS(word, seen, next);
+    if (was == seen) return last;
+    seen = was;
+  }
+}
+
+int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* workspace, cudaStream_t s);
+size_t attend_rows_workspace(int head_dim, int64_t max_rows);
+
+}  // namespace kv4
+}  // namespace tans

@@ -1,0 +1,649 @@
+// kv4_attend_rows.cu -- attention over the 4-bit cache when few queries share a key/value head (one
+// token of a sequence, or a few drafted ones): bound by the bytes of the cache, so the work is split
+// over the tokens and a code costs as few instructions as the tensor cores' operands allow.
+//
+// A warp takes 32 tokens at a time for up to 8 (or 16) query rows of one key/value head.  Both
+// products are mma.sync.m16n8k16 with the cache as the 16-row operand, so 8 columns of rows cost no
+// more than one: S^T = K Q^T (16 tokens x 16 channels) and O^T = V^T P^T (16 channels x 16 tokens).
+// Codes become float16 by masking alone: the bits of c in the low four bits of a half are the
+// subnormal c * 2^-24, in the next four c * 2^-20; the tensor cores take subnormals exactly, and the
+// powers of two go into the queries (keys) and the result (values).  That is 5 instructions for 8
+// codes of a key word (four masks, one shift), and 12 for 16 codes of two tokens' value words (two
+// byte permutes pair the tokens of a channel first).
+//
+// With a row's (s, o): q.k = s (q.c) + o sum(q), so scales and offsets never touch the codes: the
+// score takes two products and one sum, and the value's scale goes into the weight,
+//   sum p v = 2^E (sum w c - 7.5 sum w) + sum p (o + 7.5 s),  w = float16(p s 2^-E),
+// with E a running power of two over the largest s.  The 7.5 centres the codes (sum w is one more
+// row of ones in the second product), so a weight's rounding to float16 (2^-11) weighs on the code's
+// distance from the middle, not on the code: about half the error.  The sums of the softmax, the
+// offsets and all accumulators are float.  A query row is brought under 2^14 by a power of two and
+// rounded to float16, which loses nothing that bfloat16 or float16 holds above 2^-24 of the row's
+// largest.
+//
+// The running maximum follows the scores only when one passes it by over 8 (a weight under 2^9 still
+// fits float16), so most steps compare and go on.
+#include "kv4_attend.cuh"
+#include "launch.cuh"
+#include "rans_host.h"
+
+#include <algorithm>
+#include <atomic>
+
+namespace tans {
+namespace kv4 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStep = 32;   // tokens a warp takes at a time
+constexpr int kStages = 3;  // steps in flight for each warp, the one in use among them
+constexpr float kSlack = 8.0f;
+
+// A step of a warp in shared memory: 32 key rows, 32 value rows, 32 + 32 parameters.
+template <int D>
+struct Stage {
+  static constexpr int ROW = D / 2, CHUNKS = D / 32;  // bytes, 16-byte chunks of a row
+  static constexpr int K = 0, V = kStep * ROW, KP = 2 * kStep * ROW, VP = KP + kStep * 4, BYTES = VP + kStep * 4;
+
+  // Where a 16-byte chunk of a token's row lies.  Key rows are read by lane 4 g + t as the t-th
+  // quarter of row token(g), value rows as the g-th eighth of rows t + 4 j; the order of rows and
+  // chunks puts the lanes of one access on different banks for both.
+  static __device__ __forceinline__ int place(int token, int chunk) {
+    if constexpr (D == 64) return (token ^ (((token >> 2) & 1) << 1)) * ROW + chunk * 16;
+    else if constexpr (D == 128) return (token ^ ((token >> 2) & 1)) * ROW + ((chunk ^ (token & 2)) * 16);
+    else return token * ROW + ((chunk ^ (((token & 3) << 1) | ((token >> 2) & 1))) * 16);
+  }
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;  // nothing is read for 0 bytes: the place is filled with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+
+struct RowsArgs {
+  AttendArgs a;
+  Join join;
+};
+
+template <int D, int NT>
+struct Shared {
+  static constexpr int R = 8 * NT;
+  static constexpr int RING = kWarps * kStages * Stage<D>::BYTES;
+  static constexpr int MERGE = kWarps * R * (D + 1) * 4 + kWarps * R * 8;  // the ring's memory again
+  static constexpr int BYTES = RING > MERGE ? RING : MERGE;
+};
+
+// Blocks of a row tile (or of one group of them) joined: threads take channels, rows in turn.
+template <int D, int R>
+__device__ __forceinline__ void join_parts(const Join& j, int first_place, int first, int count, int step,
+                                           float (&acc)[R * D / (kWarps * 32)], float2 (&stat)[R * D / (kWarps * 32)]) {
+  // element e of this thread: row = (threadIdx.x + e * threads) / D
+  constexpr int N = R * D / (kWarps * 32);
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int at = threadIdx.x + e * kWarps * 32, row = at / D;
+    float m = -INFINITY;
+    for (int i = 0; i < count; ++i) {
+      const int c = i == 0 ? first_place : ((first + i * step) * 2);
+      m = fmaxf(m, __ldcg(&j.stats[(int64_t)c * R + row]).x);
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, v = 0.0f;
+    for (int i = 0; i < count; ++i) {
+      const int c = i == 0 ? first_place : ((first + i * step) * 2);
+      const float2 s = __ldcg(&j.stats[(int64_t)c * R + row]);
+      const float w = ex2(s.x - base);
+      sum += w * s.y;
+      v += w * __ldcg(&j.parts[((int64_t)c * R) * D + at]);
+    }
+    acc[e] = v;
+    stat[e] = make_float2(m, sum);
+  }
+}
+
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs p) {
+  const AttendArgs& a = p.a;
+  using S = Stage<D>;
+  constexpr int R = 8 * NT, KW = D / 32, VW = D / 64;  // rows of a tile; words of a key / value row's share of a lane
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int64_t sh_scan[kWarps];
+  __shared__ int64_t sh_found[2];
+  __shared__ int sh_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int heads = a.pool.kv_heads, page_size = a.pool.page_size;
+
+  zero_unowned<T>(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32);
+
+  // ---- this block's share of the steps of all sequences, row tiles and heads
+  auto tiles_of = [&](const Sequence& s) { return (s.count * (int64_t)a.group + R - 1) / R; };
+  auto steps_of = [&](const Sequence& s) { return max(1, (s.length + kStep - 1) / kStep); };
+  auto units_of = [&](const Sequence& s) { return tiles_of(s) * heads * steps_of(s); };
+  auto block_scan = [&](int64_t v, int64_t& total) {  // sum of v over the threads before this one
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh_scan[warp] = x;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh_scan[w];
+      total += sh_scan[w];
+    }
+    return before + x - v;
+  };
+  int64_t all = 0;
+  for (int64_t b = 0; b < a.batch; b += kWarps * 32) {
+    int64_t sum;
+    const int64_t mine = b + threadIdx.x < a.batch ? units_of(sequence(a, b + threadIdx.x, blockIdx.x == 0)) : 0;
+    block_scan(mine, sum);
+    all += sum;
+  }
+  const int64_t share = max((all + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)kWarps);
+  int64_t u = blockIdx.x * share;
+  const int64_t u_end = min(all, u + share);
+  if (u >= u_end) return;
+  for (int64_t b = 0, done = 0; b < a.batch; b += kWarps * 32) {
+    int64_t sum;
+    const int64_t mine = b + threadIdx.x < a.batch ? units_of(sequence(a, b + threadIdx.x, false)) : 0;
+    const int64_t before = done + block_scan(mine, sum);
+    if (u >= before && u < before + mine) {
+      sh_found[0] = b + threadIdx.x;
+      sh_found[1] = before;
+    }
+    done += sum;
+    if (u < done) break;
+  }
+  __syncthreads();
+  int64_t b = sh_found[0], b_first = sh_found[1];
+  Sequence seq = sequence(a, b, false);
+
+  uint8_t* ring = smem + warp * kStages * S::BYTES;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+
+  while (u < u_end) {
+    while (u >= b_first + units_of(seq)) {  // sequences without queries have no units
+      b_first += units_of(seq);
+      ++b;
+      seq = sequence(a, b, false);
+    }
+    const int steps = steps_of(seq);
+    const int64_t item = (u - b_first) / steps;
+    const int step0 = (int)(u - b_first - item * steps);
+    const int step1 = (int)min((int64_t)steps, step0 + (u_end - u));
+    const int64_t item_first = b_first + item * steps;
+    const int head = (int)(item % heads);
+    const int row0 = (int)(item / heads) * R, rows = min(R, seq.count * a.group - row0);
+
+    // ---- the queries: column g of each 8 is row g; a lane's channels are the t-th quarter
+    uint32_t qf[NT][KW][4];
+    float fac[NT][2], shift[NT][2];  // of columns 2t and 2t + 1: score = (acc * s) * fac + o * shift
+    int seen[NT][2];                 // tokens that the columns' queries see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + n * 8 + g;
+      const bool live = n * 8 + g < rows;
+      float x[D / 4];
+      if (live) {
+        const int i = r / a.group, h = head * a.group + (r - i * a.group);
+        const T* src = static_cast<const T*>(a.q) + (seq.start + i) * a.q_ts + h * a.q_hs + t * (D / 4);
+        if (a.vec) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + c * 8);
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = Half2<T>::unpack(v[e]);
+              x[c * 8 + 2 * e] = f.x;
+              x[c * 8 + 2 * e + 1] = f.y;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 4; ++c) x[c] = Half2<T>::load(src + c);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 4; ++c) x[c] = 0.0f;
+      }
+      float top = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 4; ++c) {
+        top = fmaxf(top, fabsf(x[c]));
+        sum += x[c];
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+      const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));  // the row times 2^e is under 2^14
+      const float up = pow2(e), up16 = pow2(e - 4);
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        // the codes of a word pair up as (0, 4), (1, 5), (2, 6), (3, 7); the odd ones come 16 times too large
+        qf[n][w][0] = Half2<__half>::pack(x[8 * w] * up, x[8 * w + 4] * up);
+        qf[n][w][1] = Half2<__half>::pack(x[8 * w + 1] * up16, x[8 * w + 5] * up16);
+        qf[n][w][2] = Half2<__half>::pack(x[8 * w + 2] * up, x[8 * w + 6] * up);
+        qf[n][w][3] = Half2<__half>::pack(x[8 * w + 3] * up16, x[8 * w + 7] * up16);
+      }
+      const float f = a.scale_log2 * pow2(24 - e), sh = a.scale_log2 * sum;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        fac[n][c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
+        shift[n][c] = __shfl_sync(0xffffffffu, sh, (2 * t + c) * 4);
+        const int col = n * 8 + 2 * t + c;
+        const int i = (row0 + col) / a.group;
+        seen[n][c] = col >= rows ? 0 : (a.causal ? min(seq.length, seq.length - seq.count + i + 1) : seq.length);
+      }
+    }
+    // every live row sees the tokens under `full`
+    const int full = a.causal ? seq.length - seq.count + row0 / a.group + 1 : seq.length;
+
+    float m[NT][2], l[NT][2], off[NT][2], acc[NT][D / 16][4], ones[NT][4];
+    int E = 27;  // exponent field of the weights' common factor
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[n][c] = -INFINITY;
+        l[n][c] = off[n][c] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.0f;
+      ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0.0f;
+    }
+
+    // ---- steps of this warp: step0 + warp, + kWarps, ...; kStages - 1 of them on their way
+    uint32_t known = 0;  // two bits a step in flight, the newest lowest: the group's page is one of the pool
+    auto fetch = [&](int step, int slot) {
+      uint32_t bits = 0;
+      if (step < step1) {
+        const uint32_t base = ring_at + slot * S::BYTES;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int token = step * kStep + h * 16;
+          int page = 0, first = 0;
+          bool there = token < seq.length;
+          if (there) {
+            const int at = token / page_size;
+            first = token - at * page_size;
+            page = a.pages[b * a.max_pages + at];
+            if (page < 0 || page >= a.pool.num_pages) {
+              there = false;
+              page = 0;
+              if (lane == 0) flag(a.status, TANS_DEV_BAD_INDEX);
+            }
+          }
+          if (there) bits |= 1u << h;
+          const int64_t kr = a.pool.row(page, 0, head) + first, vr = a.pool.row(page, 1, head) + first;
+          const uint8_t* ks = a.pool.codes + kr * S::ROW;
+          const uint8_t* vs = a.pool.codes + vr * S::ROW;
+#pragma unroll
+          for (int c0 = 0; c0 < 16 * S::CHUNKS; c0 += 32) {
+            const int c = c0 + lane, at = S::place(h * 16 + c / S::CHUNKS, c % S::CHUNKS);
+            cp16(base + S::K + at, ks + (there ? c * 16 : 0), there);
+            cp16(base + S::V + at, vs + (there ? c * 16 : 0), there);
+          }
+          if (lane < 8) {
+            const bool key = lane < 4;
+            const uint32_t* src = a.pool.params + (key ? kr : vr) + (there ? (lane & 3) * 4 : 0);
+            cp16(base + (key ? S::KP : S::VP) + h * 64 + (lane & 3) * 16, src, there);
+          }
+        }
+      }
+      known = known << 2 | bits;
+      cp_commit();
+    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(step0 + warp + i * kWarps, i);
+
+    int slot = 0;
+    for (int step = step0 + warp; step < step1; step += kWarps) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      const uint32_t bits = known >> (2 * (kStages - 2));
+      fetch(step + (kStages - 1) * kWarps, slot == 0 ? kStages - 1 : slot - 1);
+      const uint8_t* st = ring + slot * S::BYTES;
+      slot = slot == kStages - 1 ? 0 : slot + 1;
+
+      // scores: rows g and g + 8 of the product are tokens tok and tok + 8
+      const int tok = (g >> 1) + (g & 1) * 4;
+      float s[2][NT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t k0[KW], k1[KW];
+#pragma unroll
+        for (int w = 0; w < KW; w += (KW >= 4 ? 4 : 2)) {
+          if constexpr (KW >= 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(st + S::K + S::place(h * 16 + tok, t * (KW / 4) + w / 4));
+            const uint4 y = *reinterpret_cast<const uint4*>(st + S::K + S::place(h * 16 + tok + 8, t * (KW / 4) + w / 4));
+            k0[w] = x.x; k0[w + 1] = x.y; k0[w + 2] = x.z; k0[w + 3] = x.w;
+            k1[w] = y.x; k1[w + 1] = y.y; k1[w + 2] = y.z; k1[w + 3] = y.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(st + S::K + S::place(h * 16 + tok, t >> 1) + (t & 1) * 8);
+            const uint2 y = *reinterpret_cast<const uint2*>(st + S::K + S::place(h * 16 + tok + 8, t >> 1) + (t & 1) * 8);
+            k0[w] = x.x; k0[w + 1] = x.y;
+            k1[w] = y.x; k1[w + 1] = y.y;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const uint32_t x = k0[w], y = k1[w], x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma(s[h][n], x & kLow, y & kLow, x & kHigh, y & kHigh, qf[n][w][0], qf[n][w][1]);
+            mma(s[h][n], x8 & kLow, y8 & kLow, x8 & kHigh, y8 & kHigh, qf[n][w][2], qf[n][w][3]);
+          }
+        }
+      }
+      // a token's parameters; those past the end may hold anything
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(st + S::KP);
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(st + S::VP);
+      float sv[4], ov[4];
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+      const bool plain = (bits & 3u) == 3u && (step + 1) * kStep <= full;
+      uint32_t big = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = tok + 8 * j;  // j: group j / 2, row g or g + 8
+        const uint32_t kw = kp[at], vw = vp[at];
+        const float sk = scale_of(kw), ok = offset_of(kw);
+        sv[j] = scale_of(vw);
+        ov[j] = fmaf(7.5f, sv[j], offset_of(vw));
+        const uint32_t field = (vw << 16) & 0x7f800000u;
+        const bool in = plain || (step * kStep + at < seq.length && (bits >> (j >> 1) & 1));
+        big = max(big, in && field != 0x7f800000u ? field : 0u);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float& x = s[j >> 1][n][(j & 1) * 2 + c];
+            x = fmaf(x * sk, fac[n][c], ok * shift[n][c]);
+            if (!plain && !(step * kStep + at < seen[n][c] && (bits >> (j >> 1) & 1))) x = -INFINITY;
+            top[n][c] = fmaxf(top[n][c], x);
+          }
+      }
+      // ---- follow the maximum and the largest scale
+      bool move = (int)(big >> 23) > E;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) move |= top[n][0] > m[n][0] + kSlack || top[n][1] > m[n][1] + kSlack;
+      if (__any_sync(0xffffffffu, move)) {
+        const int field = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
+        const int now = min(252, max(E, field));
+        const float fall = E > now - 126 ? pow2(E - now) : 0.0f;
+        E = now;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = top[n][c];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            const float next = x > m[n][c] + kSlack ? x : m[n][c];
+            const float keep = m[n][c] == -INFINITY ? 1.0f : ex2(m[n][c] - next);
+            m[n][c] = next;
+            l[n][c] *= keep;
+            off[n][c] *= keep;
+            const float both = keep * fall;
+            ones[n][c] *= both;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              acc[n][i][c] *= both;
+              acc[n][i][c + 2] *= both;
+            }
+          }
+      }
+      const float inv = pow2(126 - E);  // 2^-(E - 126): weights are under 2 * 2^8
+      // ---- weights and sums
+      uint32_t wf[2][NT][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float sc = sv[j] * inv;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float w[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = s[j >> 1][n][(j & 1) * 2 + c];
+            const float e = ex2(x - (m[n][c] == -INFINITY ? 0.0f : m[n][c]));
+            l[n][c] += e;
+            w[c] = e * sc;
+            float d = e * ov[j];
+            if (!plain && x == -INFINITY) w[c] = d = 0.0f;  // a hidden token's parameters do not count
+            off[n][c] += d;
+          }
+          wf[j >> 1][n][j & 1] = transpose8(Half2<__half>::pack(w[0], w[1]));
+        }
+      }
+      // ---- values
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[4][VW];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int token = h * 16 + t + 4 * j;
+          if constexpr (VW == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(st + S::V + S::place(token, g));
+            v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
+          } else if constexpr (VW == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(st + S::V + S::place(token, g >> 1) + (g & 1) * 8);
+            v[j][0] = x.x; v[j][1] = x.y;
+          } else {
+            v[j][0] = *reinterpret_cast<const uint32_t*>(st + S::V + S::place(token, g >> 2) + (g & 3) * 4);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // channels 4 half .. 4 half + 3 of the word: tokens (t, t + 4) and (t + 8, t + 12)
+            uint32_t x = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
+            uint32_t y = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma(acc[n][w * 4 + half * 2 + q], x & kLow, x & kHigh, y & kLow, y & kHigh, wf[h][n][0], wf[h][n][1]);
+              x >>= 8;
+              y >>= 8;
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          mma(ones[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, wf[h][n][0], wf[h][n][1]);
+      }
+    }
+    cp_wait<0>();
+
+    // ---- join the warps: sums in shared memory (the rings' memory)
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);                                     // [warp][row][D + 1]
+    float2* sm = reinterpret_cast<float2*>(smem + kWarps * R * (D + 1) * 4);        // [warp][row]
+    const float back = pow2(min(127, E - 126));  // the weights' common factor (E <= 252)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
+          off[n][c] += __shfl_xor_sync(0xffffffffu, off[n][c], o);
+        }
+        const int row = n * 8 + 2 * t + c;
+        float* dst = so + (warp * R + row) * (D + 1) + g * (D / 8);
+        const float mid = 7.5f * ones[n][c];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          dst[2 * i] = fmaf(fmaf(acc[n][i][c], 16777216.0f, -mid), back, off[n][c]);
+          dst[2 * i + 1] = fmaf(fmaf(acc[n][i][c + 2], 1048576.0f, -mid), back, off[n][c]);
+        }
+        if (g == 0) sm[warp * R + row] = make_float2(m[n][c], l[n][c]);
+      }
+    __syncthreads();
+
+    constexpr int N = R * D / (kWarps * 32);
+    float val[N];
+    float2 stat[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int at = threadIdx.x + e * kWarps * 32, row = at / D, d = at % D;
+      float top = -INFINITY;
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * R + row].x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, v = 0.0f;
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 x = sm[w * R + row];
+        const float k = ex2(x.x - base);
+        sum += k * x.y;
+        v += k * so[(w * R + row) * (D + 1) + d];
+      }
+      val[e] = v;
+      stat[e] = make_float2(top, sum);
+    }
+    __syncthreads();  // the rings may be filled again
+
+    // ---- whole here, or joined with the other blocks' parts
+    bool whole = step0 == 0 && step1 == steps;
+    if (!whole) {
+      const Join& j = p.join;
+      const int c0 = (int)(item_first / share), c1 = (int)((item_first + steps - 1) / share);
+      auto leave = [&](int place) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const int at = threadIdx.x + e * kWarps * 32;
+          j.parts[(int64_t)place * R * D + at] = val[e];
+          if (at % D == 0) j.stats[(int64_t)place * R + at / D] = stat[e];
+        }
+        __threadfence();
+        __syncthreads();
+      };
+      auto last_of = [&](int level, int place, int expected) {
+        if (threadIdx.x == 0) sh_last = arrive(j.arrivals + (level * j.blocks * 2 + place), j.launch, expected);
+        __syncthreads();
+        const bool last = sh_last != 0;
+        __syncthreads();
+        __threadfence();
+        return last;
+      };
+      const int me = blockIdx.x;
+      leave(me * 2 + (me == c0));
+      const int f0 = max(c0, me / kFan * kFan), f1 = min(c1, me / kFan * kFan + kFan - 1);  // this block's group
+      const int place = f0 * 2 + (f0 == c0);
+      whole = f1 == f0 || last_of(0, place, f1 - f0 + 1);
+      if (whole && f1 > f0) join_parts<D, R>(j, place, f0, f1 - f0 + 1, 1, val, stat);
+      if (whole && (f0 != c0 || f1 != c1)) {  // the groups
+        if (f1 > f0) leave(place);
+        const int first_group = c0 / kFan, groups = c1 / kFan - first_group + 1;
+        whole = last_of(1, c0 * 2 + 1, groups);
+        if (whole) join_parts<D, R>(j, c0 * 2 + 1, first_group * kFan, groups, kFan, val, stat);
+      }
+    }
+    if (whole) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int at = threadIdx.x + e * kWarps * 32, row = at / D, d = at % D;
+        if (row < rows) {
+          const int r = row0 + row, i = r / a.group, h = head * a.group + (r - i * a.group);
+          const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
+          const float sum = stat[e].y;
+          static_cast<T*>(a.out)[o * D + d] = Half2<T>::round(sum == 0.0f ? 0.0f : val[e] / sum);
+          if (a.lse && d == 0)
+            a.lse[o] = sum == 0.0f ? -INFINITY : (stat[e].x + log2f(sum)) * 0.69314718055994531f;
+        }
+      }
+    }
+    u += step1 - step0;
+  }
+}
+
+template <int D, int NT, typename T>
+int blocks_per_sm() {
+  static int known = 0;
+  if (known == 0) {
+    int n = 0;
+    constexpr int bytes = Shared<D, NT>::BYTES;
+    if (cudaFuncSetAttribute(attend_rows_kernel<D, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_rows_kernel<D, NT, T>, kWarps * 32, bytes) !=
+            cudaSuccess)
+      return 0;
+    known = n;
+  }
+  return known;
+}
+
+constexpr int kMostBlocks = 6 * 160;  // blocks that the workspace has places for
+
+template <int D, int NT, typename T>
+int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
+  const int per_sm = blocks_per_sm<D, NT, T>();
+  if (per_sm < 1) return TANS_E_CUDA;
+  const int blocks = std::min(kMostBlocks, per_sm * sm_count());
+  static std::atomic<unsigned long long> launches{0};
+  constexpr int R = 8 * NT;
+  Join j;
+  j.parts = static_cast<float*>(workspace);
+  j.stats = reinterpret_cast<float2*>(j.parts + (int64_t)kMostBlocks * 2 * R * D);
+  j.arrivals = reinterpret_cast<unsigned long long*>(j.stats + (int64_t)kMostBlocks * 2 * R);
+  j.launch = (launches.fetch_add(1, std::memory_order_relaxed) + 1) << 16;
+  j.blocks = kMostBlocks;
+  attend_rows_kernel<D, NT, T><<<blocks, kWarps * 32, Shared<D, NT>::BYTES, s>>>(RowsArgs{a, j});
+  note_launch();
+  return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
+}
+
+}  // namespace
+
+size_t attend_rows_workspace(int head_dim, int64_t max_rows) {
+  const int64_t rows = max_rows <= 8 ? 8 : 16;
+  return align_up((size_t)kMostBlocks * 2 * (rows * head_dim * 4 + rows * 8 + 2 * 8));
+}
+
+int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* workspace, cudaStream_t s) {
+  auto by_rows = [&](auto d, auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int D = decltype(d)::value;
+    return max_rows <= 8 ? launch<D, 1, T>(a, workspace, s) : launch<D, 2, T>(a, workspace, s);
+  };
+  auto by_dim = [&](auto* t) {
+    return a.pool.head_dim == 64    ? by_rows(std::integral_constant<int, 64>{}, t)
+           : a.pool.head_dim == 128 ? by_rows(std::integral_constant<int, 128>{}, t)
+                                    : by_rows(std::integral_constant<int, 256>{}, t);
+  };
+  return dtype == TANS_BF16 ? by_dim(static_cast<__nv_bfloat16*>(nullptr)) : by_dim(static_cast<__half*>(nullptr));
+}
+
+}  // namespace kv4
+}  // namespace tans

@@ -29,7 +29,8 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
       q_heads % kv_heads != 0 || max_queries < 0)
     return TANS_E_INVALID_ARGUMENT;
   if (total_queries == 0) return TANS_OK;
-  if (!q || !out || (batch > 0 && (!lengths || (max_pages > 0 && !pages))) || (!q_starts && batch != total_queries))
+  if (!q || !out || (batch > 0 && (!lengths || (max_pages > 0 && !pages))) || (!q_starts && batch != total_queries) ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return TANS_E_INVALID_ARGUMENT;
   // token and query numbers are 32-bit in the kernels, with room for a tile past the end
   if (total_queries > (1 << 30) / q_heads || batch > (1 << 30) || max_pages * page_size > (1 << 30) ||

@@ -38,6 +38,8 @@ constexpr int kWarps = 4;
 constexpr int kStep = 32;   // tokens a warp takes at a time
 constexpr int kStages = 3;  // steps in flight for each warp, the one in use among them
 constexpr float kSlack = 8.0f;
+constexpr int kMostBlocks = 6 * 160;  // blocks that the workspace has places for
+constexpr int kMostParts = kMostBlocks / kFan > kFan ? kMostBlocks / kFan : kFan;  // that are joined at a time
 
 // A step of a warp in shared memory: 32 key rows, 32 value rows, 32 + 32 parameters.
 template <int D>
@@ -88,35 +90,61 @@ template <int D, int NT>
 struct Shared {
   static constexpr int R = 8 * NT;
   static constexpr int RING = kWarps * kStages * Stage<D>::BYTES;
-  static constexpr int MERGE = kWarps * R * (D + 1) * 4 + kWarps * R * 8;  // the ring's memory again
+  static constexpr int MERGE = kWarps * R * (D + 4) * 4;  // the ring's memory again
   static constexpr int BYTES = RING > MERGE ? RING : MERGE;
 };
 
-// Blocks of a row tile (or of one group of them) joined: threads take channels, rows in turn.
+// Sums of a row tile as they leave a block: a thread holds 4 channels of each of N rows.
+template <int D, int R>
+struct Sums {
+  static constexpr int N = R * D / 4 / (kWarps * 32);
+  float4 v[N];
+  static __device__ __forceinline__ int at(int e) { return threadIdx.x + e * kWarps * 32; }  // in fours
+  static __device__ __forceinline__ int row(int e) { return at(e) / (D / 4); }
+  static __device__ __forceinline__ int channel(int e) { return at(e) % (D / 4) * 4; }
+};
+
+// The parts of a row tile (or of one group of its blocks) joined: the first at first_place, the
+// others `step` blocks apart after `first`.  The statistics go through shared memory, so the loads of
+// the parts do not wait for one another.
 template <int D, int R>
 __device__ __forceinline__ void join_parts(const Join& j, int first_place, int first, int count, int step,
-                                           float (&acc)[R * D / (kWarps * 32)], float2 (&stat)[R * D / (kWarps * 32)]) {
-  // element e of this thread: row = (threadIdx.x + e * threads) / D
-  constexpr int N = R * D / (kWarps * 32);
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const int at = threadIdx.x + e * kWarps * 32, row = at / D;
-    float m = -INFINITY;
-    for (int i = 0; i < count; ++i) {
-      const int c = i == 0 ? first_place : ((first + i * step) * 2);
-      m = fmaxf(m, __ldcg(&j.stats[(int64_t)c * R + row]).x);
-    }
+                                           float (*weight)[R], float2* total, Sums<D, R>& sums) {
+  auto place = [&](int i) { return i == 0 ? first_place : (first + i * step) * 2; };
+  for (int x = threadIdx.x; x < count * R; x += kWarps * 32) {
+    const int i = x / R, row = x - i * R;
+    const float2 st = __ldcg(&j.stats[(int64_t)place(i) * R + row]);
+    weight[i][row] = st.x;
+    weight[count + i][row] = st.y;
+  }
+  __syncthreads();
+  if (threadIdx.x < R) {
+    const int row = threadIdx.x;
+    float m = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < count; ++i) m = fmaxf(m, weight[i][row]);
     const float base = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f, v = 0.0f;
     for (int i = 0; i < count; ++i) {
-      const int c = i == 0 ? first_place : ((first + i * step) * 2);
-      const float2 s = __ldcg(&j.stats[(int64_t)c * R + row]);
-      const float w = ex2(s.x - base);
-      sum += w * s.y;
-      v += w * __ldcg(&j.parts[((int64_t)c * R) * D + at]);
+      const float w = ex2(weight[i][row] - base);
+      weight[i][row] = w;
+      sum += w * weight[count + i][row];
     }
-    acc[e] = v;
-    stat[e] = make_float2(m, sum);
+    total[row] = make_float2(m, sum);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < Sums<D, R>::N; ++e) sums.v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const float4* part = reinterpret_cast<const float4*>(j.parts + (int64_t)place(i) * R * D);
+#pragma unroll
+    for (int e = 0; e < Sums<D, R>::N; ++e) {
+      const float4 x = __ldcg(part + Sums<D, R>::at(e));
+      const float w = weight[i][Sums<D, R>::row(e)];
+      sums.v[e].x += w * x.x;
+      sums.v[e].y += w * x.y;
+      sums.v[e].z += w * x.z;
+      sums.v[e].w += w * x.w;
+    }
   }
 }
 
@@ -128,11 +156,12 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t sh_scan[kWarps];
   __shared__ int64_t sh_found[2];
+  __shared__ Sequence sh_sequence;
   __shared__ int sh_last;
+  __shared__ float2 sh_stat[kWarps * R], sh_total[R];
+  __shared__ float sh_weight[2 * kMostParts][R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int heads = a.pool.kv_heads, page_size = a.pool.page_size;
-
-  zero_unowned<T>(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32);
 
   // ---- this block's share of the steps of all sequences, row tiles and heads
   auto tiles_of = [&](const Sequence& s) { return (s.count * (int64_t)a.group + R - 1) / R; };
@@ -156,31 +185,43 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
     }
     return before + x - v;
   };
-  int64_t all = 0;
+  int64_t all = 0, mine, before;
+  Sequence seq{0, 0, 0};
   for (int64_t b = 0; b < a.batch; b += kWarps * 32) {
     int64_t sum;
-    const int64_t mine = b + threadIdx.x < a.batch ? units_of(sequence(a, b + threadIdx.x, blockIdx.x == 0)) : 0;
-    block_scan(mine, sum);
+    if (b + threadIdx.x < a.batch) seq = sequence(a, b + threadIdx.x, blockIdx.x == 0);
+    mine = b + threadIdx.x < a.batch ? units_of(seq) : 0;
+    before = all + block_scan(mine, sum);
     all += sum;
   }
   const int64_t share = max((all + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)kWarps);
   int64_t u = blockIdx.x * share;
   const int64_t u_end = min(all, u + share);
-  if (u >= u_end) return;
+  auto zero_rest = [&]() {
+    zero_unowned<T>(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32);
+  };
+  if (u >= u_end) {
+    zero_rest();
+    return;
+  }
   for (int64_t b = 0, done = 0; b < a.batch; b += kWarps * 32) {
-    int64_t sum;
-    const int64_t mine = b + threadIdx.x < a.batch ? units_of(sequence(a, b + threadIdx.x, false)) : 0;
-    const int64_t before = done + block_scan(mine, sum);
+    if (a.batch > kWarps * 32) {  // more sequences than threads: once more from the start
+      int64_t sum;
+      if (b + threadIdx.x < a.batch) seq = sequence(a, b + threadIdx.x, false);
+      mine = b + threadIdx.x < a.batch ? units_of(seq) : 0;
+      before = done + block_scan(mine, sum);
+      done += sum;
+    }
     if (u >= before && u < before + mine) {
       sh_found[0] = b + threadIdx.x;
       sh_found[1] = before;
+      sh_sequence = seq;
     }
-    done += sum;
     if (u < done) break;
   }
   __syncthreads();
   int64_t b = sh_found[0], b_first = sh_found[1];
-  Sequence seq = sequence(a, b, false);
+  seq = sh_sequence;
 
   uint8_t* ring = smem + warp * kStages * S::BYTES;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
@@ -489,8 +530,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
 
     // ---- join the warps: sums in shared memory (the rings' memory)
     __syncthreads();
-    float* so = reinterpret_cast<float*>(smem);                                     // [warp][row][D + 1]
-    float2* sm = reinterpret_cast<float2*>(smem + kWarps * R * (D + 1) * 4);        // [warp][row]
+    float* so = reinterpret_cast<float*>(smem);  // [warp][row][D + 4]
     const float back = pow2(min(127, E - 126));  // the weights' common factor (E <= 252)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -502,35 +542,41 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
           off[n][c] += __shfl_xor_sync(0xffffffffu, off[n][c], o);
         }
         const int row = n * 8 + 2 * t + c;
-        float* dst = so + (warp * R + row) * (D + 1) + g * (D / 8);
+        float* dst = so + (warp * R + row) * (D + 4) + g * (D / 8);
         const float mid = 7.5f * ones[n][c];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           dst[2 * i] = fmaf(fmaf(acc[n][i][c], 16777216.0f, -mid), back, off[n][c]);
           dst[2 * i + 1] = fmaf(fmaf(acc[n][i][c + 2], 1048576.0f, -mid), back, off[n][c]);
         }
-        if (g == 0) sm[warp * R + row] = make_float2(m[n][c], l[n][c]);
+        if (g == 0) sh_stat[warp * R + row] = make_float2(m[n][c], l[n][c]);
       }
     __syncthreads();
 
-    constexpr int N = R * D / (kWarps * 32);
-    float val[N];
-    float2 stat[N];
+    using Part = Sums<D, R>;
+    Part sums;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int at = threadIdx.x + e * kWarps * 32, row = at / D, d = at % D;
+    for (int e = 0; e < Part::N; ++e) {
+      const int row = Part::row(e), d = Part::channel(e);
       float top = -INFINITY;
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * R + row].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh_stat[w * R + row].x);
       const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, v = 0.0f;
+      float sum = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float2 x = sm[w * R + row];
-        const float k = ex2(x.x - base);
-        sum += k * x.y;
-        v += k * so[(w * R + row) * (D + 1) + d];
+        const float2 st = sh_stat[w * R + row];
+        const float k = ex2(st.x - base);
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * R + row) * (D + 4) + d);
+        sum += k * st.y;
+        v.x += k * x.x;
+        v.y += k * x.y;
+        v.z += k * x.z;
+        v.w += k * x.w;
       }
-      val[e] = v;
-      stat[e] = make_float2(top, sum);
+      sums.v[e] = v;
+      if (d == 0) sh_total[row] = make_float2(top, sum);
     }
     __syncthreads();  // the rings may be filled again
 
@@ -541,11 +587,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
       const int c0 = (int)(item_first / share), c1 = (int)((item_first + steps - 1) / share);
       auto leave = [&](int place) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int at = threadIdx.x + e * kWarps * 32;
-          j.parts[(int64_t)place * R * D + at] = val[e];
-          if (at % D == 0) j.stats[(int64_t)place * R + at / D] = stat[e];
-        }
+        for (int e = 0; e < Part::N; ++e)
+          reinterpret_cast<float4*>(j.parts + (int64_t)place * R * D)[Part::at(e)] = sums.v[e];
+        if (threadIdx.x < R) j.stats[(int64_t)place * R + threadIdx.x] = sh_total[threadIdx.x];
         __threadfence();
         __syncthreads();
       };
@@ -562,30 +606,35 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
       const int f0 = max(c0, me / kFan * kFan), f1 = min(c1, me / kFan * kFan + kFan - 1);  // this block's group
       const int place = f0 * 2 + (f0 == c0);
       whole = f1 == f0 || last_of(0, place, f1 - f0 + 1);
-      if (whole && f1 > f0) join_parts<D, R>(j, place, f0, f1 - f0 + 1, 1, val, stat);
+      if (whole && f1 > f0) join_parts<D, R>(j, place, f0, f1 - f0 + 1, 1, sh_weight, sh_total, sums);
       if (whole && (f0 != c0 || f1 != c1)) {  // the groups
         if (f1 > f0) leave(place);
         const int first_group = c0 / kFan, groups = c1 / kFan - first_group + 1;
         whole = last_of(1, c0 * 2 + 1, groups);
-        if (whole) join_parts<D, R>(j, c0 * 2 + 1, first_group * kFan, groups, kFan, val, stat);
+        if (whole) join_parts<D, R>(j, c0 * 2 + 1, first_group * kFan, groups, kFan, sh_weight, sh_total, sums);
       }
     }
     if (whole) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int at = threadIdx.x + e * kWarps * 32, row = at / D, d = at % D;
+      for (int e = 0; e < Part::N; ++e) {
+        const int row = Part::row(e), d = Part::channel(e);
         if (row < rows) {
           const int r = row0 + row, i = r / a.group, h = head * a.group + (r - i * a.group);
           const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
-          const float sum = stat[e].y;
-          static_cast<T*>(a.out)[o * D + d] = Half2<T>::round(sum == 0.0f ? 0.0f : val[e] / sum);
-          if (a.lse && d == 0)
-            a.lse[o] = sum == 0.0f ? -INFINITY : (stat[e].x + log2f(sum)) * 0.69314718055994531f;
+          const float2 st = sh_total[row];
+          const float k = st.y == 0.0f ? 0.0f : 1.0f / st.y;
+          uint2 w;
+          w.x = Half2<T>::pack(sums.v[e].x * k, sums.v[e].y * k);
+          w.y = Half2<T>::pack(sums.v[e].z * k, sums.v[e].w * k);
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + o * D + d) = w;
+          if (a.lse && d == 0) a.lse[o] = st.y == 0.0f ? -INFINITY : (st.x + log2f(st.y)) * 0.69314718055994531f;
         }
       }
+      __syncthreads();  // the totals may be written again
     }
     u += step1 - step0;
   }
+  zero_rest();
 }
 
 template <int D, int NT, typename T>
@@ -603,8 +652,6 @@ int blocks_per_sm() {
   }
   return known;
 }
-
-constexpr int kMostBlocks = 6 * 160;  // blocks that the workspace has places for
 
 template <int D, int NT, typename T>
 int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {

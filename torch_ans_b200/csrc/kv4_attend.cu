@@ -33,14 +33,15 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
       ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return TANS_E_INVALID_ARGUMENT;
   // token and query numbers are 32-bit in the kernels, with room for a tile past the end
-  if (total_queries > (1 << 30) / q_heads || batch > (1 << 30) || max_pages * page_size > (1 << 30) ||
+  if (total_queries > (1 << 30) / q_heads || batch > (1 << 30) || max_pages > (1 << 30) / page_size ||
       num_pages > 0x7fffffff)
     return TANS_E_TOO_LARGE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(cuda_stream);
   const int group = q_heads / kv_heads;
   const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   const AttendArgs a{Pool{codes, static_cast<const uint32_t*>(params), num_pages, kv_heads, page_size, head_dim},
-                     q, q_token_stride, q_head_stride, total_queries, q_heads, group, pages, batch, max_pages, lengths,
+                     q, q_token_stride, q_head_stride, total_queries, q_heads,
+                     Divider::of(group), Divider::of(kv_heads), Divider::of(page_size), pages, batch, max_pages, lengths,
                      q_starts, scale * 1.4426950408889634f, causal, vec, out, lse, dev_status};
   const int64_t most = std::min(max_queries, total_queries);
   const size_t need = tans_kv4_attend_workspace_size(total_queries, q_heads, kv_heads, head_dim, batch, max_pages,

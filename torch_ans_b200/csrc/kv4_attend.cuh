@@ -8,12 +8,25 @@
 namespace tans {
 namespace kv4 {
 
+// Division by a number that the host knows: floor(n / d) for n < 2^31 is mulhi(2 n, m) >> l with
+// l = ceil(log2 d), m = ceil(2^(31 + l) / d) (Granlund and Montgomery).
+struct Divider {
+  uint32_t d, m, l;
+  static Divider of(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, (uint32_t)(((1ull << (31 + l)) + d - 1) / d), l};
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(__umulhi(2u * (uint32_t)n, m) >> l); }
+};
+
 struct AttendArgs {
   Pool pool;
   const void* q;
   int64_t q_ts, q_hs;  // strides of a token and a head, in elements
   int64_t total_queries;
-  int q_heads, group;  // query heads; those that share a key/value head
+  int q_heads;
+  Divider group, kv_heads, page_size;  // query heads that share a key/value head; the pool's
   const int32_t* pages;
   int64_t batch, max_pages;
   const int32_t* lengths;

@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace tans {
 namespace kv4 {
@@ -38,6 +39,7 @@ constexpr int kWarps = 4;
 constexpr int kStep = 32;   // tokens a warp takes at a time
 constexpr int kStages = 3;  // steps in flight for each warp, the one in use among them
 constexpr float kSlack = 8.0f;
+constexpr int kItemSteps = 8;  // what an item's start and end cost a block, in steps
 constexpr int kMostBlocks = 6 * 160;  // blocks that the workspace has places for
 constexpr int kMostParts = kMostBlocks / kFan > kFan ? kMostBlocks / kFan : kFan;  // that are joined at a time
 
@@ -45,6 +47,7 @@ constexpr int kMostParts = kMostBlocks / kFan > kFan ? kMostBlocks / kFan : kFan
 template <int D>
 struct Stage {
   static constexpr int ROW = D / 2, CHUNKS = D / 32;  // bytes, 16-byte chunks of a row
+  static constexpr int COPIES = CHUNKS / 2;           // chunks of 16 rows for each lane
   static constexpr int K = 0, V = kStep * ROW, KP = 2 * kStep * ROW, VP = KP + kStep * 4, BYTES = VP + kStep * 4;
 
   // Where a 16-byte chunk of a token's row lies.  Key rows are read by lane 4 g + t as the t-th
@@ -149,13 +152,13 @@ __device__ __forceinline__ void join_parts(const Join& j, int first_place, int f
 }
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs p) {
+__global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_rows_kernel(const RowsArgs p) {
   const AttendArgs& a = p.a;
   using S = Stage<D>;
   constexpr int R = 8 * NT, KW = D / 32, VW = D / 64;  // rows of a tile; words of a key / value row's share of a lane
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t sh_scan[kWarps];
-  __shared__ int64_t sh_found[2];
+  __shared__ int sh_found[2];
   __shared__ Sequence sh_sequence;
   __shared__ int sh_last;
   __shared__ float2 sh_stat[kWarps * R], sh_total[R];
@@ -163,10 +166,12 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int heads = a.pool.kv_heads, page_size = a.pool.page_size;
 
-  // ---- this block's share of the steps of all sequences, row tiles and heads
-  auto tiles_of = [&](const Sequence& s) { return (s.count * (int64_t)a.group + R - 1) / R; };
-  auto steps_of = [&](const Sequence& s) { return max(1, (s.length + kStep - 1) / kStep); };
-  auto units_of = [&](const Sequence& s) { return tiles_of(s) * heads * steps_of(s); };
+  // ---- this block's share of the work: the steps of every sequence, row tile and head, and a few
+  // for each of these items' start and end
+  auto steps_of = [&](const Sequence& s) { return (s.length + kStep - 1) / kStep + kItemSteps; };
+  auto units_of = [&](const Sequence& s) {
+    return (int64_t)((s.count * a.group.d + R - 1) / R) * heads * steps_of(s);
+  };
   auto block_scan = [&](int64_t v, int64_t& total) {  // sum of v over the threads before this one
     int64_t x = v;
 #pragma unroll
@@ -179,66 +184,163 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
     __syncthreads();
     int64_t before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += sh_scan[w];
       total += sh_scan[w];
     }
     return before + x - v;
   };
+  const int batch = (int)a.batch;
   int64_t all = 0, mine, before;
   Sequence seq{0, 0, 0};
-  for (int64_t b = 0; b < a.batch; b += kWarps * 32) {
+  for (int b = 0; b < batch; b += kWarps * 32) {
     int64_t sum;
-    if (b + threadIdx.x < a.batch) seq = sequence(a, b + threadIdx.x, blockIdx.x == 0);
-    mine = b + threadIdx.x < a.batch ? units_of(seq) : 0;
+    mine = 0;
+    if (b + (int)threadIdx.x < batch) {
+      seq = sequence(a, b + threadIdx.x, blockIdx.x == 0);
+      mine = units_of(seq);
+    }
     before = all + block_scan(mine, sum);
     all += sum;
   }
-  const int64_t share = max((all + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)kWarps);
-  int64_t u = blockIdx.x * share;
-  const int64_t u_end = min(all, u + share);
+  if (all > 0x7f000000) {  // starts that cross one another: no call within memory has so much work
+    if (blockIdx.x == 0 && threadIdx.x == 0) flag(a.status, TANS_DEV_BAD_VALUE);
+    return;
+  }
+  const int share = max(((int)all + (int)gridDim.x - 1) / (int)gridDim.x, kWarps + kItemSteps);
   auto zero_rest = [&]() {
     zero_unowned<T>(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32);
   };
-  if (u >= u_end) {
+  if ((int64_t)blockIdx.x * share >= all) {
     zero_rest();
     return;
   }
-  for (int64_t b = 0, done = 0; b < a.batch; b += kWarps * 32) {
-    if (a.batch > kWarps * 32) {  // more sequences than threads: once more from the start
+  int u = blockIdx.x * share;
+  const int u_end = (int)min(all, (int64_t)u + share);
+  int64_t done = 0;
+  for (int b = 0; b < batch; b += kWarps * 32) {
+    if (batch > kWarps * 32) {  // more sequences than threads: once more from the start
       int64_t sum;
-      if (b + threadIdx.x < a.batch) seq = sequence(a, b + threadIdx.x, false);
-      mine = b + threadIdx.x < a.batch ? units_of(seq) : 0;
+      mine = 0;
+      if (b + (int)threadIdx.x < batch) {
+        seq = sequence(a, b + threadIdx.x, false);
+        mine = units_of(seq);
+      }
       before = done + block_scan(mine, sum);
       done += sum;
     }
     if (u >= before && u < before + mine) {
       sh_found[0] = b + threadIdx.x;
-      sh_found[1] = before;
+      sh_found[1] = (int)before;
       sh_sequence = seq;
     }
     if (u < done) break;
   }
   __syncthreads();
-  int64_t b = sh_found[0], b_first = sh_found[1];
+  int b = sh_found[0], b_first = sh_found[1];
   seq = sh_sequence;
 
   uint8_t* ring = smem + warp * kStages * S::BYTES;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
 
+  // this lane's places in a step: what it copies (of the first 16 tokens), and what it reads.  Tokens
+  // 8 and 16 further lie 8 and 16 rows further.
+  int copy_at[S::COPIES], key_at[KW > 4 ? 2 : 1], value_at[2];
+#pragma unroll
+  for (int i = 0; i < S::COPIES; ++i) copy_at[i] = S::place((i * 32 + lane) / S::CHUNKS, (i * 32 + lane) % S::CHUNKS);
+  const int tok = (g >> 1) + (g & 1) * 4;  // rows g and g + 8 of the score's product are tokens tok and tok + 8
+  if constexpr (KW >= 4) {
+#pragma unroll
+    for (int i = 0; i < KW / 4; ++i) key_at[i] = S::K + S::place(tok, t * (KW / 4) + i);
+  } else {
+    key_at[0] = S::K + S::place(tok, t >> 1) + (t & 1) * 8;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {  // tokens t + 4 j, t + 8 + 4 j
+    const int c = VW == 4 ? g : (VW == 2 ? g >> 1 : g >> 2), in = VW == 4 ? 0 : (VW == 2 ? (g & 1) * 8 : (g & 3) * 4);
+    value_at[j] = S::V + S::place(t + 4 * j, c) + in;
+  }
+
   while (u < u_end) {
     while (u >= b_first + units_of(seq)) {  // sequences without queries have no units
-      b_first += units_of(seq);
+      b_first += (int)units_of(seq);
       ++b;
       seq = sequence(a, b, false);
     }
-    const int steps = steps_of(seq);
-    const int64_t item = (u - b_first) / steps;
-    const int step0 = (int)(u - b_first - item * steps);
-    const int step1 = (int)min((int64_t)steps, step0 + (u_end - u));
-    const int64_t item_first = b_first + item * steps;
-    const int head = (int)(item % heads);
-    const int row0 = (int)(item / heads) * R, rows = min(R, seq.count * a.group - row0);
+    const int units = steps_of(seq), steps = units - kItemSteps;
+    const int item = (u - b_first) / units, item_first = b_first + item * units;
+    const int unit1 = min(units, u_end - item_first);
+    const int step0 = max(0, u - item_first - kItemSteps), step1 = max(0, unit1 - kItemSteps);
+    const int tile = a.kv_heads.div(item), head = item - tile * heads;
+    const int row0 = tile * R, rows = min(R, seq.count * (int)a.group.d - row0);
+
+    // ---- steps of this warp: step0 + warp, + kWarps, ...; kStages - 1 of them on their way
+    uint32_t known = 0;  // two bits a step in flight, the newest lowest: the group's page is one of the pool
+    const int64_t side_bytes = (int64_t)heads * page_size * S::ROW;  // from a page's keys to its values, and half a page
+    const uint8_t* head_codes = a.pool.codes + (int64_t)head * page_size * S::ROW + lane * 16;
+    const uint32_t* head_params =
+        a.pool.params + ((lane >= 4 ? heads : 0) + (int64_t)head) * page_size + (lane & 3) * 4;
+    const int32_t* table = a.pages + (int64_t)b * a.max_pages;
+    // the page and the place in it of the next step's first token; from step to step they grow alike
+    int next = step0 + warp;
+    int at = a.page_size.div(next * kStep), first = next * kStep - at * page_size;
+    const int more_pages = a.page_size.div(kWarps * kStep), more_tokens = kWarps * kStep - more_pages * page_size;
+    // its pages are looked up a step ahead; -1: no tokens there
+    int page[2];
+    auto look_up = [&]() {
+      int h_at = at, h_first = first;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        page[h] = -1;
+        if (next < step1 && next * kStep + h * 16 < seq.length) page[h] = __ldg(table + h_at);
+        h_first += 16;
+        if (h_first == page_size) {
+          h_first = 0;
+          ++h_at;
+        }
+      }
+    };
+    look_up();
+    auto fetch = [&](int slot) {
+      uint32_t bits = 0;
+      if (next < step1) {
+        const uint32_t base = ring_at + slot * S::BYTES;
+        int h_first = first;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool there = (unsigned)page[h] < (unsigned)a.pool.num_pages;
+          if (!there && lane == 0 && next * kStep + h * 16 < seq.length) flag(a.status, TANS_DEV_BAD_INDEX);
+          if (there) bits |= 1u << h;
+          const int64_t pg = there ? page[h] : 0;
+          const uint8_t* ks = head_codes + pg * (2 * side_bytes) + h_first * S::ROW;
+          const uint8_t* vs = ks + side_bytes;
+#pragma unroll
+          for (int i = 0; i < S::COPIES; ++i) {
+            cp16(base + S::K + h * 16 * S::ROW + copy_at[i], ks + i * 512, there);
+            cp16(base + S::V + h * 16 * S::ROW + copy_at[i], vs + i * 512, there);
+          }
+          if (lane < 8)  // keys' parameters, then values'
+            cp16(base + S::KP + (lane >> 2) * kStep * 4 + h * 64 + (lane & 3) * 16,
+                 head_params + pg * (2 * (int64_t)heads * page_size) + h_first, there);
+          h_first += 16;
+          if (h_first == page_size) h_first = 0;
+        }
+        next += kWarps;
+        at += more_pages;
+        first += more_tokens;
+        if (first >= page_size) {
+          first -= page_size;
+          ++at;
+        }
+        look_up();
+      }
+      known = known << 2 | bits;
+      cp_commit();
+    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(i);
 
     // ---- the queries: column g of each 8 is row g; a lane's channels are the t-th quarter
     uint32_t qf[NT][KW][4];
@@ -250,7 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
       const bool live = n * 8 + g < rows;
       float x[D / 4];
       if (live) {
-        const int i = r / a.group, h = head * a.group + (r - i * a.group);
+        const int i = a.group.div(r), h = head * a.group.d + (r - i * a.group.d);
         const T* src = static_cast<const T*>(a.q) + (seq.start + i) * a.q_ts + h * a.q_hs + t * (D / 4);
         if (a.vec) {
 #pragma unroll
@@ -299,12 +401,12 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
         fac[n][c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
         shift[n][c] = __shfl_sync(0xffffffffu, sh, (2 * t + c) * 4);
         const int col = n * 8 + 2 * t + c;
-        const int i = (row0 + col) / a.group;
+        const int i = a.group.div(row0 + col);
         seen[n][c] = col >= rows ? 0 : (a.causal ? min(seq.length, seq.length - seq.count + i + 1) : seq.length);
       }
     }
     // every live row sees the tokens under `full`
-    const int full = a.causal ? seq.length - seq.count + row0 / a.group + 1 : seq.length;
+    const int full = a.causal ? seq.length - seq.count + a.group.div(row0) + 1 : seq.length;
 
     float m[NT][2], l[NT][2], off[NT][2], acc[NT][D / 16][4], ones[NT][4];
     int E = 27;  // exponent field of the weights' common factor
@@ -320,79 +422,32 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
       ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0.0f;
     }
 
-    // ---- steps of this warp: step0 + warp, + kWarps, ...; kStages - 1 of them on their way
-    uint32_t known = 0;  // two bits a step in flight, the newest lowest: the group's page is one of the pool
-    auto fetch = [&](int step, int slot) {
-      uint32_t bits = 0;
-      if (step < step1) {
-        const uint32_t base = ring_at + slot * S::BYTES;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int token = step * kStep + h * 16;
-          int page = 0, first = 0;
-          bool there = token < seq.length;
-          if (there) {
-            const int at = token / page_size;
-            first = token - at * page_size;
-            page = a.pages[b * a.max_pages + at];
-            if (page < 0 || page >= a.pool.num_pages) {
-              there = false;
-              page = 0;
-              if (lane == 0) flag(a.status, TANS_DEV_BAD_INDEX);
-            }
-          }
-          if (there) bits |= 1u << h;
-          const int64_t kr = a.pool.row(page, 0, head) + first, vr = a.pool.row(page, 1, head) + first;
-          const uint8_t* ks = a.pool.codes + kr * S::ROW;
-          const uint8_t* vs = a.pool.codes + vr * S::ROW;
-#pragma unroll
-          for (int c0 = 0; c0 < 16 * S::CHUNKS; c0 += 32) {
-            const int c = c0 + lane, at = S::place(h * 16 + c / S::CHUNKS, c % S::CHUNKS);
-            cp16(base + S::K + at, ks + (there ? c * 16 : 0), there);
-            cp16(base + S::V + at, vs + (there ? c * 16 : 0), there);
-          }
-          if (lane < 8) {
-            const bool key = lane < 4;
-            const uint32_t* src = a.pool.params + (key ? kr : vr) + (there ? (lane & 3) * 4 : 0);
-            cp16(base + (key ? S::KP : S::VP) + h * 64 + (lane & 3) * 16, src, there);
-          }
-        }
-      }
-      known = known << 2 | bits;
-      cp_commit();
-    };
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(step0 + warp + i * kWarps, i);
-
     int slot = 0;
     for (int step = step0 + warp; step < step1; step += kWarps) {
       cp_wait<kStages - 2>();
       __syncwarp();
       const uint32_t bits = known >> (2 * (kStages - 2));
-      fetch(step + (kStages - 1) * kWarps, slot == 0 ? kStages - 1 : slot - 1);
+      fetch(slot == 0 ? kStages - 1 : slot - 1);
       const uint8_t* st = ring + slot * S::BYTES;
       slot = slot == kStages - 1 ? 0 : slot + 1;
 
-      // scores: rows g and g + 8 of the product are tokens tok and tok + 8
-      const int tok = (g >> 1) + (g & 1) * 4;
       float s[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t k0[KW], k1[KW];
+        if constexpr (KW >= 4) {
 #pragma unroll
-        for (int w = 0; w < KW; w += (KW >= 4 ? 4 : 2)) {
-          if constexpr (KW >= 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(st + S::K + S::place(h * 16 + tok, t * (KW / 4) + w / 4));
-            const uint4 y = *reinterpret_cast<const uint4*>(st + S::K + S::place(h * 16 + tok + 8, t * (KW / 4) + w / 4));
-            k0[w] = x.x; k0[w + 1] = x.y; k0[w + 2] = x.z; k0[w + 3] = x.w;
-            k1[w] = y.x; k1[w + 1] = y.y; k1[w + 2] = y.z; k1[w + 3] = y.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(st + S::K + S::place(h * 16 + tok, t >> 1) + (t & 1) * 8);
-            const uint2 y = *reinterpret_cast<const uint2*>(st + S::K + S::place(h * 16 + tok + 8, t >> 1) + (t & 1) * 8);
-            k0[w] = x.x; k0[w + 1] = x.y;
-            k1[w] = y.x; k1[w + 1] = y.y;
+          for (int i = 0; i < KW / 4; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(st + key_at[i] + h * 16 * S::ROW);
+            const uint4 y = *reinterpret_cast<const uint4*>(st + key_at[i] + (h * 16 + 8) * S::ROW);
+            k0[4 * i] = x.x; k0[4 * i + 1] = x.y; k0[4 * i + 2] = x.z; k0[4 * i + 3] = x.w;
+            k1[4 * i] = y.x; k1[4 * i + 1] = y.y; k1[4 * i + 2] = y.z; k1[4 * i + 3] = y.w;
           }
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(st + key_at[0] + h * 16 * S::ROW);
+          const uint2 y = *reinterpret_cast<const uint2*>(st + key_at[0] + (h * 16 + 8) * S::ROW);
+          k0[0] = x.x; k0[1] = x.y;
+          k1[0] = y.x; k1[1] = y.y;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.0f;
@@ -406,102 +461,112 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
           }
         }
       }
-      // a token's parameters; those past the end may hold anything
-      const uint32_t* kp = reinterpret_cast<const uint32_t*>(st + S::KP);
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>(st + S::VP);
-      float sv[4], ov[4];
-      float top[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-      const bool plain = (bits & 3u) == 3u && (step + 1) * kStep <= full;
-      uint32_t big = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = tok + 8 * j;  // j: group j / 2, row g or g + 8
-        const uint32_t kw = kp[at], vw = vp[at];
-        const float sk = scale_of(kw), ok = offset_of(kw);
-        sv[j] = scale_of(vw);
-        ov[j] = fmaf(7.5f, sv[j], offset_of(vw));
-        const uint32_t field = (vw << 16) & 0x7f800000u;
-        const bool in = plain || (step * kStep + at < seq.length && (bits >> (j >> 1) & 1));
-        big = max(big, in && field != 0x7f800000u ? field : 0u);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float& x = s[j >> 1][n][(j & 1) * 2 + c];
-            x = fmaf(x * sk, fac[n][c], ok * shift[n][c]);
-            if (!plain && !(step * kStep + at < seen[n][c] && (bits >> (j >> 1) & 1))) x = -INFINITY;
-            top[n][c] = fmaxf(top[n][c], x);
-          }
-      }
-      // ---- follow the maximum and the largest scale
-      bool move = (int)(big >> 23) > E;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) move |= top[n][0] > m[n][0] + kSlack || top[n][1] > m[n][1] + kSlack;
-      if (__any_sync(0xffffffffu, move)) {
-        const int field = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
-        const int now = min(252, max(E, field));
-        const float fall = E > now - 126 ? pow2(E - now) : 0.0f;
-        E = now;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float x = top[n][c];
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            const float next = x > m[n][c] + kSlack ? x : m[n][c];
-            const float keep = m[n][c] == -INFINITY ? 1.0f : ex2(m[n][c] - next);
-            m[n][c] = next;
-            l[n][c] *= keep;
-            off[n][c] *= keep;
-            const float both = keep * fall;
-            ones[n][c] *= both;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              acc[n][i][c] *= both;
-              acc[n][i][c + 2] *= both;
-            }
-          }
-      }
-      const float inv = pow2(126 - E);  // 2^-(E - 126): weights are under 2 * 2^8
-      // ---- weights and sums
+
+      // Scores to weights.  `masked` steps hold tokens past the end, of unknown pages or past a query:
+      // their scores are -inf and their parameters, which may be anything, count nowhere.
       uint32_t wf[2][NT][2];
+      auto weigh = [&](auto masked_) {
+        constexpr bool masked = decltype(masked_)::value;
+        const uint32_t* kp = reinterpret_cast<const uint32_t*>(st + S::KP) + tok;
+        const uint32_t* vp = reinterpret_cast<const uint32_t*>(st + S::VP) + tok;
+        float sv[4], ov[4], top[NT][2];
+        bool in[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float sc = sv[j] * inv;
+        for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+        uint32_t big = 0;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[2];
+        for (int j = 0; j < 4; ++j) {  // j: group j / 2, row g or g + 8
+          const uint32_t kw = kp[8 * j], vw = vp[8 * j];
+          const float sk = scale_of(kw), ok = offset_of(kw);
+          sv[j] = scale_of(vw);
+          ov[j] = fmaf(7.5f, sv[j], offset_of(vw));
+          const int token = step * kStep + tok + 8 * j;
+          in[j] = !masked || (token < seq.length && (bits >> (j >> 1) & 1));
+          const uint32_t field = (vw << 16) & 0x7f800000u;
+          big = max(big, in[j] && field != 0x7f800000u ? field : 0u);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float x = s[j >> 1][n][(j & 1) * 2 + c];
-            const float e = ex2(x - (m[n][c] == -INFINITY ? 0.0f : m[n][c]));
-            l[n][c] += e;
-            w[c] = e * sc;
-            float d = e * ov[j];
-            if (!plain && x == -INFINITY) w[c] = d = 0.0f;  // a hidden token's parameters do not count
-            off[n][c] += d;
-          }
-          wf[j >> 1][n][j & 1] = transpose8(Half2<__half>::pack(w[0], w[1]));
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float& x = s[j >> 1][n][(j & 1) * 2 + c];
+              x = fmaf(x * sk, fac[n][c], ok * shift[n][c]);
+              if (masked && !(in[j] && token < seen[n][c])) x = -INFINITY;
+              top[n][c] = fmaxf(top[n][c], x);
+            }
         }
-      }
+        // follow the maximum and the largest scale
+        bool move = (int)(big >> 23) > E;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) move |= top[n][0] > m[n][0] + kSlack || top[n][1] > m[n][1] + kSlack;
+        if (__any_sync(0xffffffffu, move)) {
+          const int field = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
+          const int now = min(252, max(E, field));
+          const float fall = E > now - 126 ? pow2(E - now) : 0.0f;
+          E = now;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = top[n][c];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+              const float top_now = x > m[n][c] + kSlack ? x : m[n][c];
+              const float keep = m[n][c] == -INFINITY ? 1.0f : ex2(m[n][c] - top_now);
+              m[n][c] = top_now;
+              l[n][c] *= keep;
+              off[n][c] *= keep;
+              const float both = keep * fall;
+              ones[n][c] *= both;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                acc[n][i][c] *= both;
+                acc[n][i][c + 2] *= both;
+              }
+            }
+        }
+        const float inv = pow2(126 - E);  // weights are under 2^8
+        float base[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) base[n][c] = m[n][c] == -INFINITY ? 0.0f : m[n][c];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float sc = sv[j] * inv;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float w[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float x = s[j >> 1][n][(j & 1) * 2 + c];
+              const float e = ex2(x - base[n][c]);
+              const bool hidden = masked && x == -INFINITY;
+              l[n][c] += e;
+              w[c] = hidden ? 0.0f : e * sc;
+              off[n][c] = hidden ? off[n][c] : fmaf(e, ov[j], off[n][c]);
+            }
+            wf[j >> 1][n][j & 1] = transpose8(Half2<__half>::pack(w[0], w[1]));
+          }
+        }
+      };
+      if ((bits & 3u) == 3u && (step + 1) * kStep <= full) weigh(std::false_type{});
+      else weigh(std::true_type{});
+
       // ---- values
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t v[4][VW];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int token = h * 16 + t + 4 * j;
+          const uint8_t* src = st + value_at[j & 1] + (h * 16 + (j & 2) * 4) * S::ROW;
           if constexpr (VW == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(st + S::V + S::place(token, g));
+            const uint4 x = *reinterpret_cast<const uint4*>(src);
             v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
           } else if constexpr (VW == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(st + S::V + S::place(token, g >> 1) + (g & 1) * 8);
+            const uint2 x = *reinterpret_cast<const uint2*>(src);
             v[j][0] = x.x; v[j][1] = x.y;
           } else {
-            v[j][0] = *reinterpret_cast<const uint32_t*>(st + S::V + S::place(token, g >> 2) + (g & 3) * 4);
+            v[j][0] = *reinterpret_cast<const uint32_t*>(src);
           }
         }
 #pragma unroll
@@ -581,10 +646,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
     __syncthreads();  // the rings may be filled again
 
     // ---- whole here, or joined with the other blocks' parts
-    bool whole = step0 == 0 && step1 == steps;
+    bool whole = u == item_first && unit1 == units;
     if (!whole) {
       const Join& j = p.join;
-      const int c0 = (int)(item_first / share), c1 = (int)((item_first + steps - 1) / share);
+      const int c0 = item_first / share, c1 = (item_first + units - 1) / share;
       auto leave = [&](int place) {
 #pragma unroll
         for (int e = 0; e < Part::N; ++e)
@@ -619,7 +684,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
       for (int e = 0; e < Part::N; ++e) {
         const int row = Part::row(e), d = Part::channel(e);
         if (row < rows) {
-          const int r = row0 + row, i = r / a.group, h = head * a.group + (r - i * a.group);
+          const int r = row0 + row, i = a.group.div(r), h = head * a.group.d + (r - i * a.group.d);
           const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
           const float2 st = sh_total[row];
           const float k = st.y == 0.0f ? 0.0f : 1.0f / st.y;
@@ -632,7 +697,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_rows_kernel(const RowsArgs
       }
       __syncthreads();  // the totals may be written again
     }
-    u += step1 - step0;
+    u = item_first + unit1;
   }
   zero_rest();
 }

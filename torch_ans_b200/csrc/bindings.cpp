@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <map>
 #include <tuple>
 #include <mutex>
 #include <unordered_map>
@@ -888,6 +889,32 @@ std::tuple<Tensor, Tensor> kv4_gather(const Tensor& codes, const Tensor& params,
   return {k, v};
 }
 
+// A workspace for the current stream.  Calls on one stream are ordered, so each stream keeps one (it
+// only grows); its counts are zero between calls.  A captured call gets one of its graph's own, which
+// the graph clears: a graph may be replayed on any stream.
+Tensor kv4_workspace(const at::Device& dev, int64_t bytes) {
+  const auto opt = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
+  const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  TORCH_CHECK(cudaStreamIsCapturing(stream.stream(), &capture) == cudaSuccess, "torch_ans_b200: no capture status");
+  static std::mutex mu;
+  static auto& kept = *new std::map<std::pair<int, cudaStream_t>, Tensor>();  // never freed: no CUDA calls at exit
+  const bool captured = capture != cudaStreamCaptureStatusNone;
+  Tensor ws;
+  if (!captured) {
+    std::lock_guard<std::mutex> g(mu);
+    auto it = kept.find({dev.index(), stream.stream()});
+    if (it != kept.end() && it->second.numel() >= bytes) return it->second;
+  }
+  ws = torch::empty({bytes}, opt);
+  ws.narrow(0, 0, TANS_KV4_ATTEND_COUNTS).zero_();
+  if (!captured) {
+    std::lock_guard<std::mutex> g(mu);
+    kept[{dev.index(), stream.stream()}] = ws;
+  }
+  return ws;
+}
+
 Tensor kv4_attend(const Tensor& q, const Tensor& codes, const Tensor& params, const Tensor& pages, const Tensor& lengths,
                   const std::optional<Tensor>& q_starts, std::optional<int64_t> max_queries, std::optional<double> scale,
                   bool causal, const std::optional<Tensor>& lse) {
@@ -918,7 +945,7 @@ Tensor kv4_attend(const Tensor& q, const Tensor& codes, const Tensor& params, co
   const size_t need = tans_kv4_attend_workspace_size(n, (int)heads, (int)p.kv_heads, (int)p.head_dim, batch,
                                                      pages.size(1), (int)p.page_size, most);
   Tensor ws;
-  if (need) ws = torch::empty({(int64_t)need}, torch::TensorOptions().dtype(torch::kUInt8).device(p.dev));
+  if (need) ws = kv4_workspace(p.dev, (int64_t)need);
   check_rc(tans_kv4_attend(q.data_ptr(), q.stride(0), q.stride(1), n, (int)heads, dtype, codes.data_ptr<uint8_t>(),
                            params.data_ptr(), p.num_pages, (int)p.kv_heads, (int)p.page_size, (int)p.head_dim,
                            pages.data_ptr<int32_t>(), batch, pages.size(1), lengths.data_ptr<int32_t>(),

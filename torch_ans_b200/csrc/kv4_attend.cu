@@ -7,6 +7,8 @@
 #include "kv4_attend.cuh"
 #include "rans_host.h"
 
+static_assert(tans::kv4::Join::kArrivalBytes == TANS_KV4_ATTEND_COUNTS, "the header names the size");
+
 extern "C" size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim,
                                                  int64_t batch, int64_t max_pages, int page_size, int64_t max_queries) {
   using namespace tans::kv4;
@@ -49,6 +51,10 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
   void* ws = workspace;
   if (!ws) {
     if (cudaMallocAsync(&ws, need, s) != cudaSuccess) return TANS_E_CUDA;
+    if (cudaMemsetAsync(ws, 0, Join::kArrivalBytes, s) != cudaSuccess) {
+      cudaFreeAsync(ws, s);
+      return TANS_E_CUDA;
+    }
   } else if (workspace_bytes < need) {
     return TANS_E_WORKSPACE;
   }

@@ -96,31 +96,33 @@ __device__ __forceinline__ float pow2(int x) { return __int_as_float((x + 127) <
 // shares of all (sequence, row tile, head, token) work, so a tile's blocks are neighbours c0 .. c1.
 // Each leaves its sums in one of its two places (1: the tile starts in this block, 0: it started
 // before), and the last of them to arrive joins them, in the order of the blocks whatever the order
-// of arrival, so results repeat.  Over kFan blocks join in two levels.
-//
-// A place of arrival is a 64-bit word: the launch's number above 16 bits of count.  A word of another
-// launch (or of memory that was never written) counts as none, and the last arrival leaves 0, which
-// is no launch's number: the workspace needs no clearing, and a captured launch can be replayed.
-constexpr int kFan = 24;
+// of arrival, so results repeat.  Over kFan blocks join in two levels.  The counts of arrivals are
+// zero between launches: the last arrival takes its count back.
+constexpr int kFan = 64;
+constexpr int kMostBlocks = 3 * 160;  // blocks that a workspace has places for
 
 struct Join {
-  float* parts;       // [blocks][2][rows][dim]
-  float2* stats;      // [blocks][2][rows]: maximum (a power of two's exponent) and sum
-  unsigned long long* arrivals;  // [2 levels][blocks][2]
-  unsigned long long launch;     // the launch's number << 16
-  int blocks;
+  int* arrivals;  // [2 levels][kMostBlocks][2]
+  float2* stats;  // [kMostBlocks][2][rows]: maximum (a power of two's exponent) and sum
+  float* parts;   // [kMostBlocks][2][rows][dim]
+
+  static size_t bytes(int64_t rows, int64_t dim) {
+    return kArrivalBytes + (size_t)kMostBlocks * 2 * rows * (8 + dim * 4);
+  }
+  static constexpr size_t kArrivalBytes = 2 * kMostBlocks * 2 * sizeof(int);
+  static Join in(void* workspace, int64_t rows) {
+    Join j;
+    j.arrivals = static_cast<int*>(workspace);
+    j.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + kArrivalBytes);
+    j.parts = reinterpret_cast<float*>(j.stats + kMostBlocks * 2 * rows);
+    return j;
+  }
 };
 
-__device__ __forceinline__ bool arrive(unsigned long long* word, unsigned long long launch, int expected) {
-  unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
-  for (;;) {  // each failed try means that another block's arrival went in: at most `expected` rounds
-    unsigned long long next = (seen >> 16) == (launch >> 16) ? seen + 1 : launch + 1;
-    const bool last = (int)(next & 0xffff) == expected;
-    if (last) next = 0;
-    const unsigned long long was = atomicCAS(word, seen, next);
-    if (was == seen) return last;
-    seen = was;
-  }
+__device__ __forceinline__ bool arrive(int* count, int expected) {
+  if (atomicAdd(count, 1) + 1 < expected) return false;
+  *count = 0;  // nobody else comes in this launch
+  return true;
 }
 
 int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* workspace, cudaStream_t s);

@@ -28,19 +28,17 @@
 #include "rans_host.h"
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace tans {
 namespace kv4 {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kStep = 32;   // tokens a warp takes at a time
 constexpr int kStages = 3;  // steps in flight for each warp, the one in use among them
 constexpr float kSlack = 8.0f;
 constexpr int kItemSteps = 8;  // what an item's start and end cost a block, in steps
-constexpr int kMostBlocks = 6 * 160;  // blocks that the workspace has places for
 constexpr int kMostParts = kMostBlocks / kFan > kFan ? kMostBlocks / kFan : kFan;  // that are joined at a time
 
 // A step of a warp in shared memory: 32 key rows, 32 value rows, 32 + 32 parameters.
@@ -100,10 +98,11 @@ struct Shared {
 // Sums of a row tile as they leave a block: a thread holds 4 channels of each of N rows.
 template <int D, int R>
 struct Sums {
-  static constexpr int N = R * D / 4 / (kWarps * 32);
+  static constexpr int N = (R * D / 4 + kWarps * 32 - 1) / (kWarps * 32);  // D = 64, R = 8: half of the threads hold one
   float4 v[N];
   static __device__ __forceinline__ int at(int e) { return threadIdx.x + e * kWarps * 32; }  // in fours
-  static __device__ __forceinline__ int row(int e) { return at(e) / (D / 4); }
+  static __device__ __forceinline__ bool some(int e) { return R * D / 4 % (kWarps * 32) == 0 || at(e) < R * D / 4; }
+  static __device__ __forceinline__ int row(int e) { return at(e) / (D / 4) % R; }
   static __device__ __forceinline__ int channel(int e) { return at(e) % (D / 4) * 4; }
 };
 
@@ -136,11 +135,12 @@ __device__ __forceinline__ void join_parts(const Join& j, int first_place, int f
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < Sums<D, R>::N; ++e) sums.v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 0; i < count; ++i) {
     const float4* part = reinterpret_cast<const float4*>(j.parts + (int64_t)place(i) * R * D);
 #pragma unroll
     for (int e = 0; e < Sums<D, R>::N; ++e) {
+      if (!Sums<D, R>::some(e)) continue;
       const float4 x = __ldcg(part + Sums<D, R>::at(e));
       const float w = weight[i][Sums<D, R>::row(e)];
       sums.v[e].x += w * x.x;
@@ -152,7 +152,7 @@ __device__ __forceinline__ void join_parts(const Join& j, int first_place, int f
 }
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_rows_kernel(const RowsArgs p) {
+__global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_rows_kernel(const RowsArgs p) {
   const AttendArgs& a = p.a;
   using S = Stage<D>;
   constexpr int R = 8 * NT, KW = D / 32, VW = D / 64;  // rows of a tile; words of a key / value row's share of a lane
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
         v.w += k * x.w;
       }
       sums.v[e] = v;
-      if (d == 0) sh_total[row] = make_float2(top, sum);
+      if (d == 0 && Part::some(e)) sh_total[row] = make_float2(top, sum);
     }
     __syncthreads();  // the rings may be filled again
 
@@ -653,13 +653,13 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
       auto leave = [&](int place) {
 #pragma unroll
         for (int e = 0; e < Part::N; ++e)
-          reinterpret_cast<float4*>(j.parts + (int64_t)place * R * D)[Part::at(e)] = sums.v[e];
+          if (Part::some(e)) reinterpret_cast<float4*>(j.parts + (int64_t)place * R * D)[Part::at(e)] = sums.v[e];
         if (threadIdx.x < R) j.stats[(int64_t)place * R + threadIdx.x] = sh_total[threadIdx.x];
         __threadfence();
         __syncthreads();
       };
       auto last_of = [&](int level, int place, int expected) {
-        if (threadIdx.x == 0) sh_last = arrive(j.arrivals + (level * j.blocks * 2 + place), j.launch, expected);
+        if (threadIdx.x == 0) sh_last = arrive(j.arrivals + level * kMostBlocks * 2 + place, expected);
         __syncthreads();
         const bool last = sh_last != 0;
         __syncthreads();
@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
 #pragma unroll
       for (int e = 0; e < Part::N; ++e) {
         const int row = Part::row(e), d = Part::channel(e);
-        if (row < rows) {
+        if (row < rows && Part::some(e)) {
           const int r = row0 + row, i = a.group.div(r), h = head * a.group.d + (r - i * a.group.d);
           const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
           const float2 st = sh_total[row];
@@ -723,14 +723,7 @@ int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
   const int per_sm = blocks_per_sm<D, NT, T>();
   if (per_sm < 1) return TANS_E_CUDA;
   const int blocks = std::min(kMostBlocks, per_sm * sm_count());
-  static std::atomic<unsigned long long> launches{0};
-  constexpr int R = 8 * NT;
-  Join j;
-  j.parts = static_cast<float*>(workspace);
-  j.stats = reinterpret_cast<float2*>(j.parts + (int64_t)kMostBlocks * 2 * R * D);
-  j.arrivals = reinterpret_cast<unsigned long long*>(j.stats + (int64_t)kMostBlocks * 2 * R);
-  j.launch = (launches.fetch_add(1, std::memory_order_relaxed) + 1) << 16;
-  j.blocks = kMostBlocks;
+  const Join j = Join::in(workspace, 8 * NT);
   attend_rows_kernel<D, NT, T><<<blocks, kWarps * 32, Shared<D, NT>::BYTES, s>>>(RowsArgs{a, j});
   note_launch();
   return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
@@ -740,7 +733,7 @@ int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
 
 size_t attend_rows_workspace(int head_dim, int64_t max_rows) {
   const int64_t rows = max_rows <= 8 ? 8 : 16;
-  return align_up((size_t)kMostBlocks * 2 * (rows * head_dim * 4 + rows * 8 + 2 * 8));
+  return align_up(Join::bytes(rows, head_dim));
 }
 
 int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* workspace, cudaStream_t s) {

@@ -9,6 +9,11 @@
 
 static_assert(tans::kv4::Join::kArrivalBytes == TANS_KV4_ATTEND_COUNTS, "the header names the size");
 
+namespace {
+// rows of queries that share a key/value head
+bool few_rows(int64_t rows) { return rows <= 32; }
+}  // namespace
+
 extern "C" size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim,
                                                  int64_t batch, int64_t max_pages, int page_size, int64_t max_queries) {
   using namespace tans::kv4;
@@ -16,7 +21,8 @@ extern "C" size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_he
   (void)max_pages;
   (void)page_size;
   if (total_queries < 1 || kv_heads < 1 || q_heads < kv_heads) return 0;
-  return attend_rows_workspace(head_dim, std::min(max_queries, total_queries) * (q_heads / kv_heads));
+  const int64_t rows = std::min(max_queries, total_queries) * (q_heads / kv_heads);
+  return few_rows(rows) ? attend_rows_workspace(head_dim, rows) : 0;
 }
 
 extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t total_queries,
@@ -46,6 +52,7 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
                      Divider::of(group), Divider::of(kv_heads), Divider::of(page_size), pages, batch, max_pages, lengths,
                      q_starts, scale * 1.4426950408889634f, causal, vec, out, lse, dev_status};
   const int64_t most = std::min(max_queries, total_queries);
+  if (!few_rows(most * group)) return launch_attend_prompt(a, dtype, s);
   const size_t need = tans_kv4_attend_workspace_size(total_queries, q_heads, kv_heads, head_dim, batch, max_pages,
                                                      page_size, max_queries);
   void* ws = workspace;

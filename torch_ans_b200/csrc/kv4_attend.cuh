@@ -127,6 +127,7 @@ __device__ __forceinline__ bool arrive(int* count, int expected) {
 
 int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* workspace, cudaStream_t s);
 size_t attend_rows_workspace(int head_dim, int64_t max_rows);
+int launch_attend_prompt(const AttendArgs& a, int dtype, cudaStream_t s);
 
 }  // namespace kv4
 }  // namespace tans

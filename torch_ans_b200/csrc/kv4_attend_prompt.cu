@@ -1,0 +1,627 @@
+// kv4_attend_prompt.cu -- attention over the 4-bit cache when many query rows share a key/value head
+// (whole prompts, chunks of them, many drafted tokens or very wide groups): bound by arithmetic, so
+// both products run on tcgen05 with their accumulators in tensor memory.
+//
+// A block takes 128 (head_dim 256) or 2 x 128 query rows of one key/value head, row r being head
+// r mod group of query r / group, and walks over the tokens 128 at a time:
+//   softmax warps   4 for each 128 rows, a thread for a row: they read the scores S from tensor
+//                   memory, keep the row's running maximum and sum, and put the weights P back over S
+//                   as float16;
+//   unpacking warps 4, a thread for a token: its codes become float16 c * s + o in shared memory, in
+//                   the swizzled rows that the tensor cores read (keys K-major; the same rows of
+//                   values are an MN-major operand, so nothing is transposed);
+//   one warp        issues S = Q K^T (both from shared memory) and O += P V (P from tensor memory).
+// The two row tiles take turns: while one's weights are computed the other's products run.
+//
+// All operands are float16 brought into range by powers of two: a query row by its own, 128 keys by
+// theirs, values by one that only grows over the tokens (O is rescaled when it does, as when a
+// maximum moves).  So nothing that bfloat16 or float16 holds overflows, and the rounding is 2^-11 of
+// each value, key and weight; sums are float.  A maximum moves only when it is passed by over 8
+// (weights under 2^9), which rescales O rarely.
+#include "kv4_attend.cuh"
+#include "launch.cuh"
+#include "rans_host.h"
+
+#include <algorithm>
+
+namespace tans {
+namespace kv4 {
+namespace {
+
+constexpr int kTile = 128;  // rows of a tile, tokens of a step
+constexpr float kSlack = 8.0f;
+constexpr int kInfos = 4;   // steps whose factors are kept: the unpacking warps run at most 2 ahead
+constexpr int kTries = 1 << 20;
+
+template <int D>
+struct Plan {
+  static constexpr int TILES = D == 256 ? 1 : 2;   // row tiles of a block
+  static constexpr int STAGES = D == 256 ? 1 : 2;  // steps of unpacked keys and values
+  static constexpr int WARPS = 4 * TILES + 4 + 1;
+  static constexpr int BLOCK = kTile * 128;        // bytes of 64 channels of 128 rows
+  static constexpr int ROWS = BLOCK * (D / 64);    // bytes of 128 rows
+  static constexpr int Q = 0, K = ROWS * TILES, V = K + ROWS * STAGES, END = V + ROWS * STAGES;
+  // over half of an SM's shared memory even for head_dim 64: one block on an SM, which takes all of
+  // its tensor memory
+  static constexpr int BYTES = (END > 120 * 1024 ? END : 120 * 1024) + 1024;
+  static constexpr int S_COLUMNS = 128;
+  static constexpr int O = S_COLUMNS * TILES;  // first column of O
+};
+
+struct Info {  // of a step, from the unpacking warps to the softmax warps
+  float key_factor;  // what the scores are to be multiplied by
+  int value_shift;   // values are 2^value_shift times too large
+  uint32_t hidden[4], bad[4];  // tokens that no row sees, and those whose value is not finite
+};
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bar_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_of(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(bar)) : "memory");
+}
+// A bounded wait.  One that runs out is recorded in `stalled`; waits after that return at once, so the
+// block comes to its end (with values that are not valid) and frees its tensor memory.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatile int* stalled) {
+  const uint32_t at = smem_of(bar);
+  for (int i = 0; i < kTries; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(at), "r"(parity), "r"(1000)  // a microsecond each
+        : "memory");
+    if (done) return;
+    if (*stalled) return;
+  }
+  *stalled = 1;
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_of(bar))
+               : "memory");
+}
+
+// Shared memory operand: rows of 128 bytes in the 128-byte swizzle, 8 rows to 1024 bytes; `leading` is
+// the distance of the next 64 values of an MN-major operand.
+__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t leading) {
+  return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// float16 operands, float accumulator, 128 rows, n columns
+__host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+  return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool more) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)more)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool more) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)more)
+      : "memory");
+}
+
+#define TANS_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define TANS_W4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
+// 32 columns of this warp's 32 rows: a thread has its row's
+__device__ __forceinline__ void load32(uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : TANS_R4(r, 0), TANS_R4(r, 4), TANS_R4(r, 8), TANS_R4(r, 12), TANS_R4(r, 16), TANS_R4(r, 20), TANS_R4(r, 24),
+        TANS_R4(r, 28)
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void store32(const uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::TANS_W4(r, 0),
+      TANS_W4(r, 4), TANS_W4(r, 8), TANS_W4(r, 12), TANS_W4(r, 16), TANS_W4(r, 20), TANS_W4(r, 24), TANS_W4(r, 28),
+      "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void store16(const uint32_t (&r)[16], uint32_t at) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::TANS_W4(
+          r, 0),
+      TANS_W4(r, 4), TANS_W4(r, 8), TANS_W4(r, 12), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7.  The bits of c in the low
+// places of 1024 are 1024 + c, in the next four 1024 + 16 c.
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s, __half2 o) {
+  const __half2 one = __floats2half2_rn(1024.0f, 1024.0f), sixteenth = __floats2half2_rn(0.0625f, 0.0625f),
+                back = __floats2half2_rn(-64.0f, -64.0f);
+  auto low = [&](uint32_t x) {
+    const uint32_t c = (x & 0x000f000fu) | 0x64006400u;
+    const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), one), s, o);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  auto high = [&](uint32_t x) {
+    const uint32_t c = (x & 0x00f000f0u) | 0x64006400u;
+    const __half2 v = __hfma2(__hfma2(*reinterpret_cast<const __half2*>(&c), sixteenth, back), s, o);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  const uint32_t x = w >> 8;
+  return make_uint4(low(w), high(w), low(x), high(x));
+}
+
+__device__ __forceinline__ bool finite_row(uint32_t p) {
+  return fabsf(scale_of(p)) < INFINITY && fabsf(offset_of(p)) < INFINITY;  // neither for NaN
+}
+// exponent field of the larger of a row's two ends; 0 for a row that is not finite
+__device__ __forceinline__ uint32_t reach(uint32_t p) {
+  const float o = offset_of(p), top = fmaxf(fabsf(o), fabsf(fmaf(15.0f, scale_of(p), o)));
+  return finite_row(p) ? min(__float_as_uint(top) >> 23, 254u) : 0u;
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a) {
+  using P = Plan<D>;
+  constexpr int TILES = P::TILES, STAGES = P::STAGES, RT = kTile * TILES, WORDS = D / 8;
+  constexpr int kUnpack = 4 * TILES, kIssue = kUnpack + 4;  // first warps of their kind
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
+      s_full[TILES], p_full[TILES], o_full;
+  __shared__ uint32_t tensor_base;
+  __shared__ int stalled_, found[2];
+  __shared__ Sequence sh_seq;
+  __shared__ Info infos[kInfos];
+  __shared__ uint32_t top_k[2][4], top_v[2][4];
+  volatile int* stalled = &stalled_;
+  uint8_t* smem = raw + ((1024 - (smem_of(raw) & 1023)) & 1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = a.pool.kv_heads;
+
+  zero_unowned<T>(a, D, blockIdx.x * (int64_t)(P::WARPS * 32) + threadIdx.x, (int64_t)gridDim.x * P::WARPS * 32);
+
+  // ---- this block's sequence, row tiles and head; the later tiles of a sequence, which see more,
+  // come first
+  const int item = a.kv_heads.div(blockIdx.x), head = blockIdx.x - item * heads;
+  if (warp == 0) {
+    if (lane == 0) found[0] = -1;
+    __syncwarp();
+    int64_t before = 0;
+    for (int64_t b0 = 0; b0 < a.batch; b0 += 32) {
+      Sequence s{0, 0, 0};
+      int64_t n = 0;
+      if (b0 + lane < a.batch) {
+        s = sequence(a, b0 + lane, blockIdx.x == 0);
+        n = ((int64_t)s.count * a.group.d + RT - 1) / RT;
+      }
+      int64_t x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (item >= before + x - n && item < before + x) {
+        found[0] = (int)(b0 + lane);
+        found[1] = (int)(before + x - 1 - item);
+        sh_seq = s;
+      }
+      before += __shfl_sync(0xffffffffu, x, 31);
+      if (blockIdx.x != 0 && before > item) break;
+    }
+  }
+  if (threadIdx.x == 0) {
+    stalled_ = 0;
+    bar_init(&q_full, kTile * TILES);
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(&k_full[i], kTile);
+      bar_init(&v_full[i], kTile);
+      bar_init(&k_empty[i], 1);
+      bar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < TILES; ++i) {
+      bar_init(&s_full[i], 1);
+      bar_init(&p_full[i], kTile);
+    }
+    bar_init(&o_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (found[0] < 0) return;
+  const int b = found[0];
+  const Sequence seq = sh_seq;
+  const int row0 = found[1] * RT, rows = min(RT, seq.count * (int)a.group.d - row0);
+  // tokens that some row sees
+  const int ahead = seq.length - seq.count + 1;
+  const int reach_end = a.causal ? min(seq.length, ahead + a.group.div(row0 + rows - 1)) : seq.length;
+  const int steps = max(0, (reach_end + kTile - 1) / kTile);
+
+  if (warp == kIssue) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&tensor_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  const uint32_t tensor = tensor_base;
+
+  if (warp < kUnpack) {
+    // ---------------------------------------------------------------- softmax: a row of a tile
+    const int tile = warp >> 2, r = threadIdx.x & (kTile - 1), row = tile * kTile + r;
+    const bool live = row < rows;
+    const int i = a.group.div(row0 + (live ? row : 0)), h = head * a.group.d + (row0 + (live ? row : 0) - i * a.group.d);
+    const int seen = !live ? 0 : (a.causal ? min(seq.length, ahead + i) : seq.length);
+    float factor;  // scores are `factor` and the step's factor times the product, in powers of two
+    {
+      const T* src = static_cast<const T*>(a.q) + (int64_t)(seq.start + i) * a.q_ts + h * a.q_hs;
+      float top = 0.0f;
+      // twice over the row: its largest, then its values
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));
+        const float up = a.scale_log2 < 0.0f ? -pow2(e) : pow2(e);
+        factor = fabsf(a.scale_log2) * pow2(-e);
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          float x[8];
+          if (!live) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+          } else if (a.vec) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + c * 8);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = Half2<T>::unpack(u[k]);
+              x[2 * k] = f.x;
+              x[2 * k + 1] = f.y;
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = Half2<T>::load(src + c * 8 + k);
+          }
+          if (pass == 0) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
+          } else {  // channels in the order that codes unpack in
+            uint4 w;
+            w.x = Half2<__half>::pack(x[0] * up, x[4] * up);
+            w.y = Half2<__half>::pack(x[1] * up, x[5] * up);
+            w.z = Half2<__half>::pack(x[2] * up, x[6] * up);
+            w.w = Half2<__half>::pack(x[3] * up, x[7] * up);
+            *reinterpret_cast<uint4*>(smem + P::Q + tile * P::ROWS + (c >> 3) * P::BLOCK + r * 128 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = w;
+          }
+        }
+      }
+    }
+    fence_smem();
+    bar_arrive(&q_full);
+
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 rows of tensor memory
+    const uint32_t s_at = tensor + lanes + tile * P::S_COLUMNS, o_at = tensor + lanes + P::O + tile * D;
+    float m = -INFINITY, l = 0.0f;
+    bool poisoned = false;
+    int shift = 0;
+    for (int j = 0; j < steps; ++j) {
+      bar_wait(&s_full[tile], j & 1, stalled);
+      __syncwarp();
+      fence_after();
+      const Info& info = infos[j & (kInfos - 1)];
+      const float f = factor * info.key_factor;
+      const int now = info.value_shift;
+      const bool special = (info.hidden[0] | info.hidden[1] | info.hidden[2] | info.hidden[3] | info.bad[0] |
+                            info.bad[1] | info.bad[2] | info.bad[3]) != 0;
+      const int left = seen - j * kTile;  // tokens of this step that the row sees
+      const bool masked = __any_sync(0xffffffffu, left < kTile) || special;
+      uint32_t visible[4];
+      float top = -INFINITY;
+      if (masked) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int n = left - w * 32;
+          visible[w] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1);
+          if (special) {
+            visible[w] &= ~info.hidden[w];
+            poisoned |= (visible[w] & info.bad[w]) != 0;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[32];
+          load32(x, s_at + w * 32);
+          loaded();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) top = visible[w] >> k & 1 ? fmaxf(top, __uint_as_float(x[k])) : top;
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[32];
+          load32(x, s_at + w * 32);
+          loaded();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(x[k]));
+        }
+      }
+      top = top == -INFINITY ? top : top * f;
+      const bool moves = top > m + kSlack;
+      const float next = moves ? top : m;
+      if (__any_sync(0xffffffffu, moves || now != shift)) {
+        const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
+        l *= keep;
+        if (j > 0) {  // O is not yet written before the first step
+          const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t x[32];
+            load32(x, o_at + c);
+            loaded();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * both);
+            store32(x, o_at + c);
+          }
+        }
+      }
+      m = next;
+      shift = now;
+      const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t x[32], p[16];
+        load32(x, s_at + w * 32);
+        loaded();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float e0 = ex2(fmaf(__uint_as_float(x[2 * k]), f, -base)), e1 = ex2(fmaf(__uint_as_float(x[2 * k + 1]), f, -base));
+          if (masked) {
+            e0 = visible[w] >> (2 * k) & 1 ? e0 : 0.0f;
+            e1 = visible[w] >> (2 * k + 1) & 1 ? e1 : 0.0f;
+          }
+          l += e0 + e1;
+          p[k] = Half2<__half>::pack(e0, e1);
+        }
+        store16(p, s_at + w * 16);  // over scores that are already read
+      }
+      stored();
+      fence_before();
+      bar_arrive(&p_full[tile]);
+    }
+    // ---- the rows' results
+    if (steps > 0) {
+      bar_wait(&o_full, 0, stalled);
+      __syncwarp();
+      fence_after();
+    }
+    const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
+    float k = l == 0.0f ? 0.0f : pow2(max(-126, min(127, -shift))) / l;
+    if (poisoned) k = __int_as_float(0x7fffffff);
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t x[32];
+      if (steps > 0) {
+        load32(x, o_at + c);
+        loaded();
+      }
+      if (live) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e]) * k;
+            v[e + 4] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e + 1]) * k;
+          }
+          uint4 w;
+          w.x = Half2<T>::pack(v[0], v[1]);
+          w.y = Half2<T>::pack(v[2], v[3]);
+          w.z = Half2<T>::pack(v[4], v[5]);
+          w.w = Half2<T>::pack(v[6], v[7]);
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + c + g * 8) = w;
+        }
+      }
+    }
+    if (live && a.lse) a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  } else if (warp < kIssue) {
+    // ---------------------------------------------------------------- unpacking: a token of a step
+    const int t = threadIdx.x - kUnpack * 32;
+    const int32_t* table = a.pages + (int64_t)b * a.max_pages;
+    const int64_t side_rows = (int64_t)heads * a.pool.page_size;
+    uint4 kc[D / 32], vc[D / 32];
+    uint32_t kp = 0, vp = 0;
+    int page = -1, state = 0;  // 0: past the end, 1: a row of the cache, 2: hidden
+    auto look_up = [&](int j) {
+      const int token = j * kTile + t;
+      page = j < steps && token < seq.length ? __ldg(table + a.page_size.div(token)) : -1;
+    };
+    const uint8_t* from = nullptr;
+    auto fetch_keys = [&](int j) {  // and both rows' parameters
+      const int token = j * kTile + t;
+      state = 0;
+      kp = vp = 0;
+      if (j < steps && token < seq.length) {
+        if ((unsigned)page < (unsigned)a.pool.num_pages) {
+          state = 1;
+          const int64_t at = a.pool.row(page, 0, head) + (token - a.page_size.div(token) * a.pool.page_size);
+          kp = __ldg(a.pool.params + at);
+          vp = __ldg(a.pool.params + at + side_rows);
+          from = a.pool.codes + at * (D / 2);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) kc[c] = __ldg(reinterpret_cast<const uint4*>(from) + c);
+        } else {
+          state = 2;
+          flag(a.status, TANS_DEV_BAD_INDEX);
+        }
+      }
+      if (state != 1) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) kc[c] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto fetch_values = [&]() {
+      if (state == 1) {
+        const uint4* src = reinterpret_cast<const uint4*>(from + side_rows * (D / 2));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) vc[c] = __ldg(src + c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) vc[c] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto spread = [&](const uint4 (&codes)[D / 32], float scale, float offset, uint8_t* dst) {
+      const __half2 s = __float2half2_rn(scale), o = __float2half2_rn(offset);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const uint32_t w[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int chunk = c * 4 + k;
+          *reinterpret_cast<uint4*>(dst + (chunk >> 3) * P::BLOCK + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) =
+              unpack8(w[k], s, o);
+        }
+      }
+    };
+    look_up(0);
+    fetch_keys(0);
+    fetch_values();
+    look_up(1);
+    uint32_t value_top = 27;  // exponent field of the largest value so far
+    for (int j = 0; j < steps; ++j) {
+      const int stage = j % STAGES;
+      const uint32_t filled = (uint32_t)(j / STAGES) & 1;
+      // the largest key and value, over the step
+      const uint32_t wk = __reduce_max_sync(0xffffffffu, reach(kp)), wv = __reduce_max_sync(0xffffffffu, reach(vp));
+      if (lane == 0) {
+        top_k[j & 1][warp - kUnpack] = wk;
+        top_v[j & 1][warp - kUnpack] = wv;
+      }
+      const bool bad = state == 1 && !finite_row(vp);
+      const uint32_t hidden = __ballot_sync(0xffffffffu, state == 2), wrong = __ballot_sync(0xffffffffu, bad);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      uint32_t key_top = 27;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        key_top = max(key_top, top_k[j & 1][w]);
+        value_top = max(value_top, top_v[j & 1][w]);
+      }
+      const int key_shift = 140 - (int)key_top, value_shift = 140 - (int)value_top;  // under 2^14
+      bar_wait(&k_empty[stage], filled ^ 1, stalled);
+      Info& info = infos[j & (kInfos - 1)];
+      if (t == 0) {
+        info.key_factor = pow2(-key_shift);
+        info.value_shift = value_shift;
+      }
+      if (lane == 0) {
+        info.hidden[warp - kUnpack] = hidden;
+        info.bad[warp - kUnpack] = wrong;
+      }
+      spread(kc, scale_of(kp) * pow2(key_shift), offset_of(kp) * pow2(key_shift), smem + P::K + stage * P::ROWS);
+      fence_smem();
+      bar_arrive(&k_full[stage]);
+      const float vs = bad || state != 1 ? 0.0f : scale_of(vp) * pow2(value_shift);
+      const float vo = bad || state != 1 ? 0.0f : offset_of(vp) * pow2(value_shift);
+      fetch_keys(j + 1);
+      look_up(j + 2);
+      bar_wait(&v_empty[stage], filled ^ 1, stalled);
+      spread(vc, vs, vo, smem + P::V + stage * P::ROWS);
+      fence_smem();
+      bar_arrive(&v_full[stage]);
+      fetch_values();
+    }
+  } else if (lane == 0 && steps > 0) {
+    // ---------------------------------------------------------------- products
+    const uint32_t base = smem_of(smem);
+    constexpr uint32_t id_s = instruction(kTile, false), id_o = instruction(D, true);
+    auto scores = [&](int tile, int stage) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t in = (k >> 2) * P::BLOCK + (k & 3) * 32;
+        mma_ss(tensor + tile * P::S_COLUMNS, operand(base + P::Q + tile * P::ROWS + in, 16),
+               operand(base + P::K + stage * P::ROWS + in, 16), id_s, k > 0);
+      }
+    };
+    auto values = [&](int tile, int stage, bool more) {
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        mma_ts(tensor + P::O + tile * D, tensor + tile * P::S_COLUMNS + k * 8,
+               operand(base + P::V + stage * P::ROWS + k * 2048, P::BLOCK), id_o, more || k > 0);
+    };
+    bar_wait(&q_full, 0, stalled);
+    bar_wait(&k_full[0], 0, stalled);
+    fence_after();
+    for (int tile = 0; tile < TILES; ++tile) {
+      scores(tile, 0);
+      commit(&s_full[tile]);
+    }
+    commit(&k_empty[0]);
+    for (int j = 0; j < steps; ++j) {
+      const int stage = j % STAGES, next = (j + 1) % STAGES;
+      const uint32_t filled = (uint32_t)(j / STAGES) & 1, next_filled = (uint32_t)((j + 1) / STAGES) & 1;
+      bar_wait(&v_full[stage], filled, stalled);
+      if (j + 1 < steps) bar_wait(&k_full[next], next_filled, stalled);
+      for (int tile = 0; tile < TILES; ++tile) {
+        bar_wait(&p_full[tile], j & 1, stalled);
+        fence_after();
+        values(tile, stage, j > 0);
+        if (tile == TILES - 1) commit(&v_empty[stage]);
+        if (j + 1 < steps) {
+          scores(tile, next);
+          commit(&s_full[tile]);
+        }
+      }
+      if (j + 1 < steps) commit(&k_empty[next]);
+    }
+    commit(&o_full);
+    // nothing is in flight when the tensor memory is given back, even after a wait that ran out
+    volatile int late = 0;
+    bar_wait(&o_full, 0, &late);
+  }
+  fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && stalled_) flag(a.status, TANS_DEV_STALLED);
+  if (warp == kIssue) {
+    __syncwarp();
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tensor));
+  }
+}
+
+template <int D, typename T>
+int launch(const AttendArgs& a, cudaStream_t s) {
+  using P = Plan<D>;
+  static bool ready = false;
+  if (!ready) {
+    if (cudaFuncSetAttribute(attend_prompt_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) !=
+        cudaSuccess)
+      return TANS_E_CUDA;
+    ready = true;
+  }
+  // row tiles: at most one that is not full for each sequence
+  const int64_t rows = a.total_queries * a.group.d, tile = kTile * P::TILES;
+  const int64_t blocks = (rows / tile + std::min(a.batch, a.total_queries)) * a.pool.kv_heads;
+  if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
+  attend_prompt_kernel<D, T><<<(unsigned)std::max<int64_t>(blocks, 1), P::WARPS * 32, P::BYTES, s>>>(a);
+  note_launch();
+  return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
+}
+
+}  // namespace
+
+int launch_attend_prompt(const AttendArgs& a, int dtype, cudaStream_t s) {
+  auto by_dim = [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return a.pool.head_dim == 64 ? launch<64, T>(a, s) : a.pool.head_dim == 128 ? launch<128, T>(a, s) : launch<256, T>(a, s);
+  };
+  return dtype == TANS_BF16 ? by_dim(static_cast<__nv_bfloat16*>(nullptr)) : by_dim(static_cast<__half*>(nullptr));
+}
+
+}  // namespace kv4
+}  // namespace tans

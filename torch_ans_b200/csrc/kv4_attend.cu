@@ -17,12 +17,11 @@ bool few_rows(int64_t rows) { return rows <= 32; }
 extern "C" size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim,
                                                  int64_t batch, int64_t max_pages, int page_size, int64_t max_queries) {
   using namespace tans::kv4;
-  (void)batch;
-  (void)max_pages;
-  (void)page_size;
   if (total_queries < 1 || kv_heads < 1 || q_heads < kv_heads) return 0;
   const int64_t rows = std::min(max_queries, total_queries) * (q_heads / kv_heads);
-  return few_rows(rows) ? attend_rows_workspace(head_dim, rows) : 0;
+  return few_rows(rows) ? attend_rows_workspace(head_dim, rows)
+                        : attend_prompt_workspace(head_dim, total_queries * (q_heads / kv_heads),
+                                                  std::min(batch, total_queries), kv_heads, max_pages * page_size);
 }
 
 extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t total_queries,
@@ -52,10 +51,10 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
                      Divider::of(group), Divider::of(kv_heads), Divider::of(page_size), pages, batch, max_pages, lengths,
                      q_starts, scale * 1.4426950408889634f, causal, vec, out, lse, dev_status};
   const int64_t most = std::min(max_queries, total_queries);
-  if (!few_rows(most * group)) return launch_attend_prompt(a, dtype, s);
   const size_t need = tans_kv4_attend_workspace_size(total_queries, q_heads, kv_heads, head_dim, batch, max_pages,
                                                      page_size, max_queries);
   void* ws = workspace;
+  if (need == 0) return launch_attend_prompt(a, dtype, nullptr, s);
   if (!ws) {
     if (cudaMallocAsync(&ws, need, s) != cudaSuccess) return TANS_E_CUDA;
     if (cudaMemsetAsync(ws, 0, Join::kArrivalBytes, s) != cudaSuccess) {
@@ -65,7 +64,8 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
   } else if (workspace_bytes < need) {
     return TANS_E_WORKSPACE;
   }
-  const int rc = launch_attend_rows(a, dtype, most * group, ws, s);
+  const int rc = few_rows(most * group) ? launch_attend_rows(a, dtype, most * group, ws, s)
+                                        : launch_attend_prompt(a, dtype, ws, s);
   if (!workspace) cudaFreeAsync(ws, s);
   return rc;
 }

@@ -127,7 +127,8 @@ __device__ __forceinline__ bool arrive(int* count, int expected) {
 
 int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* workspace, cudaStream_t s);
 size_t attend_rows_workspace(int head_dim, int64_t max_rows);
-int launch_attend_prompt(const AttendArgs& a, int dtype, cudaStream_t s);
+int launch_attend_prompt(const AttendArgs& a, int dtype, void* workspace, cudaStream_t s);
+size_t attend_prompt_workspace(int head_dim, int64_t total_rows, int64_t batch, int kv_heads, int64_t max_tokens);
 
 }  // namespace kv4
 }  // namespace tans

@@ -13,6 +13,9 @@
 //   one warp        issues S = Q K^T (both from shared memory) and O += P V (P from tensor memory).
 // The two row tiles take turns: while one's weights are computed the other's products run.
 //
+// Where there are fewer such row tiles than SMs, several blocks share the tokens of each, leave their
+// sums in the workspace, and the last of them joins them in the order of the tokens.
+//
 // All operands are float16 brought into range by powers of two: a query row by its own, 128 keys by
 // theirs, values by one that only grows over the tokens (O is rescaled when it does, as when a
 // maximum moves).  So nothing that bfloat16 or float16 holds overflows, and the rounding is 2^-11 of
@@ -47,6 +50,15 @@ struct Plan {
   static constexpr int S_COLUMNS = 128;
   static constexpr int O = S_COLUMNS * TILES;  // first column of O
 };
+
+// The blocks that share a row tile's tokens, and where they leave their sums.
+struct Split {
+  int splits;     // blocks for each row tile and head
+  int* arrivals;  // one for each of these
+  float2* stats;  // [row tile and head][splits][rows]: maximum (a power of two's exponent) and sum
+  float4* parts;  // [row tile and head][splits][dim / 4][rows]
+};
+constexpr int kLeastSteps = 4;  // that a block takes, if there are as many
 
 struct Info {  // of a step, from the unpacking warps to the softmax warps
   float key_factor;  // what the scores are to be multiplied by
@@ -169,7 +181,7 @@ __device__ __forceinline__ uint32_t reach(uint32_t p) {
 }
 
 template <int D, typename T>
-__global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a, const Split split) {
   using P = Plan<D>;
   constexpr int TILES = P::TILES, STAGES = P::STAGES, RT = kTile * TILES, WORDS = D / 8;
   constexpr int kUnpack = 4 * TILES, kIssue = kUnpack + 4;  // first warps of their kind
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
       s_full[TILES], p_full[TILES], o_full;
   __shared__ uint32_t tensor_base;
-  __shared__ int stalled_, found[2];
+  __shared__ int stalled_, found[2], sh_last;
   __shared__ Sequence sh_seq;
   __shared__ Info infos[kInfos];
   __shared__ uint32_t top_k[2][4], top_v[2][4];
@@ -190,7 +202,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
 
   // ---- this block's sequence, row tiles and head; the later tiles of a sequence, which see more,
   // come first
-  const int item = a.kv_heads.div(blockIdx.x), head = blockIdx.x - item * heads;
+  const int tile_head = blockIdx.x / split.splits, part = blockIdx.x - tile_head * split.splits;
+  const int item = a.kv_heads.div(tile_head), head = tile_head - item * heads;
   if (warp == 0) {
     if (lane == 0) found[0] = -1;
     __syncwarp();
@@ -241,7 +254,11 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   // tokens that some row sees
   const int ahead = seq.length - seq.count + 1;
   const int reach_end = a.causal ? min(seq.length, ahead + a.group.div(row0 + rows - 1)) : seq.length;
-  const int steps = max(0, (reach_end + kTile - 1) / kTile);
+  const int all_steps = max(0, (reach_end + kTile - 1) / kTile);
+  const int share = max(kLeastSteps, (all_steps + split.splits - 1) / split.splits);
+  const int parts = max(1, (all_steps + share - 1) / share);
+  if (part >= parts) return;
+  const int step0 = part * share, steps = min(share, all_steps - step0);  // this block's
 
   if (warp == kIssue) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&tensor_base))
@@ -320,7 +337,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       const int now = info.value_shift;
       const bool special = (info.hidden[0] | info.hidden[1] | info.hidden[2] | info.hidden[3] | info.bad[0] |
                             info.bad[1] | info.bad[2] | info.bad[3]) != 0;
-      const int left = seen - j * kTile;  // tokens of this step that the row sees
+      const int left = seen - (step0 + j) * kTile;  // tokens of this step that the row sees
       const bool masked = __any_sync(0xffffffffu, left < kTile) || special;
       uint32_t visible[4];
       float top = -INFINITY;
@@ -402,8 +419,19 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       fence_after();
     }
     const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
-    float k = l == 0.0f ? 0.0f : pow2(max(-126, min(127, -shift))) / l;
-    if (poisoned) k = __int_as_float(0x7fffffff);
+    const float back = pow2(max(-126, min(127, -shift)));
+    if (poisoned) l = __int_as_float(0x7fffffff);
+    // 8 channels of the row, unpacking's order undone
+    auto write8 = [&](int d, const float (&v)[8], float k) {
+      uint4 w;
+      w.x = Half2<T>::pack(v[0] * k, v[1] * k);
+      w.y = Half2<T>::pack(v[2] * k, v[3] * k);
+      w.z = Half2<T>::pack(v[4] * k, v[5] * k);
+      w.w = Half2<T>::pack(v[6] * k, v[7] * k);
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + d) = w;
+    };
+    const int64_t mine = (int64_t)tile_head * split.splits + part;
+    const float k = l == 0.0f ? 0.0f : back / l;
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t x[32];
@@ -417,19 +445,59 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
           float v[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e]) * k;
-            v[e + 4] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e + 1]) * k;
+            v[e] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e]);
+            v[e + 4] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e + 1]);
           }
-          uint4 w;
-          w.x = Half2<T>::pack(v[0], v[1]);
-          w.y = Half2<T>::pack(v[2], v[3]);
-          w.z = Half2<T>::pack(v[4], v[5]);
-          w.w = Half2<T>::pack(v[6], v[7]);
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + c + g * 8) = w;
+          if (parts == 1) {
+            write8(c + g * 8, v, k);
+          } else {
+            float4* to = split.parts + (mine * (D / 4) + c / 4 + g * 2) * RT + row;
+            to[0] = make_float4(v[0] * back, v[1] * back, v[2] * back, v[3] * back);
+            to[RT] = make_float4(v[4] * back, v[5] * back, v[6] * back, v[7] * back);
+          }
         }
       }
     }
-    if (live && a.lse) a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    if (parts > 1) {
+      split.stats[mine * RT + row] = make_float2(m, l);
+      __threadfence();
+      asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
+      if (threadIdx.x == 0) sh_last = arrive(split.arrivals + tile_head, parts);
+      asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
+      if (sh_last) {
+        __threadfence();
+        const int64_t first = (int64_t)tile_head * split.splits;
+        m = -INFINITY;
+        for (int p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&split.stats[(first + p) * RT + row]).x);
+        const float base = m == -INFINITY ? 0.0f : m;
+        l = 0.0f;
+        for (int p = 0; p < parts; ++p) {
+          const float2 st = __ldcg(&split.stats[(first + p) * RT + row]);
+          l += ex2(st.x - base) * st.y;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int d = 0; live && d < D; d += 16) {
+          float v[2][8] = {};
+          for (int p = 0; p < parts; ++p) {
+            const float w = ex2(__ldcg(&split.stats[(first + p) * RT + row]).x - base);
+            const float4* from = split.parts + ((first + p) * (D / 4) + d / 4) * RT + row;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 x = __ldcg(from + e * RT);
+              v[e >> 1][(e & 1) * 4] += w * x.x;
+              v[e >> 1][(e & 1) * 4 + 1] += w * x.y;
+              v[e >> 1][(e & 1) * 4 + 2] += w * x.z;
+              v[e >> 1][(e & 1) * 4 + 3] += w * x.w;
+            }
+          }
+          write8(d, v[0], inv);
+          write8(d + 8, v[1], inv);
+        }
+      }
+    }
+    if (live && a.lse && (parts == 1 || sh_last))
+      a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   } else if (warp < kIssue) {
     // ---------------------------------------------------------------- unpacking: a token of a step
     const int t = threadIdx.x - kUnpack * 32;
@@ -439,12 +507,12 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     uint32_t kp = 0, vp = 0;
     int page = -1, state = 0;  // 0: past the end, 1: a row of the cache, 2: hidden
     auto look_up = [&](int j) {
-      const int token = j * kTile + t;
+      const int token = (step0 + j) * kTile + t;
       page = j < steps && token < seq.length ? __ldg(table + a.page_size.div(token)) : -1;
     };
     const uint8_t* from = nullptr;
     auto fetch_keys = [&](int j) {  // and both rows' parameters
-      const int token = j * kTile + t;
+      const int token = (step0 + j) * kTile + t;
       state = 0;
       kp = vp = 0;
       if (j < steps && token < seq.length) {
@@ -594,8 +662,33 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   }
 }
 
+// Row tiles times heads, at most: one tile that is not full for each sequence that has queries.
+int64_t most_tiles(int tile, int64_t total_rows, int64_t sequences, int kv_heads) {
+  return std::max<int64_t>(1, (total_rows / tile + sequences) * kv_heads);
+}
+
+// Blocks for each row tile: all tiles at once when they fill the SMs; else the number that ends first,
+// with as many rounds of blocks as it takes and a block's start and end (and its part in the join)
+// costing it as much as 4 steps.  The lengths are only known by their bound here; a block that finds
+// nothing to do ends at once.
+int splits_for(int64_t tiles, int64_t max_tokens) {
+  const int sms = sm_count();
+  const int64_t steps = (max_tokens + kTile - 1) / kTile;
+  if (tiles >= sms) return 1;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= 64 && tiles * n <= 2 * sms && (n == 1 || (n - 1) * kLeastSteps < steps); ++n) {
+    const int64_t cost = (tiles * n + sms - 1) / sms * ((steps + n - 1) / n + 4);
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+
 template <int D, typename T>
-int launch(const AttendArgs& a, cudaStream_t s) {
+int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
   using P = Plan<D>;
   static bool ready = false;
   if (!ready) {
@@ -604,21 +697,36 @@ int launch(const AttendArgs& a, cudaStream_t s) {
       return TANS_E_CUDA;
     ready = true;
   }
-  // row tiles: at most one that is not full for each sequence
-  const int64_t rows = a.total_queries * a.group.d, tile = kTile * P::TILES;
-  const int64_t blocks = (rows / tile + std::min(a.batch, a.total_queries)) * a.pool.kv_heads;
-  if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
-  attend_prompt_kernel<D, T><<<(unsigned)std::max<int64_t>(blocks, 1), P::WARPS * 32, P::BYTES, s>>>(a);
+  constexpr int RT = kTile * P::TILES;
+  const int64_t tiles = most_tiles(RT, a.total_queries * a.group.d, std::min(a.batch, a.total_queries), a.pool.kv_heads);
+  if (tiles > 0x7fffffff) return TANS_E_TOO_LARGE;
+  Split split{1, nullptr, nullptr, nullptr};
+  if (workspace) {
+    split.splits = splits_for(tiles, a.max_pages * a.pool.page_size);
+    split.arrivals = static_cast<int*>(workspace);
+    split.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + Join::kArrivalBytes);
+    split.parts = reinterpret_cast<float4*>(split.stats + tiles * split.splits * RT);
+  }
+  attend_prompt_kernel<D, T><<<(unsigned)(tiles * split.splits), P::WARPS * 32, P::BYTES, s>>>(a, split);
   note_launch();
   return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
 }
 
 }  // namespace
 
-int launch_attend_prompt(const AttendArgs& a, int dtype, cudaStream_t s) {
+size_t attend_prompt_workspace(int head_dim, int64_t total_rows, int64_t sequences, int kv_heads, int64_t max_tokens) {
+  const int64_t rows = head_dim == 256 ? kTile : 2 * kTile;
+  const int64_t tiles = most_tiles((int)rows, total_rows, sequences, kv_heads);
+  const int splits = splits_for(tiles, max_tokens);
+  return splits == 1 ? 0 : align_up(Join::kArrivalBytes + (size_t)tiles * splits * rows * (8 + head_dim * 4));
+}
+
+int launch_attend_prompt(const AttendArgs& a, int dtype, void* workspace, cudaStream_t s) {
   auto by_dim = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return a.pool.head_dim == 64 ? launch<64, T>(a, s) : a.pool.head_dim == 128 ? launch<128, T>(a, s) : launch<256, T>(a, s);
+    return a.pool.head_dim == 64    ? launch<64, T>(a, workspace, s)
+           : a.pool.head_dim == 128 ? launch<128, T>(a, workspace, s)
+                                    : launch<256, T>(a, workspace, s);
   };
   return dtype == TANS_BF16 ? by_dim(static_cast<__nv_bfloat16*>(nullptr)) : by_dim(static_cast<__half*>(nullptr));
 }

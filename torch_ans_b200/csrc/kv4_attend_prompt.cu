@@ -26,6 +26,7 @@
 #include "rans_host.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tans {
 namespace kv4 {
@@ -40,7 +41,13 @@ template <int D>
 struct Plan {
   static constexpr int TILES = D == 256 ? 1 : 2;   // row tiles of a block
   static constexpr int STAGES = D == 256 ? 1 : 2;  // steps of unpacked keys and values
-  static constexpr int WARPS = 4 * TILES + 4 + 1;
+  static constexpr int WARPS = 4 * TILES + 4 + 4;  // a warpgroup each for a row tile, unpacking, and issuing (one warp)
+  // Registers of a thread, moved from the groups that need few; each group's share comes out of the
+  // launch's 512 (of 384 threads: 504) for the four warps that an SM's quarter holds.
+  static constexpr int LAUNCH_REGS = D == 256 ? 168 : 128;
+  static constexpr int SOFTMAX_REGS = D == 256 ? 240 : 192, UNPACK_REGS = D == 256 ? 192 : 96,
+                       ISSUE_REGS = D == 256 ? 40 : 32;
+  static_assert(TILES * SOFTMAX_REGS + UNPACK_REGS + ISSUE_REGS <= LAUNCH_REGS * WARPS / 4, "a wait without end");
   static constexpr int BLOCK = kTile * 128;        // bytes of 64 channels of 128 rows
   static constexpr int ROWS = BLOCK * (D / 64);    // bytes of 128 rows
   static constexpr int Q = 0, K = ROWS * TILES, V = K + ROWS * STAGES, END = V + ROWS * STAGES;
@@ -134,12 +141,11 @@ __device__ __forceinline__ void load32(uint32_t (&r)[32], uint32_t at) {
       : "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void store32(const uint32_t (&r)[32], uint32_t at) {
+__device__ __forceinline__ void load16(uint32_t (&r)[16], uint32_t at) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::TANS_W4(r, 0),
-      TANS_W4(r, 4), TANS_W4(r, 8), TANS_W4(r, 12), TANS_W4(r, 16), TANS_W4(r, 20), TANS_W4(r, 24), TANS_W4(r, 28),
-      "r"(at)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : TANS_R4(r, 0), TANS_R4(r, 4), TANS_R4(r, 8), TANS_R4(r, 12)
+      : "r"(at)
       : "memory");
 }
 __device__ __forceinline__ void store16(const uint32_t (&r)[16], uint32_t at) {
@@ -150,6 +156,16 @@ __device__ __forceinline__ void store16(const uint32_t (&r)[16], uint32_t at) {
       : "memory");
 }
 __device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+#define TANS_RW4(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3])
+// no use of these registers comes before this place (the wait that the loads into them need)
+__device__ __forceinline__ void hold(uint32_t (&r)[16]) {
+  asm volatile("" : TANS_RW4(r, 0), TANS_RW4(r, 4), TANS_RW4(r, 8), TANS_RW4(r, 12));
+}
+__device__ __forceinline__ void hold(uint32_t (&r)[32]) {
+  asm volatile(""
+               : TANS_RW4(r, 0), TANS_RW4(r, 4), TANS_RW4(r, 8), TANS_RW4(r, 12), TANS_RW4(r, 16), TANS_RW4(r, 20),
+                 TANS_RW4(r, 24), TANS_RW4(r, 28));
+}
 __device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7.  The bits of c in the low
@@ -183,7 +199,7 @@ __device__ __forceinline__ uint32_t reach(uint32_t p) {
 template <int D, typename T>
 __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a, const Split split) {
   using P = Plan<D>;
-  constexpr int TILES = P::TILES, STAGES = P::STAGES, RT = kTile * TILES, WORDS = D / 8;
+  constexpr int TILES = P::TILES, STAGES = P::STAGES, RT = kTile * TILES;
   constexpr int kUnpack = 4 * TILES, kIssue = kUnpack + 4;  // first warps of their kind
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
@@ -271,6 +287,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   const uint32_t tensor = tensor_base;
 
   if (warp < kUnpack) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::SOFTMAX_REGS));
     // ---------------------------------------------------------------- softmax: a row of a tile
     const int tile = warp >> 2, r = threadIdx.x & (kTile - 1), row = tile * kTile + r;
     const bool live = row < rows;
@@ -339,8 +356,14 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
                             info.bad[1] | info.bad[2] | info.bad[3]) != 0;
       const int left = seen - (step0 + j) * kTile;  // tokens of this step that the row sees
       const bool masked = __any_sync(0xffffffffu, left < kTile) || special;
+      uint32_t x[4][32];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) load32(x[w], s_at + w * 32);
+      loaded();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) hold(x[w]);
       uint32_t visible[4];
-      float top = -INFINITY;
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (masked) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -350,25 +373,16 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
             visible[w] &= ~info.hidden[w];
             poisoned |= (visible[w] & info.bad[w]) != 0;
           }
-        }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t x[32];
-          load32(x, s_at + w * 32);
-          loaded();
-#pragma unroll
-          for (int k = 0; k < 32; ++k) top = visible[w] >> k & 1 ? fmaxf(top, __uint_as_float(x[k])) : top;
+          for (int k = 0; k < 32; ++k) tops[k & 3] = visible[w] >> k & 1 ? fmaxf(tops[k & 3], __uint_as_float(x[w][k])) : tops[k & 3];
         }
       } else {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t x[32];
-          load32(x, s_at + w * 32);
-          loaded();
+        for (int w = 0; w < 4; ++w)
 #pragma unroll
-          for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(x[k]));
-        }
+          for (int k = 0; k < 32; ++k) tops[k & 3] = fmaxf(tops[k & 3], __uint_as_float(x[w][k]));
       }
+      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       top = top == -INFINITY ? top : top * f;
       const bool moves = top > m + kSlack;
       const float next = moves ? top : m;
@@ -378,36 +392,43 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         if (j > 0) {  // O is not yet written before the first step
           const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t x[32];
-            load32(x, o_at + c);
+          for (int c = 0; c < D; c += 16) {
+            uint32_t y[16];
+            load16(y, o_at + c);
             loaded();
+            hold(y);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * both);
-            store32(x, o_at + c);
+            for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * both);
+            store16(y, o_at + c);
           }
         }
       }
       m = next;
       shift = now;
       const float base = m == -INFINITY ? 0.0f : m;
+      float sums[2] = {0.0f, 0.0f};
+      auto weigh = [&](auto masked_) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t x[32], p[16];
-        load32(x, s_at + w * 32);
-        loaded();
+        for (int w = 0; w < 4; ++w) {
+          uint32_t p[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          float e0 = ex2(fmaf(__uint_as_float(x[2 * k]), f, -base)), e1 = ex2(fmaf(__uint_as_float(x[2 * k + 1]), f, -base));
-          if (masked) {
-            e0 = visible[w] >> (2 * k) & 1 ? e0 : 0.0f;
-            e1 = visible[w] >> (2 * k + 1) & 1 ? e1 : 0.0f;
+          for (int k = 0; k < 16; ++k) {
+            float e0 = ex2(fmaf(__uint_as_float(x[w][2 * k]), f, -base));
+            float e1 = ex2(fmaf(__uint_as_float(x[w][2 * k + 1]), f, -base));
+            if constexpr (decltype(masked_)::value) {
+              e0 = visible[w] >> (2 * k) & 1 ? e0 : 0.0f;
+              e1 = visible[w] >> (2 * k + 1) & 1 ? e1 : 0.0f;
+            }
+            sums[0] += e0;
+            sums[1] += e1;
+            p[k] = Half2<__half>::pack(e0, e1);
           }
-          l += e0 + e1;
-          p[k] = Half2<__half>::pack(e0, e1);
+          store16(p, s_at + w * 16);  // over the scores
         }
-        store16(p, s_at + w * 16);  // over scores that are already read
-      }
+      };
+      if (masked) weigh(std::true_type{});
+      else weigh(std::false_type{});
+      l += sums[0] + sums[1];
       stored();
       fence_before();
       bar_arrive(&p_full[tile]);
@@ -438,6 +459,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       if (steps > 0) {
         load32(x, o_at + c);
         loaded();
+        hold(x);
       }
       if (live) {
 #pragma unroll
@@ -499,6 +521,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     if (live && a.lse && (parts == 1 || sh_last))
       a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   } else if (warp < kIssue) {
+    if constexpr (P::UNPACK_REGS > P::LAUNCH_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
     // ---------------------------------------------------------------- unpacking: a token of a step
     const int t = threadIdx.x - kUnpack * 32;
     const int32_t* table = a.pages + (int64_t)b * a.max_pages;
@@ -604,7 +628,9 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       bar_arrive(&v_full[stage]);
       fetch_values();
     }
-  } else if (lane == 0 && steps > 0) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::ISSUE_REGS));
+    if (warp == kIssue && lane == 0 && steps > 0) {
     // ---------------------------------------------------------------- products
     const uint32_t base = smem_of(smem);
     constexpr uint32_t id_s = instruction(kTile, false), id_o = instruction(D, true);
@@ -651,6 +677,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     // nothing is in flight when the tensor memory is given back, even after a wait that ran out
     volatile int late = 0;
     bar_wait(&o_full, 0, &late);
+    }
   }
   fence_before();
   __syncthreads();

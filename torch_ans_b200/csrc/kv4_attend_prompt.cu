@@ -68,7 +68,7 @@ struct Split {
 constexpr int kLeastSteps = 4;  // that a block takes, if there are as many
 
 struct Info {  // of a step, from the unpacking warps to the softmax warps
-  float key_factor;  // what the scores are to be multiplied by
+  int key_shift;     // keys are 2^key_shift times too large
   int value_shift;   // values are 2^value_shift times too large
   uint32_t hidden[4], bad[4];  // tokens that no row sees, and those whose value is not finite
 };
@@ -85,8 +85,13 @@ __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
 // block comes to its end (with values that are not valid) and frees its tensor memory.
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatile int* stalled) {
   const uint32_t at = smem_of(bar);
+  uint32_t done;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}\n"
+               : "=r"(done)
+               : "r"(at), "r"(parity)
+               : "memory");
+  if (done) return;
   for (int i = 0; i < kTries; ++i) {
-    uint32_t done;
     asm volatile(
         "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n"
         : "=r"(done)
@@ -96,6 +101,13 @@ __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatil
     if (*stalled) return;
   }
   *stalled = 1;
+}
+
+// true for one thread of the warp
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -168,32 +180,32 @@ __device__ __forceinline__ void hold(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7.  The bits of c in the low
-// places of 1024 are 1024 + c, in the next four 1024 + 16 c.
-__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s, __half2 o) {
-  const __half2 one = __floats2half2_rn(1024.0f, 1024.0f), sixteenth = __floats2half2_rn(0.0625f, 0.0625f),
-                back = __floats2half2_rn(-64.0f, -64.0f);
-  auto low = [&](uint32_t x) {
-    const uint32_t c = (x & 0x000f000fu) | 0x64006400u;
-    const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), one), s, o);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  };
-  auto high = [&](uint32_t x) {
-    const uint32_t c = (x & 0x00f000f0u) | 0x64006400u;
-    const __half2 v = __hfma2(__hfma2(*reinterpret_cast<const __half2*>(&c), sixteenth, back), s, o);
+// 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7, from s24 = s * 2^24 and s20 =
+// s * 2^20: the bits of c in the low four bits of a half are c * 2^-24, in the next four c * 2^-20.  The
+// product is exact, so a value is rounded once.
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s24, __half2 s20, __half2 o) {
+  auto value = [&](uint32_t c, __half2 s) {
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c), s, o);
     return *reinterpret_cast<const uint32_t*>(&v);
   };
   const uint32_t x = w >> 8;
-  return make_uint4(low(w), high(w), low(x), high(x));
+  return make_uint4(value(w & 0x000f000fu, s24), value(w & 0x00f000f0u, s20), value(x & 0x000f000fu, s24),
+                    value(x & 0x00f000f0u, s20));
 }
+
+// v * 2^n, n in -252 .. 254
+__device__ __forceinline__ float scaled(float v, int n) { return v * pow2(n >> 1) * pow2(n - (n >> 1)); }
 
 __device__ __forceinline__ bool finite_row(uint32_t p) {
   return fabsf(scale_of(p)) < INFINITY && fabsf(offset_of(p)) < INFINITY;  // neither for NaN
 }
-// exponent field of the larger of a row's two ends; 0 for a row that is not finite
+// How far a row reaches, as an exponent field: 2^(kReach - field) brings its values under 2^14 and its
+// scale times 2^24 under 2^15.  0 for a row that is not finite.
+constexpr int kReach = 140;
 __device__ __forceinline__ uint32_t reach(uint32_t p) {
-  const float o = offset_of(p), top = fmaxf(fabsf(o), fabsf(fmaf(15.0f, scale_of(p), o)));
-  return finite_row(p) ? min(__float_as_uint(top) >> 23, 254u) : 0u;
+  const float s = scale_of(p), o = offset_of(p), top = fmaxf(fabsf(o), fabsf(fmaf(15.0f, s, o)));
+  const uint32_t field = max(min(__float_as_uint(top) >> 23, 254u), (__float_as_uint(fabsf(s)) >> 23) + 23);
+  return finite_row(p) ? field : 0u;
 }
 
 template <int D, typename T>
@@ -203,7 +215,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   constexpr int kUnpack = 4 * TILES, kIssue = kUnpack + 4;  // first warps of their kind
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
-      s_full[TILES], p_full[TILES], o_full;
+      s_full[TILES], p_half[TILES], p_full[TILES], o_full;
   __shared__ uint32_t tensor_base;
   __shared__ int stalled_, found[2], sh_last;
   __shared__ Sequence sh_seq;
@@ -211,10 +223,9 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   __shared__ uint32_t top_k[2][4], top_v[2][4];
   volatile int* stalled = &stalled_;
   uint8_t* smem = raw + ((1024 - (smem_of(raw) & 1023)) & 1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all of a warp's threads, which the compiler sees by the shuffle
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int heads = a.pool.kv_heads;
-
-  zero_unowned<T>(a, D, blockIdx.x * (int64_t)(P::WARPS * 32) + threadIdx.x, (int64_t)gridDim.x * P::WARPS * 32);
 
   // ---- this block's sequence, row tiles and head; the later tiles of a sequence, which see more,
   // come first
@@ -257,13 +268,21 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     }
     for (int i = 0; i < TILES; ++i) {
       bar_init(&s_full[i], 1);
+      bar_init(&p_half[i], kTile);
       bar_init(&p_full[i], kTile);
     }
     bar_init(&o_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  if (found[0] < 0) return;
+  // the queries that nobody has, by blocks that are done or have nothing else to do
+  auto zero_rest = [&]() {
+    zero_unowned<T>(a, D, blockIdx.x * (int64_t)(P::WARPS * 32) + threadIdx.x, (int64_t)gridDim.x * P::WARPS * 32);
+  };
+  if (found[0] < 0) {
+    zero_rest();
+    return;
+  }
   const int b = found[0];
   const Sequence seq = sh_seq;
   const int row0 = found[1] * RT, rows = min(RT, seq.count * (int)a.group.d - row0);
@@ -273,18 +292,19 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   const int all_steps = max(0, (reach_end + kTile - 1) / kTile);
   const int share = max(kLeastSteps, (all_steps + split.splits - 1) / split.splits);
   const int parts = max(1, (all_steps + share - 1) / share);
-  if (part >= parts) return;
+  if (part >= parts) {
+    zero_rest();
+    return;
+  }
   const int step0 = part * share, steps = min(share, all_steps - step0);  // this block's
 
-  if (warp == kIssue) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&tensor_base))
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  // Each group begins with what needs no tensor memory, then waits for its address.
+  auto tensor_memory = [&]() {
     fence_before();
-  }
-  __syncthreads();
-  fence_after();
-  const uint32_t tensor = tensor_base;
+    __syncthreads();
+    fence_after();
+    return tensor_base;
+  };
 
   if (warp < kUnpack) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::SOFTMAX_REGS));
@@ -293,52 +313,57 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     const bool live = row < rows;
     const int i = a.group.div(row0 + (live ? row : 0)), h = head * a.group.d + (row0 + (live ? row : 0) - i * a.group.d);
     const int seen = !live ? 0 : (a.causal ? min(seq.length, ahead + i) : seq.length);
-    float factor;  // scores are `factor` and the step's factor times the product, in powers of two
-    {
-      const T* src = static_cast<const T*>(a.q) + (int64_t)(seq.start + i) * a.q_ts + h * a.q_hs;
-      float top = 0.0f;
-      // twice over the row: its largest, then its values
+    // The warp loads its 32 rows together, LANES lanes a row with 8 channels each: first as they are
+    // into their places, then from there as float16.  Short loops: this code runs once a block, and
+    // fetching it costs more than running it.
+    constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+    const int c = lane % LANES, of = lane / LANES;
+    uint8_t* const place = smem + P::Q + tile * P::ROWS + (c >> 3) * P::BLOCK;
 #pragma unroll 1
-      for (int pass = 0; pass < 2; ++pass) {
-        const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));
-        const float up = a.scale_log2 < 0.0f ? -pow2(e) : pow2(e);
-        factor = fabsf(a.scale_log2) * pow2(-e);
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          float x[8];
-          if (!live) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-          } else if (a.vec) {
-            const uint4 w = *reinterpret_cast<const uint4*>(src + c * 8);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = Half2<T>::unpack(u[k]);
-              x[2 * k] = f.x;
-              x[2 * k + 1] = f.y;
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = Half2<T>::load(src + c * 8 + k);
-          }
-          if (pass == 0) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
-          } else {  // channels in the order that codes unpack in
-            uint4 w;
-            w.x = Half2<__half>::pack(x[0] * up, x[4] * up);
-            w.y = Half2<__half>::pack(x[1] * up, x[5] * up);
-            w.z = Half2<__half>::pack(x[2] * up, x[6] * up);
-            w.w = Half2<__half>::pack(x[3] * up, x[7] * up);
-            *reinterpret_cast<uint4*>(smem + P::Q + tile * P::ROWS + (c >> 3) * P::BLOCK + r * 128 +
-                                      (((c & 7) ^ (r & 7)) << 4)) = w;
-          }
-        }
+    for (int n = 0; n < 32; n += AT_ONCE) {
+      const int rr = (warp & 3) * 32 + n + of;  // this lane's row of the tile
+      const int gr = row0 + tile * kTile + rr;
+      const bool there = tile * kTile + rr < rows;
+      const int qi = a.group.div(there ? gr : row0), qh = head * a.group.d + ((there ? gr : row0) - qi * a.group.d);
+      const T* src = static_cast<const T*>(a.q) + (int64_t)(seq.start + qi) * a.q_ts + qh * a.q_hs + c * 8;
+      uint8_t* dst = place + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+      if (a.vec) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(dst)), "l"(src), "r"(there ? 16 : 0)
+                     : "memory");
+      } else {
+        const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = there ? u[k] : (uint16_t)0;
       }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // each lane reads what it wrote
+    float factor = 0.0f;  // scores are `factor` and the step's factor times the product, in powers of two
+#pragma unroll 4
+    for (int n = 0; n < 32; n += AT_ONCE) {
+      const int rr = (warp & 3) * 32 + n + of;
+      uint4* at = reinterpret_cast<uint4*>(place + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+      const uint4 x = *at;
+      const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
+                   f3 = Half2<T>::unpack(x.w);
+      float top = fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                        fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));
+      const float up = a.scale_log2 < 0.0f ? -pow2(e) : pow2(e);
+      uint4 w;  // channels in the order that codes unpack in
+      w.x = Half2<__half>::pack(f0.x * up, f2.x * up);
+      w.y = Half2<__half>::pack(f0.y * up, f2.y * up);
+      w.z = Half2<__half>::pack(f1.x * up, f3.x * up);
+      w.w = Half2<__half>::pack(f1.y * up, f3.y * up);
+      *at = w;
+      // the row's own thread is lane n + of
+      const float down = __shfl_sync(0xffffffffu, pow2(-e), ((lane - n) & (AT_ONCE - 1)) * LANES);
+      if (lane >= n && lane < n + AT_ONCE) factor = fabsf(a.scale_log2) * down;
     }
     fence_smem();
     bar_arrive(&q_full);
+    const uint32_t tensor = tensor_memory();
 
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 rows of tensor memory
     const uint32_t s_at = tensor + lanes + tile * P::S_COLUMNS, o_at = tensor + lanes + P::O + tile * D;
@@ -350,7 +375,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       __syncwarp();
       fence_after();
       const Info& info = infos[j & (kInfos - 1)];
-      const float f = factor * info.key_factor;
+      const float f = scaled(factor, -info.key_shift);
       const int now = info.value_shift;
       const bool special = (info.hidden[0] | info.hidden[1] | info.hidden[2] | info.hidden[3] | info.bad[0] |
                             info.bad[1] | info.bad[2] | info.bad[3]) != 0;
@@ -424,6 +449,11 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
             p[k] = Half2<__half>::pack(e0, e1);
           }
           store16(p, s_at + w * 16);  // over the scores
+          if (w == 1) {  // the first half of the second product may start
+            stored();
+            fence_before();
+            bar_arrive(&p_half[tile]);
+          }
         }
       };
       if (masked) weigh(std::true_type{});
@@ -440,7 +470,6 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       fence_after();
     }
     const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
-    const float back = pow2(max(-126, min(127, -shift)));
     if (poisoned) l = __int_as_float(0x7fffffff);
     // 8 channels of the row, unpacking's order undone
     auto write8 = [&](int d, const float (&v)[8], float k) {
@@ -452,7 +481,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + d) = w;
     };
     const int64_t mine = (int64_t)tile_head * split.splits + part;
-    const float k = l == 0.0f ? 0.0f : back / l;
+    const float k = l == 0.0f ? 0.0f : scaled(1.0f / l, -shift);
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t x[32];
@@ -474,8 +503,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
             write8(c + g * 8, v, k);
           } else {
             float4* to = split.parts + (mine * (D / 4) + c / 4 + g * 2) * RT + row;
-            to[0] = make_float4(v[0] * back, v[1] * back, v[2] * back, v[3] * back);
-            to[RT] = make_float4(v[4] * back, v[5] * back, v[6] * back, v[7] * back);
+            to[0] = make_float4(scaled(v[0], -shift), scaled(v[1], -shift), scaled(v[2], -shift), scaled(v[3], -shift));
+            to[RT] = make_float4(scaled(v[4], -shift), scaled(v[5], -shift), scaled(v[6], -shift), scaled(v[7], -shift));
           }
         }
       }
@@ -568,8 +597,10 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         for (int c = 0; c < D / 32; ++c) vc[c] = make_uint4(0, 0, 0, 0);
       }
     };
-    auto spread = [&](const uint4 (&codes)[D / 32], float scale, float offset, uint8_t* dst) {
-      const __half2 s = __float2half2_rn(scale), o = __float2half2_rn(offset);
+    auto spread = [&](const uint4 (&codes)[D / 32], uint32_t p, int shift, uint8_t* dst) {
+      const float scale = scaled(scale_of(p), shift);
+      const __half2 s24 = __float2half2_rn(scale * 16777216.0f), s20 = __float2half2_rn(scale * 1048576.0f),
+                    o = __float2half2_rn(scaled(offset_of(p), shift));
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         const uint32_t w[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
@@ -577,7 +608,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         for (int k = 0; k < 4; ++k) {
           const int chunk = c * 4 + k;
           *reinterpret_cast<uint4*>(dst + (chunk >> 3) * P::BLOCK + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) =
-              unpack8(w[k], s, o);
+              unpack8(w[k], s24, s20, o);
         }
       }
     };
@@ -585,6 +616,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     fetch_keys(0);
     fetch_values();
     look_up(1);
+    tensor_memory();
     uint32_t value_top = 27;  // exponent field of the largest value so far
     for (int j = 0; j < steps; ++j) {
       const int stage = j % STAGES;
@@ -604,79 +636,110 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         key_top = max(key_top, top_k[j & 1][w]);
         value_top = max(value_top, top_v[j & 1][w]);
       }
-      const int key_shift = 140 - (int)key_top, value_shift = 140 - (int)value_top;  // under 2^14
+      const int key_shift = kReach - (int)key_top, value_shift = kReach - (int)value_top;
       bar_wait(&k_empty[stage], filled ^ 1, stalled);
       Info& info = infos[j & (kInfos - 1)];
       if (t == 0) {
-        info.key_factor = pow2(-key_shift);
+        info.key_shift = key_shift;
         info.value_shift = value_shift;
       }
       if (lane == 0) {
         info.hidden[warp - kUnpack] = hidden;
         info.bad[warp - kUnpack] = wrong;
       }
-      spread(kc, scale_of(kp) * pow2(key_shift), offset_of(kp) * pow2(key_shift), smem + P::K + stage * P::ROWS);
+      spread(kc, kp, key_shift, smem + P::K + stage * P::ROWS);
       fence_smem();
       bar_arrive(&k_full[stage]);
-      const float vs = bad || state != 1 ? 0.0f : scale_of(vp) * pow2(value_shift);
-      const float vo = bad || state != 1 ? 0.0f : offset_of(vp) * pow2(value_shift);
+      const uint32_t value_params = bad ? 0 : vp;  // a value that is not finite is left to its rows
       fetch_keys(j + 1);
       look_up(j + 2);
       bar_wait(&v_empty[stage], filled ^ 1, stalled);
-      spread(vc, vs, vo, smem + P::V + stage * P::ROWS);
+      spread(vc, value_params, value_shift, smem + P::V + stage * P::ROWS);
       fence_smem();
       bar_arrive(&v_full[stage]);
       fetch_values();
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::ISSUE_REGS));
-    if (warp == kIssue && lane == 0 && steps > 0) {
-    // ---------------------------------------------------------------- products
-    const uint32_t base = smem_of(smem);
-    constexpr uint32_t id_s = instruction(kTile, false), id_o = instruction(D, true);
-    auto scores = [&](int tile, int stage) {
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t in = (k >> 2) * P::BLOCK + (k & 3) * 32;
-        mma_ss(tensor + tile * P::S_COLUMNS, operand(base + P::Q + tile * P::ROWS + in, 16),
-               operand(base + P::K + stage * P::ROWS + in, 16), id_s, k > 0);
-      }
-    };
-    auto values = [&](int tile, int stage, bool more) {
-#pragma unroll
-      for (int k = 0; k < kTile / 16; ++k)
-        mma_ts(tensor + P::O + tile * D, tensor + tile * P::S_COLUMNS + k * 8,
-               operand(base + P::V + stage * P::ROWS + k * 2048, P::BLOCK), id_o, more || k > 0);
-    };
-    bar_wait(&q_full, 0, stalled);
-    bar_wait(&k_full[0], 0, stalled);
-    fence_after();
-    for (int tile = 0; tile < TILES; ++tile) {
-      scores(tile, 0);
-      commit(&s_full[tile]);
+    if (warp == kIssue) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&tensor_base))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    commit(&k_empty[0]);
-    for (int j = 0; j < steps; ++j) {
-      const int stage = j % STAGES, next = (j + 1) % STAGES;
-      const uint32_t filled = (uint32_t)(j / STAGES) & 1, next_filled = (uint32_t)((j + 1) / STAGES) & 1;
-      bar_wait(&v_full[stage], filled, stalled);
-      if (j + 1 < steps) bar_wait(&k_full[next], next_filled, stalled);
-      for (int tile = 0; tile < TILES; ++tile) {
-        bar_wait(&p_full[tile], j & 1, stalled);
-        fence_after();
-        values(tile, stage, j > 0);
-        if (tile == TILES - 1) commit(&v_empty[stage]);
-        if (j + 1 < steps) {
-          scores(tile, next);
+    const uint32_t tensor = tensor_memory();
+    if (warp == kIssue && steps > 0) {
+      // ---------------------------------------------------------------- products
+      // The whole warp walks along, so that operands stay in uniform registers; one thread issues.
+      const uint32_t base = smem_of(smem), into = __shfl_sync(0xffffffffu, tensor, 0);
+      constexpr uint32_t id_s = instruction(kTile, false), id_o = instruction(D, true);
+      const uint64_t q_at = operand(base + P::Q, 16), k_at = operand(base + P::K, 16),
+                     v_at = operand(base + P::V, P::BLOCK);
+      const bool one = elected();
+      auto scores = [&](int tile, int stage) {
+        const uint64_t q = q_at + tile * (P::ROWS >> 4), k = k_at + stage * (P::ROWS >> 4);
+        if (one) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const int in = ((i >> 2) * P::BLOCK + (i & 3) * 32) >> 4;
+            mma_ss(into + tile * P::S_COLUMNS, q + in, k + in, id_s, i > 0);
+          }
           commit(&s_full[tile]);
         }
+        __syncwarp();
+      };
+      // half of a step's tokens
+      auto values = [&](int tile, int stage, int half, bool more) {
+        const uint64_t v = v_at + stage * (P::ROWS >> 4);
+        if (one) {
+#pragma unroll
+          for (int i = 0; i < kTile / 32; ++i) {
+            const int k = half * (kTile / 32) + i;
+            mma_ts(into + P::O + tile * D, into + tile * P::S_COLUMNS + k * 8, v + k * (2048 >> 4), id_o, more || i > 0);
+          }
+        }
+        __syncwarp();
+      };
+      bar_wait(&q_full, 0, stalled);
+      bar_wait(&k_full[0], 0, stalled);
+      fence_after();
+      scores(0, 0);
+      if (TILES == 2) {
+        // the tiles keep the distance that they start at: half a step, so that one's 2^x and the
+        // other's products run at the same time
+        bar_wait(&p_half[0], 0, stalled);
+        scores(1, 0);
       }
-      if (j + 1 < steps) commit(&k_empty[next]);
-    }
-    commit(&o_full);
-    // nothing is in flight when the tensor memory is given back, even after a wait that ran out
-    volatile int late = 0;
-    bar_wait(&o_full, 0, &late);
+      if (one) commit(&k_empty[0]);
+      int stage = 0;
+      uint32_t filled = 0;
+#pragma unroll 1
+      for (int j = 0; j < steps; ++j) {
+        const int next = stage + 1 == STAGES ? 0 : stage + 1;
+        const uint32_t next_filled = filled ^ (next == 0);
+        bar_wait(&v_full[stage], filled, stalled);
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+          bar_wait(&p_half[tile], j & 1, stalled);
+          fence_after();
+          values(tile, stage, 0, j > 0);
+          bar_wait(&p_full[tile], j & 1, stalled);
+          fence_after();
+          values(tile, stage, 1, true);
+          if (one && tile == TILES - 1) commit(&v_empty[stage]);
+          if (j + 1 < steps) {
+            if (tile == 0) bar_wait(&k_full[next], next_filled, stalled);
+            fence_after();
+            scores(tile, next);
+          }
+        }
+        if (one && j + 1 < steps) commit(&k_empty[next]);
+        stage = next;
+        filled = next_filled;
+      }
+      if (one) commit(&o_full);
+      // nothing is in flight when the tensor memory is given back, even after a wait that ran out
+      volatile int late = 0;
+      bar_wait(&o_full, 0, &late);
     }
   }
   fence_before();
@@ -685,8 +748,9 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   if (warp == kIssue) {
     __syncwarp();
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tensor));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tensor_base));
   }
+  zero_rest();
 }
 
 // Row tiles times heads, at most: one tile that is not full for each sequence that has queries.

@@ -11,7 +11,8 @@
 //                   the swizzled rows that the tensor cores read (keys K-major; the same rows of
 //                   values are an MN-major operand, so nothing is transposed);
 //   one warp        issues S = Q K^T (both from shared memory) and O += P V (P from tensor memory).
-// The two row tiles take turns: while one's weights are computed the other's products run.
+// Scores come 64 tokens at a time into two places of each tile in turn, so the softmax of one half step
+// runs while the products of the half steps around it do, and waits for none of them.
 //
 // Where there are fewer such row tiles than SMs, several blocks share the tokens of each, leave their
 // sums in the workspace, and the last of them joins them in the order of the tokens.
@@ -33,6 +34,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kTile = 128;  // rows of a tile, tokens of a step
+constexpr int kHalf = 64;   // tokens of a half step
 constexpr float kSlack = 8.0f;
 constexpr int kInfos = 4;   // steps whose factors are kept: the unpacking warps run at most 2 ahead
 constexpr int kTries = 1 << 20;
@@ -41,13 +43,13 @@ template <int D>
 struct Plan {
   static constexpr int TILES = D == 256 ? 1 : 2;   // row tiles of a block
   static constexpr int STAGES = D == 256 ? 1 : 2;  // steps of unpacked keys and values
-  static constexpr int WARPS = 4 * TILES + 4 + 4;  // a warpgroup each for a row tile, unpacking, and issuing (one warp)
-  // Registers of a thread, moved from the groups that need few; each group's share comes out of the
-  // launch's 512 (of 384 threads: 504) for the four warps that an SM's quarter holds.
-  static constexpr int LAUNCH_REGS = D == 256 ? 168 : 128;
-  static constexpr int SOFTMAX_REGS = D == 256 ? 240 : 192, UNPACK_REGS = D == 256 ? 192 : 96,
-                       ISSUE_REGS = D == 256 ? 40 : 32;
-  static_assert(TILES * SOFTMAX_REGS + UNPACK_REGS + ISSUE_REGS <= LAUNCH_REGS * WARPS / 4, "a wait without end");
+  // a warpgroup for each row tile, two for unpacking, one for issuing (of which one warp works)
+  static constexpr int UNPACK = 4 * TILES, ISSUE = UNPACK + 8, WARPS = ISSUE + 4;
+  // Registers of a thread, moved to the groups that need more.  What the groups' threads hold together
+  // must not be more than the launch gave them.
+  static constexpr int LAUNCH_REGS = TILES == 2 ? 96 : 128;
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 136 : 200, UNPACK_REGS = TILES == 2 ? 72 : 112, ISSUE_REGS = 40;
+  static_assert(UNPACK * SOFTMAX_REGS + 8 * UNPACK_REGS + 4 * ISSUE_REGS <= WARPS * LAUNCH_REGS, "a wait without end");
   static constexpr int BLOCK = kTile * 128;        // bytes of 64 channels of 128 rows
   static constexpr int ROWS = BLOCK * (D / 64);    // bytes of 128 rows
   static constexpr int Q = 0, K = ROWS * TILES, V = K + ROWS * STAGES, END = V + ROWS * STAGES;
@@ -141,6 +143,27 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
+// Two float products and sums in one instruction.
+__device__ __forceinline__ uint64_t pair(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)), "l"(pair(c)));
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+
 #define TANS_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
 #define TANS_W4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
 // 32 columns of this warp's 32 rows: a thread has its row's
@@ -212,10 +235,10 @@ template <int D, typename T>
 __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a, const Split split) {
   using P = Plan<D>;
   constexpr int TILES = P::TILES, STAGES = P::STAGES, RT = kTile * TILES;
-  constexpr int kUnpack = 4 * TILES, kIssue = kUnpack + 4;  // first warps of their kind
+  constexpr int kUnpack = P::UNPACK, kIssue = P::ISSUE;  // first warps of their kind
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
-      s_full[TILES], p_half[TILES], p_full[TILES], o_full;
+      s_full[TILES][2], p_full[TILES][2], o_done[TILES], o_full;
   __shared__ uint32_t tensor_base;
   __shared__ int stalled_, found[2], sh_last;
   __shared__ Sequence sh_seq;
@@ -261,15 +284,17 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     stalled_ = 0;
     bar_init(&q_full, kTile * TILES);
     for (int i = 0; i < STAGES; ++i) {
-      bar_init(&k_full[i], kTile);
-      bar_init(&v_full[i], kTile);
+      bar_init(&k_full[i], 2 * kTile);
+      bar_init(&v_full[i], 2 * kTile);
       bar_init(&k_empty[i], 1);
       bar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < TILES; ++i) {
-      bar_init(&s_full[i], 1);
-      bar_init(&p_half[i], kTile);
-      bar_init(&p_full[i], kTile);
+      for (int h = 0; h < 2; ++h) {
+        bar_init(&s_full[i][h], 1);
+        bar_init(&p_full[i][h], kTile);
+      }
+      bar_init(&o_done[i], 1);
     }
     bar_init(&o_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -297,6 +322,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     return;
   }
   const int step0 = part * share, steps = min(share, all_steps - step0);  // this block's
+  const int halves = min(2 * steps, (reach_end + kHalf - 1) / kHalf - 2 * step0);
 
   // Each group begins with what needs no tensor memory, then waits for its address.
   auto tensor_memory = [&]() {
@@ -313,53 +339,57 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     const bool live = row < rows;
     const int i = a.group.div(row0 + (live ? row : 0)), h = head * a.group.d + (row0 + (live ? row : 0) - i * a.group.d);
     const int seen = !live ? 0 : (a.causal ? min(seq.length, ahead + i) : seq.length);
-    // The warp loads its 32 rows together, LANES lanes a row with 8 channels each: first as they are
-    // into their places, then from there as float16.  Short loops: this code runs once a block, and
-    // fetching it costs more than running it.
+    // The warp copies its 32 rows as they are into their places, LANES lanes a row; then each thread
+    // brings its own row to float16.  Short loops: this code runs once a block, and fetching long code
+    // costs more than running it.
     constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
-    const int c = lane % LANES, of = lane / LANES;
-    uint8_t* const place = smem + P::Q + tile * P::ROWS + (c >> 3) * P::BLOCK;
+    uint8_t* const q_tile = smem + P::Q + tile * P::ROWS;
+    {
+      const T* row_at = static_cast<const T*>(a.q) + (int64_t)(seq.start + i) * a.q_ts + h * a.q_hs;
+      const int c = lane % LANES;
+#pragma unroll 4
+      for (int n = lane / LANES; n < 32; n += AT_ONCE) {
+        const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(row_at), n)) + c * 8;
+        const bool there = row - lane + n < rows;
+        const int rr = (warp & 3) * 32 + n;
+        uint8_t* dst = q_tile + (c >> 3) * P::BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+        if (a.vec) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(dst)), "l"(src), "r"(there ? 16 : 0)
+                       : "memory");
+        } else {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll 1
-    for (int n = 0; n < 32; n += AT_ONCE) {
-      const int rr = (warp & 3) * 32 + n + of;  // this lane's row of the tile
-      const int gr = row0 + tile * kTile + rr;
-      const bool there = tile * kTile + rr < rows;
-      const int qi = a.group.div(there ? gr : row0), qh = head * a.group.d + ((there ? gr : row0) - qi * a.group.d);
-      const T* src = static_cast<const T*>(a.q) + (int64_t)(seq.start + qi) * a.q_ts + qh * a.q_hs + c * 8;
-      uint8_t* dst = place + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-      if (a.vec) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(dst)), "l"(src), "r"(there ? 16 : 0)
-                     : "memory");
-      } else {
-        const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll 1
-        for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = there ? u[k] : (uint16_t)0;
+          for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = there ? u[k] : (uint16_t)0;
+        }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");  // each lane reads what it wrote
-    float factor = 0.0f;  // scores are `factor` and the step's factor times the product, in powers of two
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    float top_q = 0.0f;
 #pragma unroll 4
-    for (int n = 0; n < 32; n += AT_ONCE) {
-      const int rr = (warp & 3) * 32 + n + of;
-      uint4* at = reinterpret_cast<uint4*>(place + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (c >> 3) * P::BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
+                   f3 = Half2<T>::unpack(x.w);
+      top_q = fmaxf(top_q, fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                                 fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y)))));
+    }
+    const int e_q = 13 - max(-87, min(116, (int)(__float_as_uint(top_q) >> 23) - 127));
+    const float up = a.scale_log2 < 0.0f ? -pow2(e_q) : pow2(e_q);
+    // scores are `factor` and the step's factor times the product, in powers of two
+    const float factor = fabsf(a.scale_log2) * pow2(-e_q);
+#pragma unroll 4
+    for (int c = 0; c < D / 8; ++c) {
+      uint4* at = reinterpret_cast<uint4*>(q_tile + (c >> 3) * P::BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
       const uint4 x = *at;
       const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
                    f3 = Half2<T>::unpack(x.w);
-      float top = fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
-                        fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
-#pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));
-      const float up = a.scale_log2 < 0.0f ? -pow2(e) : pow2(e);
       uint4 w;  // channels in the order that codes unpack in
       w.x = Half2<__half>::pack(f0.x * up, f2.x * up);
       w.y = Half2<__half>::pack(f0.y * up, f2.y * up);
       w.z = Half2<__half>::pack(f1.x * up, f3.x * up);
       w.w = Half2<__half>::pack(f1.y * up, f3.y * up);
       *at = w;
-      // the row's own thread is lane n + of
-      const float down = __shfl_sync(0xffffffffu, pow2(-e), ((lane - n) & (AT_ONCE - 1)) * LANES);
-      if (lane >= n && lane < n + AT_ONCE) factor = fabsf(a.scale_log2) * down;
     }
     fence_smem();
     bar_arrive(&q_full);
@@ -370,42 +400,51 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     float m = -INFINITY, l = 0.0f;
     bool poisoned = false;
     int shift = 0;
-    for (int j = 0; j < steps; ++j) {
-      bar_wait(&s_full[tile], j & 1, stalled);
+    uint32_t x[2][32];
+    auto scores_of = [&](int n) {  // half step n's are there
+      bar_wait(&s_full[tile][n & 1], (n >> 1) & 1, stalled);
       __syncwarp();
       fence_after();
+    };
+    if (halves > 0) {
+      scores_of(0);
+      load32(x[0], s_at);
+      load32(x[1], s_at + 32);
+    }
+#pragma unroll 1
+    for (int n = 0; n < halves; ++n) {
+      const int j = n >> 1, h = n & 1;
+      const uint32_t at = s_at + h * kHalf, at_next = s_at + (h ^ 1) * kHalf;
       const Info& info = infos[j & (kInfos - 1)];
       const float f = scaled(factor, -info.key_shift);
       const int now = info.value_shift;
-      const bool special = (info.hidden[0] | info.hidden[1] | info.hidden[2] | info.hidden[3] | info.bad[0] |
-                            info.bad[1] | info.bad[2] | info.bad[3]) != 0;
-      const int left = seen - (step0 + j) * kTile;  // tokens of this step that the row sees
-      const bool masked = __any_sync(0xffffffffu, left < kTile) || special;
-      uint32_t x[4][32];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) load32(x[w], s_at + w * 32);
+      const bool special = (info.hidden[2 * h] | info.hidden[2 * h + 1] | info.bad[2 * h] | info.bad[2 * h + 1]) != 0;
+      const int left = seen - (step0 + j) * kTile - h * kHalf;  // tokens of this half step that the row sees
+      const bool masked = __any_sync(0xffffffffu, left < kHalf) || special;
       loaded();
-#pragma unroll
-      for (int w = 0; w < 4; ++w) hold(x[w]);
-      uint32_t visible[4];
+      hold(x[0]);
+      hold(x[1]);
+      uint32_t visible[2];
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (masked) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int n = left - w * 32;
-          visible[w] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1);
+        for (int w = 0; w < 2; ++w) {
+          const int some = left - w * 32;
+          visible[w] = some >= 32 ? 0xffffffffu : (some <= 0 ? 0u : (1u << some) - 1);
           if (special) {
-            visible[w] &= ~info.hidden[w];
-            poisoned |= (visible[w] & info.bad[w]) != 0;
+            visible[w] &= ~info.hidden[2 * h + w];
+            poisoned |= (visible[w] & info.bad[2 * h + w]) != 0;
           }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) tops[k & 3] = visible[w] >> k & 1 ? fmaxf(tops[k & 3], __uint_as_float(x[w][k])) : tops[k & 3];
+          for (int k = 0; k < 32; ++k)
+            tops[k & 3] = visible[w] >> k & 1 ? fmaxf(tops[k & 3], __uint_as_float(x[w][k])) : tops[k & 3];
         }
       } else {
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int k = 0; k < 32; ++k) tops[k & 3] = fmaxf(tops[k & 3], __uint_as_float(x[w][k]));
+          for (int k = 0; k < 32; k += 2)
+            tops[k / 2 & 3] = fmaxf(fmaxf(__uint_as_float(x[w][k]), __uint_as_float(x[w][k + 1])), tops[k / 2 & 3]);
       }
       float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       top = top == -INFINITY ? top : top * f;
@@ -414,7 +453,10 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       if (__any_sync(0xffffffffu, moves || now != shift)) {
         const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
         l *= keep;
-        if (j > 0) {  // O is not yet written before the first step
+        if (n > 0) {  // O is not yet written before the first half step, and at rest after the last one's
+          bar_wait(&o_done[tile], (n - 1) & 1, stalled);
+          __syncwarp();
+          fence_after();
           const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
@@ -431,37 +473,39 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       m = next;
       shift = now;
       const float base = m == -INFINITY ? 0.0f : m;
-      float sums[2] = {0.0f, 0.0f};
+      float2 sum = make_float2(0.0f, 0.0f);
+      // Weights of 32 tokens, put over the scores; two at a time where the hardware has it.  The next
+      // scores take the registers of those that are done, so that they come while others are worked on.
       auto weigh = [&](auto masked_) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 2; ++w) {
           uint32_t p[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            float e0 = ex2(fmaf(__uint_as_float(x[w][2 * k]), f, -base));
-            float e1 = ex2(fmaf(__uint_as_float(x[w][2 * k + 1]), f, -base));
+            float2 e = fma2(make_float2(__uint_as_float(x[w][2 * k]), __uint_as_float(x[w][2 * k + 1])),
+                            make_float2(f, f), make_float2(-base, -base));
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
             if constexpr (decltype(masked_)::value) {
-              e0 = visible[w] >> (2 * k) & 1 ? e0 : 0.0f;
-              e1 = visible[w] >> (2 * k + 1) & 1 ? e1 : 0.0f;
+              e.x = visible[w] >> (2 * k) & 1 ? e.x : 0.0f;
+              e.y = visible[w] >> (2 * k + 1) & 1 ? e.y : 0.0f;
             }
-            sums[0] += e0;
-            sums[1] += e1;
-            p[k] = Half2<__half>::pack(e0, e1);
+            sum = add2(sum, e);
+            p[k] = Half2<__half>::pack(e.x, e.y);
           }
-          store16(p, s_at + w * 16);  // over the scores
-          if (w == 1) {  // the first half of the second product may start
-            stored();
-            fence_before();
-            bar_arrive(&p_half[tile]);
+          store16(p, at + w * 16);
+          if (n + 1 < halves) {
+            if (w == 0) scores_of(n + 1);
+            load32(x[w], at_next + w * 32);
           }
         }
       };
       if (masked) weigh(std::true_type{});
       else weigh(std::false_type{});
-      l += sums[0] + sums[1];
+      l += sum.x + sum.y;
       stored();
       fence_before();
-      bar_arrive(&p_full[tile]);
+      bar_arrive(&p_full[tile][h]);
     }
     // ---- the rows' results
     if (steps > 0) {
@@ -552,11 +596,12 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   } else if (warp < kIssue) {
     if constexpr (P::UNPACK_REGS > P::LAUNCH_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
-    // ---------------------------------------------------------------- unpacking: a token of a step
-    const int t = threadIdx.x - kUnpack * 32;
+    // ---------------------------------------------------------------- unpacking: half a token's row
+    constexpr int CODES = D / 64;  // 16 bytes each of a thread's keys or values
+    const int quarter = (warp - kUnpack) & 3, t = quarter * 32 + lane, part_of_row = (warp - kUnpack) >> 2;
     const int32_t* table = a.pages + (int64_t)b * a.max_pages;
     const int64_t side_rows = (int64_t)heads * a.pool.page_size;
-    uint4 kc[D / 32], vc[D / 32];
+    uint4 kc[CODES], vc[CODES];
     uint32_t kp = 0, vp = 0;
     int page = -1, state = 0;  // 0: past the end, 1: a row of the cache, 2: hidden
     auto look_up = [&](int j) {
@@ -574,39 +619,39 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
           const int64_t at = a.pool.row(page, 0, head) + (token - a.page_size.div(token) * a.pool.page_size);
           kp = __ldg(a.pool.params + at);
           vp = __ldg(a.pool.params + at + side_rows);
-          from = a.pool.codes + at * (D / 2);
+          from = a.pool.codes + at * (D / 2) + part_of_row * (D / 4);
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) kc[c] = __ldg(reinterpret_cast<const uint4*>(from) + c);
+          for (int c = 0; c < CODES; ++c) kc[c] = __ldg(reinterpret_cast<const uint4*>(from) + c);
         } else {
           state = 2;
-          flag(a.status, TANS_DEV_BAD_INDEX);
+          if (part_of_row == 0) flag(a.status, TANS_DEV_BAD_INDEX);
         }
       }
       if (state != 1) {
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) kc[c] = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < CODES; ++c) kc[c] = make_uint4(0, 0, 0, 0);
       }
     };
     auto fetch_values = [&]() {
       if (state == 1) {
         const uint4* src = reinterpret_cast<const uint4*>(from + side_rows * (D / 2));
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) vc[c] = __ldg(src + c);
+        for (int c = 0; c < CODES; ++c) vc[c] = __ldg(src + c);
       } else {
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) vc[c] = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < CODES; ++c) vc[c] = make_uint4(0, 0, 0, 0);
       }
     };
-    auto spread = [&](const uint4 (&codes)[D / 32], uint32_t p, int shift, uint8_t* dst) {
+    auto spread = [&](const uint4 (&codes)[CODES], uint32_t p, int shift, uint8_t* dst) {
       const float scale = scaled(scale_of(p), shift);
       const __half2 s24 = __float2half2_rn(scale * 16777216.0f), s20 = __float2half2_rn(scale * 1048576.0f),
                     o = __float2half2_rn(scaled(offset_of(p), shift));
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < CODES; ++c) {
         const uint32_t w[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int chunk = c * 4 + k;
+          const int chunk = (part_of_row * CODES + c) * 4 + k;
           *reinterpret_cast<uint4*>(dst + (chunk >> 3) * P::BLOCK + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) =
               unpack8(w[k], s24, s20, o);
         }
@@ -623,13 +668,13 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       const uint32_t filled = (uint32_t)(j / STAGES) & 1;
       // the largest key and value, over the step
       const uint32_t wk = __reduce_max_sync(0xffffffffu, reach(kp)), wv = __reduce_max_sync(0xffffffffu, reach(vp));
-      if (lane == 0) {
-        top_k[j & 1][warp - kUnpack] = wk;
-        top_v[j & 1][warp - kUnpack] = wv;
+      if (lane == 0 && part_of_row == 0) {
+        top_k[j & 1][quarter] = wk;
+        top_v[j & 1][quarter] = wv;
       }
       const bool bad = state == 1 && !finite_row(vp);
       const uint32_t hidden = __ballot_sync(0xffffffffu, state == 2), wrong = __ballot_sync(0xffffffffu, bad);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       uint32_t key_top = 27;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -639,13 +684,11 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       const int key_shift = kReach - (int)key_top, value_shift = kReach - (int)value_top;
       bar_wait(&k_empty[stage], filled ^ 1, stalled);
       Info& info = infos[j & (kInfos - 1)];
-      if (t == 0) {
-        info.key_shift = key_shift;
+      if (lane == 0 && part_of_row == 0) {
+        info.key_shift = key_shift;  // the same in all
         info.value_shift = value_shift;
-      }
-      if (lane == 0) {
-        info.hidden[warp - kUnpack] = hidden;
-        info.bad[warp - kUnpack] = wrong;
+        info.hidden[quarter] = hidden;
+        info.bad[quarter] = wrong;
       }
       spread(kc, kp, key_shift, smem + P::K + stage * P::ROWS);
       fence_smem();
@@ -671,70 +714,71 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       // ---------------------------------------------------------------- products
       // The whole warp walks along, so that operands stay in uniform registers; one thread issues.
       const uint32_t base = smem_of(smem), into = __shfl_sync(0xffffffffu, tensor, 0);
-      constexpr uint32_t id_s = instruction(kTile, false), id_o = instruction(D, true);
+      constexpr uint32_t id_s = instruction(kHalf, false), id_o = instruction(D, true);
+      constexpr int HALF = kHalf * 128 >> 4, STAGE = P::ROWS >> 4;  // of an operand's address
       const uint64_t q_at = operand(base + P::Q, 16), k_at = operand(base + P::K, 16),
                      v_at = operand(base + P::V, P::BLOCK);
       const bool one = elected();
-      auto scores = [&](int tile, int stage) {
-        const uint64_t q = q_at + tile * (P::ROWS >> 4), k = k_at + stage * (P::ROWS >> 4);
+      auto scores = [&](int tile, int stage, int h) {
+        const uint64_t q = q_at + tile * STAGE, k = k_at + stage * STAGE + h * HALF;
         if (one) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             const int in = ((i >> 2) * P::BLOCK + (i & 3) * 32) >> 4;
-            mma_ss(into + tile * P::S_COLUMNS, q + in, k + in, id_s, i > 0);
+            mma_ss(into + tile * P::S_COLUMNS + h * kHalf, q + in, k + in, id_s, i > 0);
           }
-          commit(&s_full[tile]);
+          commit(&s_full[tile][h]);
         }
         __syncwarp();
       };
-      // half of a step's tokens
-      auto values = [&](int tile, int stage, int half, bool more) {
-        const uint64_t v = v_at + stage * (P::ROWS >> 4);
+      auto values = [&](int tile, int stage, int h, bool more) {
+        const uint64_t v = v_at + stage * STAGE + h * HALF;
         if (one) {
 #pragma unroll
-          for (int i = 0; i < kTile / 32; ++i) {
-            const int k = half * (kTile / 32) + i;
-            mma_ts(into + P::O + tile * D, into + tile * P::S_COLUMNS + k * 8, v + k * (2048 >> 4), id_o, more || i > 0);
-          }
+          for (int i = 0; i < kHalf / 16; ++i)
+            mma_ts(into + P::O + tile * D, into + tile * P::S_COLUMNS + h * kHalf + i * 8, v + i * (2048 >> 4), id_o,
+                   more || i > 0);
+          commit(&o_done[tile]);
         }
         __syncwarp();
       };
       bar_wait(&q_full, 0, stalled);
       bar_wait(&k_full[0], 0, stalled);
       fence_after();
-      scores(0, 0);
-      if (TILES == 2) {
-        // the tiles keep the distance that they start at: half a step, so that one's 2^x and the
-        // other's products run at the same time
-        bar_wait(&p_half[0], 0, stalled);
-        scores(1, 0);
-      }
+#pragma unroll 1
+      for (int n = 0; n < min(2, halves); ++n)
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) scores(tile, 0, n);
       if (one) commit(&k_empty[0]);
       int stage = 0;
       uint32_t filled = 0;
 #pragma unroll 1
-      for (int j = 0; j < steps; ++j) {
-        const int next = stage + 1 == STAGES ? 0 : stage + 1;
-        const uint32_t next_filled = filled ^ (next == 0);
-        bar_wait(&v_full[stage], filled, stalled);
+      for (int n = 0; n < halves; ++n) {
+        const int h = n & 1, next = stage + 1 == STAGES ? 0 : stage + 1;
+        const uint32_t phase = (n >> 1) & 1, next_filled = filled ^ (next == 0);
+        if (h == 0) bar_wait(&v_full[stage], filled, stalled);
 #pragma unroll
         for (int tile = 0; tile < TILES; ++tile) {
-          bar_wait(&p_half[tile], j & 1, stalled);
+          bar_wait(&p_full[tile][h], phase, stalled);
           fence_after();
-          values(tile, stage, 0, j > 0);
-          bar_wait(&p_full[tile], j & 1, stalled);
-          fence_after();
-          values(tile, stage, 1, true);
-          if (one && tile == TILES - 1) commit(&v_empty[stage]);
-          if (j + 1 < steps) {
-            if (tile == 0) bar_wait(&k_full[next], next_filled, stalled);
-            fence_after();
-            scores(tile, next);
+          values(tile, stage, h, n > 0);
+          if (n + 2 < halves) {
+            if (h == 0 && tile == 0) {
+              bar_wait(&k_full[next], next_filled, stalled);
+              fence_after();
+            }
+            scores(tile, next, h);
           }
         }
-        if (one && j + 1 < steps) commit(&k_empty[next]);
-        stage = next;
-        filled = next_filled;
+        if (h == 1) {
+          if (one) {
+            commit(&v_empty[stage]);
+            commit(&k_empty[next]);
+          }
+          __syncwarp();
+          stage = next;
+          filled = next_filled;
+        }
       }
       if (one) commit(&o_full);
       // nothing is in flight when the tensor memory is given back, even after a wait that ran out

@@ -54,7 +54,6 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
   const size_t need = tans_kv4_attend_workspace_size(total_queries, q_heads, kv_heads, head_dim, batch, max_pages,
                                                      page_size, max_queries);
   void* ws = workspace;
-  if (need == 0) return launch_attend_prompt(a, dtype, nullptr, s);
   if (!ws) {
     if (cudaMallocAsync(&ws, need, s) != cudaSuccess) return TANS_E_CUDA;
     if (cudaMemsetAsync(ws, 0, Join::kArrivalBytes, s) != cudaSuccess) {

@@ -14,6 +14,9 @@
 // Scores come 64 tokens at a time into two places of each tile in turn, so the softmax of one half step
 // runs while the products of the half steps around it do, and waits for none of them.
 //
+// A block goes on to the next of its row tiles by itself: the unpacking warps are then already there,
+// and the next queries come while the last results leave.
+//
 // Where there are fewer such row tiles than SMs, several blocks share the tokens of each, leave their
 // sums in the workspace, and the last of them joins them in the order of the tokens.
 //
@@ -48,7 +51,8 @@ struct Plan {
   // Registers of a thread, moved to the groups that need more.  What the groups' threads hold together
   // must not be more than the launch gave them.
   static constexpr int LAUNCH_REGS = TILES == 2 ? 96 : 128;
-  static constexpr int SOFTMAX_REGS = TILES == 2 ? 136 : 200, UNPACK_REGS = TILES == 2 ? 72 : 112, ISSUE_REGS = 40;
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 144 : 240, UNPACK_REGS = TILES == 2 ? 72 : 112,
+                       ISSUE_REGS = TILES == 2 ? 48 : 40;
   static_assert(UNPACK * SOFTMAX_REGS + 8 * UNPACK_REGS + 4 * ISSUE_REGS <= WARPS * LAUNCH_REGS, "a wait without end");
   static constexpr int BLOCK = kTile * 128;        // bytes of 64 channels of 128 rows
   static constexpr int ROWS = BLOCK * (D / 64);    // bytes of 128 rows
@@ -63,7 +67,7 @@ struct Plan {
 // The blocks that share a row tile's tokens, and where they leave their sums.
 struct Split {
   int splits;     // blocks for each row tile and head
-  int* arrivals;  // one for each of these
+  int* arrivals;  // one for each of these; without a split: pieces of work given out, blocks that have no more
   float2* stats;  // [row tile and head][splits][rows]: maximum (a power of two's exponent) and sum
   float4* parts;  // [row tile and head][splits][dim / 4][rows]
 };
@@ -231,18 +235,83 @@ __device__ __forceinline__ uint32_t reach(uint32_t p) {
   return finite_row(p) ? field : 0u;
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a, const Split split) {
+// A block's piece of work: the rows of a row tile (or two) and head, and the steps of tokens it takes.
+struct Work {
+  Sequence seq;
+  int b, head, row0, rows;
+  int ahead;                 // query i sees ahead + i tokens
+  int step0, steps, halves;  // first step of 128 tokens, steps, half steps; no steps: nothing is seen
+  int part, parts, tile_head;
+  bool some;  // false: this number has no work (in the queue: there is no more)
+};
+constexpr int kQueue = 8;  // pieces from the one that leaves to the one that is looked up: these are a few steps apart
+
+// Number `n` of the work, found by a whole warp.  The later tiles of a sequence, which see more, come
+// first.
+template <int RT>
+__device__ __forceinline__ Work work_at(const AttendArgs& a, const Split& split, int n, int lane) {
+  Work w{};
+  const int heads = a.pool.kv_heads;
+  w.tile_head = n / split.splits;
+  w.part = n - w.tile_head * split.splits;
+  const int item = a.kv_heads.div(w.tile_head);
+  w.head = w.tile_head - item * heads;
+  int before = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < (int)a.batch && !w.some; b0 += 32) {
+    Sequence s{0, 0, 0};
+    int tiles = 0;
+    if (b0 + lane < a.batch) {
+      s = sequence(a, b0 + lane, false);
+      tiles = (s.count * (int)a.group.d + RT - 1) / RT;
+    }
+    int x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const uint32_t here = __ballot_sync(0xffffffffu, item >= before + x - tiles && item < before + x);
+    if (here) {
+      const int from = __ffs(here) - 1;
+      w.some = true;
+      w.b = b0 + from;
+      w.seq.length = __shfl_sync(0xffffffffu, s.length, from);
+      w.seq.start = __shfl_sync(0xffffffffu, s.start, from);
+      w.seq.count = __shfl_sync(0xffffffffu, s.count, from);
+      w.row0 = (before + __shfl_sync(0xffffffffu, x, from) - 1 - item) * RT;
+    }
+    before = min(before + __shfl_sync(0xffffffffu, x, 31), 0x40000000);
+  }
+  if (!w.some) return w;
+  w.rows = min(RT, w.seq.count * (int)a.group.d - w.row0);
+  w.ahead = w.seq.length - w.seq.count + 1;
+  const int end = a.causal ? max(0, min(w.seq.length, w.ahead + a.group.div(w.row0 + w.rows - 1))) : w.seq.length;
+  const int all = (end + kTile - 1) / kTile;
+  const int share = max(kLeastSteps, (all + split.splits - 1) / split.splits);
+  w.parts = max(1, (all + share - 1) / share);
+  w.some = w.part < w.parts;
+  w.step0 = w.part * share;
+  w.steps = min(share, all - w.step0);
+  w.halves = min(2 * w.steps, (end + kHalf - 1) / kHalf - 2 * w.step0);
+  return w;
+}
+
+// SPLIT: blocks share row tiles, one piece of work for each block.
+template <int D, typename T, bool SPLIT>
+__global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(const AttendArgs a, const Split split, const int work) {
   using P = Plan<D>;
   constexpr int TILES = P::TILES, STAGES = P::STAGES, RT = kTile * TILES;
   constexpr int kUnpack = P::UNPACK, kIssue = P::ISSUE;  // first warps of their kind
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
-      s_full[TILES][2], p_full[TILES][2], o_done[TILES], o_full;
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES],
+      s_full[TILES][2], p_full[TILES][2], o_done[TILES], o_full, w_next, w_full[kQueue],
+      w_empty[kQueue];
   __shared__ uint32_t tensor_base;
-  __shared__ int stalled_, found[2], sh_last;
-  __shared__ Sequence sh_seq;
+  __shared__ int stalled_, sh_last;
   __shared__ Info infos[kInfos];
+  __shared__ Work queue[kQueue];
+  __shared__ float factors[2][RT];  // of two pieces' rows
   __shared__ uint32_t top_k[2][4], top_v[2][4];
   volatile int* stalled = &stalled_;
   uint8_t* smem = raw + ((1024 - (smem_of(raw) & 1023)) & 1023);
@@ -250,39 +319,10 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int heads = a.pool.kv_heads;
 
-  // ---- this block's sequence, row tiles and head; the later tiles of a sequence, which see more,
-  // come first
-  const int tile_head = blockIdx.x / split.splits, part = blockIdx.x - tile_head * split.splits;
-  const int item = a.kv_heads.div(tile_head), head = tile_head - item * heads;
-  if (warp == 0) {
-    if (lane == 0) found[0] = -1;
-    __syncwarp();
-    int64_t before = 0;
-    for (int64_t b0 = 0; b0 < a.batch; b0 += 32) {
-      Sequence s{0, 0, 0};
-      int64_t n = 0;
-      if (b0 + lane < a.batch) {
-        s = sequence(a, b0 + lane, blockIdx.x == 0);
-        n = ((int64_t)s.count * a.group.d + RT - 1) / RT;
-      }
-      int64_t x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (item >= before + x - n && item < before + x) {
-        found[0] = (int)(b0 + lane);
-        found[1] = (int)(before + x - 1 - item);
-        sh_seq = s;
-      }
-      before += __shfl_sync(0xffffffffu, x, 31);
-      if (blockIdx.x != 0 && before > item) break;
-    }
-  }
   if (threadIdx.x == 0) {
     stalled_ = 0;
-    bar_init(&q_full, kTile * TILES);
+    bar_init(&q_full, RT);
+    bar_init(&q_empty, 1);
     for (int i = 0; i < STAGES; ++i) {
       bar_init(&k_full[i], 2 * kTile);
       bar_init(&v_full[i], 2 * kTile);
@@ -297,34 +337,27 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       bar_init(&o_done[i], 1);
     }
     bar_init(&o_full, 1);
+    bar_init(&w_next, 1);
+    for (int i = 0; i < kQueue; ++i) {
+      bar_init(&w_full[i], 1);
+      bar_init(&w_empty[i], 4 * TILES + 8 + 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  // the queries that nobody has, by blocks that are done or have nothing else to do
-  auto zero_rest = [&]() {
-    zero_unowned<T>(a, D, blockIdx.x * (int64_t)(P::WARPS * 32) + threadIdx.x, (int64_t)gridDim.x * P::WARPS * 32);
+  if (blockIdx.x == 0)  // what is wrong with lengths and starts is reported once
+    for (int64_t b = threadIdx.x; b < a.batch; b += P::WARPS * 32) sequence(a, b, true);
+  // A group's next piece of work, and its return once it is read by the whole warp.
+  auto take = [&](int number) -> const Work& {
+    bar_wait(&w_full[number % kQueue], number / kQueue & 1, stalled);
+    __syncwarp();
+    return queue[number % kQueue];
   };
-  if (found[0] < 0) {
-    zero_rest();
-    return;
-  }
-  const int b = found[0];
-  const Sequence seq = sh_seq;
-  const int row0 = found[1] * RT, rows = min(RT, seq.count * (int)a.group.d - row0);
-  // tokens that some row sees
-  const int ahead = seq.length - seq.count + 1;
-  const int reach_end = a.causal ? min(seq.length, ahead + a.group.div(row0 + rows - 1)) : seq.length;
-  const int all_steps = max(0, (reach_end + kTile - 1) / kTile);
-  const int share = max(kLeastSteps, (all_steps + split.splits - 1) / split.splits);
-  const int parts = max(1, (all_steps + share - 1) / share);
-  if (part >= parts) {
-    zero_rest();
-    return;
-  }
-  const int step0 = part * share, steps = min(share, all_steps - step0);  // this block's
-  const int halves = min(2 * steps, (reach_end + kHalf - 1) / kHalf - 2 * step0);
-
-  // Each group begins with what needs no tensor memory, then waits for its address.
+  auto give_back = [&](int number) {
+    __syncwarp();
+    if (lane == 0) bar_arrive(&w_empty[number % kQueue]);
+  };
+  // All groups begin with this: the scheduling warp must not wait for one that waits for work.
   auto tensor_memory = [&]() {
     fence_before();
     __syncthreads();
@@ -336,78 +369,32 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::SOFTMAX_REGS));
     // ---------------------------------------------------------------- softmax: a row of a tile
     const int tile = warp >> 2, r = threadIdx.x & (kTile - 1), row = tile * kTile + r;
-    const bool live = row < rows;
-    const int i = a.group.div(row0 + (live ? row : 0)), h = head * a.group.d + (row0 + (live ? row : 0) - i * a.group.d);
-    const int seen = !live ? 0 : (a.causal ? min(seq.length, ahead + i) : seq.length);
-    // The warp copies its 32 rows as they are into their places, LANES lanes a row; then each thread
-    // brings its own row to float16.  Short loops: this code runs once a block, and fetching long code
-    // costs more than running it.
-    constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
-    uint8_t* const q_tile = smem + P::Q + tile * P::ROWS;
-    {
-      const T* row_at = static_cast<const T*>(a.q) + (int64_t)(seq.start + i) * a.q_ts + h * a.q_hs;
-      const int c = lane % LANES;
-#pragma unroll 4
-      for (int n = lane / LANES; n < 32; n += AT_ONCE) {
-        const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(row_at), n)) + c * 8;
-        const bool there = row - lane + n < rows;
-        const int rr = (warp & 3) * 32 + n;
-        uint8_t* dst = q_tile + (c >> 3) * P::BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-        if (a.vec) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(dst)), "l"(src), "r"(there ? 16 : 0)
-                       : "memory");
-        } else {
-          const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll 1
-          for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = there ? u[k] : (uint16_t)0;
-        }
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncwarp();
-    float top_q = 0.0f;
-#pragma unroll 4
-    for (int c = 0; c < D / 8; ++c) {
-      const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (c >> 3) * P::BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-      const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
-                   f3 = Half2<T>::unpack(x.w);
-      top_q = fmaxf(top_q, fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
-                                 fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y)))));
-    }
-    const int e_q = 13 - max(-87, min(116, (int)(__float_as_uint(top_q) >> 23) - 127));
-    const float up = a.scale_log2 < 0.0f ? -pow2(e_q) : pow2(e_q);
-    // scores are `factor` and the step's factor times the product, in powers of two
-    const float factor = fabsf(a.scale_log2) * pow2(-e_q);
-#pragma unroll 4
-    for (int c = 0; c < D / 8; ++c) {
-      uint4* at = reinterpret_cast<uint4*>(q_tile + (c >> 3) * P::BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-      const uint4 x = *at;
-      const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
-                   f3 = Half2<T>::unpack(x.w);
-      uint4 w;  // channels in the order that codes unpack in
-      w.x = Half2<__half>::pack(f0.x * up, f2.x * up);
-      w.y = Half2<__half>::pack(f0.y * up, f2.y * up);
-      w.z = Half2<__half>::pack(f1.x * up, f3.x * up);
-      w.w = Half2<__half>::pack(f1.y * up, f3.y * up);
-      *at = w;
-    }
-    fence_smem();
-    bar_arrive(&q_full);
     const uint32_t tensor = tensor_memory();
-
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 rows of tensor memory
     const uint32_t s_at = tensor + lanes + tile * P::S_COLUMNS, o_at = tensor + lanes + P::O + tile * D;
+    uint32_t done0 = 0, done1 = 0, items = 0, steps_done = 0;  // half steps in each place, pieces, steps before this piece
+    int number = 0;
+#pragma unroll 1
+    for (;; ++number) {
+    const Work& k = take(number);  // read again where it is used: registers are dear here
+    if (!k.some || *stalled) break;
+    const int seen = row >= k.rows ? 0 : (a.causal ? min(k.seq.length, k.ahead + a.group.div(k.row0 + row)) : k.seq.length);
+    const int halves = k.halves;
+    int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
     float m = -INFINITY, l = 0.0f;
     bool poisoned = false;
     int shift = 0;
     uint32_t x[2][32];
     auto scores_of = [&](int n) {  // half step n's are there
-      bar_wait(&s_full[tile][n & 1], (n >> 1) & 1, stalled);
+      bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, stalled);
       __syncwarp();
       fence_after();
     };
+    // scores are `factor` and the step's factor times the product, in powers of two
+    float factor = 0.0f;
     if (halves > 0) {
       scores_of(0);
+      factor = factors[items & 1][row];
       load32(x[0], s_at);
       load32(x[1], s_at + 32);
     }
@@ -415,11 +402,12 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     for (int n = 0; n < halves; ++n) {
       const int j = n >> 1, h = n & 1;
       const uint32_t at = s_at + h * kHalf, at_next = s_at + (h ^ 1) * kHalf;
-      const Info& info = infos[j & (kInfos - 1)];
+      const Info& info = infos[(steps_done + j) & (kInfos - 1)];
       const float f = scaled(factor, -info.key_shift);
       const int now = info.value_shift;
       const bool special = (info.hidden[2 * h] | info.hidden[2 * h + 1] | info.bad[2 * h] | info.bad[2 * h + 1]) != 0;
-      const int left = seen - (step0 + j) * kTile - h * kHalf;  // tokens of this half step that the row sees
+      const int left = left_all;
+      left_all -= kHalf;
       const bool masked = __any_sync(0xffffffffu, left < kHalf) || special;
       loaded();
       hold(x[0]);
@@ -454,7 +442,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
         l *= keep;
         if (n > 0) {  // O is not yet written before the first half step, and at rest after the last one's
-          bar_wait(&o_done[tile], (n - 1) & 1, stalled);
+          bar_wait(&o_done[tile], (done0 + done1 + n - 1) & 1, stalled);
           __syncwarp();
           fence_after();
           const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
@@ -508,12 +496,16 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       bar_arrive(&p_full[tile][h]);
     }
     // ---- the rows' results
-    if (steps > 0) {
-      bar_wait(&o_full, 0, stalled);
+    const bool live = row < k.rows;
+    const int i = a.group.div(k.row0 + (live ? row : 0)),
+              h = k.head * a.group.d + (k.row0 + (live ? row : 0) - i * a.group.d);
+    const int64_t o = (int64_t)(k.seq.start + i) * a.q_heads + h;
+    const int tile_head = k.tile_head, part = k.part, parts = SPLIT ? k.parts : 1;
+    if (halves > 0) {
+      bar_wait(&o_full, items & 1, stalled);
       __syncwarp();
       fence_after();
     }
-    const int64_t o = (int64_t)(seq.start + i) * a.q_heads + h;
     if (poisoned) l = __int_as_float(0x7fffffff);
     // 8 channels of the row, unpacking's order undone
     auto write8 = [&](int d, const float (&v)[8], float k) {
@@ -525,11 +517,14 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + d) = w;
     };
     const int64_t mine = (int64_t)tile_head * split.splits + part;
-    const float k = l == 0.0f ? 0.0f : scaled(1.0f / l, -shift);
+    const float inv_l = l == 0.0f ? 0.0f : (SPLIT && parts > 1 ? 1.0f : 1.0f / l);
+    const float back0 = pow2((-shift) >> 1) * inv_l, back1 = pow2(-shift - ((-shift) >> 1));
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t x[32];
-      if (steps > 0) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = 0;
+      if (halves > 0) {
         load32(x, o_at + c);
         loaded();
         hold(x);
@@ -540,20 +535,20 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
           float v[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e]);
-            v[e + 4] = l == 0.0f ? 0.0f : __uint_as_float(x[8 * g + 2 * e + 1]);
+            v[e] = __uint_as_float(x[8 * g + 2 * e]) * back0;
+            v[e + 4] = __uint_as_float(x[8 * g + 2 * e + 1]) * back0;
           }
-          if (parts == 1) {
-            write8(c + g * 8, v, k);
+          if (!SPLIT || parts == 1) {
+            write8(c + g * 8, v, back1);
           } else {
             float4* to = split.parts + (mine * (D / 4) + c / 4 + g * 2) * RT + row;
-            to[0] = make_float4(scaled(v[0], -shift), scaled(v[1], -shift), scaled(v[2], -shift), scaled(v[3], -shift));
-            to[RT] = make_float4(scaled(v[4], -shift), scaled(v[5], -shift), scaled(v[6], -shift), scaled(v[7], -shift));
+            to[0] = make_float4(v[0] * back1, v[1] * back1, v[2] * back1, v[3] * back1);
+            to[RT] = make_float4(v[4] * back1, v[5] * back1, v[6] * back1, v[7] * back1);
           }
         }
       }
     }
-    if (parts > 1) {
+    if (SPLIT && parts > 1) {
       split.stats[mine * RT + row] = make_float2(m, l);
       __threadfence();
       asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
@@ -593,30 +588,64 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     }
     if (live && a.lse && (parts == 1 || sh_last))
       a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    if (halves > 0) {
+      done0 += (halves + 1) >> 1;
+      done1 += halves >> 1;
+      steps_done += k.steps;
+      ++items;
+      fence_before();
+    }
+    if (SPLIT) break;
+    give_back(number);
+    }
   } else if (warp < kIssue) {
     if constexpr (P::UNPACK_REGS > P::LAUNCH_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
     // ---------------------------------------------------------------- unpacking: half a token's row
     constexpr int CODES = D / 64;  // 16 bytes each of a thread's keys or values
     const int quarter = (warp - kUnpack) & 3, t = quarter * 32 + lane, part_of_row = (warp - kUnpack) >> 2;
-    const int32_t* table = a.pages + (int64_t)b * a.max_pages;
     const int64_t side_rows = (int64_t)heads * a.pool.page_size;
     uint4 kc[CODES], vc[CODES];
     uint32_t kp = 0, vp = 0;
-    int page = -1, state = 0;  // 0: past the end, 1: a row of the cache, 2: hidden
-    auto look_up = [&](int j) {
-      const int token = (step0 + j) * kTile + t;
-      page = j < steps && token < seq.length ? __ldg(table + a.page_size.div(token)) : -1;
+    int state = 0;  // 0: past the end, 1: a row of the cache, 2: hidden
+    // The step whose pages are looked up (two ahead of the one that is unpacked), and what is known of
+    // the one before it.
+    int number = 0, slot = 0, slot_now = 0, items = 0, steps_left = 0, token = 0, length = 0, page = -1, place = 0, in_head = 0;
+    const int32_t* table = nullptr;
+    bool in = false, first = false, valid = true, begun = false;
+    auto look_up = [&]() {
+      first = steps_left <= 0;
+      if (valid && first) {
+        do {  // pieces in which nothing is seen are passed over
+          const Work& k = take(number);
+          valid = k.some && !*stalled;
+          steps_left = k.steps;
+          length = k.seq.length;
+          in_head = k.head;
+          token = k.step0 * kTile + t;
+          table = a.pages + (int64_t)k.b * a.max_pages;
+          if (threadIdx.x == kUnpack * 32) bar_arrive(&w_next);  // time to find the one after it
+          if (valid && steps_left <= 0) give_back(number);
+          ++number;
+        } while (valid && steps_left <= 0);
+        slot = number - 1;
+      }
+      if (!valid) return;
+      const int at = a.page_size.div(token);
+      in = token < length;
+      place = token - at * a.pool.page_size;
+      page = in ? __ldg(table + at) : -1;
+      token += kTile;
+      --steps_left;
     };
     const uint8_t* from = nullptr;
-    auto fetch_keys = [&](int j) {  // and both rows' parameters
-      const int token = (step0 + j) * kTile + t;
+    auto fetch_keys = [&]() {  // of the looked up step, and both rows' parameters
       state = 0;
       kp = vp = 0;
-      if (j < steps && token < seq.length) {
+      if (valid && in) {
         if ((unsigned)page < (unsigned)a.pool.num_pages) {
           state = 1;
-          const int64_t at = a.pool.row(page, 0, head) + (token - a.page_size.div(token) * a.pool.page_size);
+          const int64_t at = a.pool.row(page, 0, in_head) + place;
           kp = __ldg(a.pool.params + at);
           vp = __ldg(a.pool.params + at + side_rows);
           from = a.pool.codes + at * (D / 2) + part_of_row * (D / 4);
@@ -657,15 +686,88 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         }
       }
     };
-    look_up(0);
-    fetch_keys(0);
-    fetch_values();
-    look_up(1);
+    // The queries of the piece whose first step is looked up.  A warp copies 32 rows as they are into
+    // their places, LANES lanes a row; then each thread brings a row to float16 by its own power of two.
+    auto copy_queries = [&](const Work& k) {
+      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+      const int row = part_of_row * kTile + t;
+      if (row >= RT) return;
+      uint8_t* const q_tile = smem + P::Q + part_of_row * P::ROWS;
+      const int gr = k.row0 + (row < k.rows ? row : 0), i = a.group.div(gr), h = k.head * a.group.d + (gr - i * a.group.d);
+      const T* row_at = static_cast<const T*>(a.q) + (int64_t)(k.seq.start + i) * a.q_ts + h * a.q_hs;
+      const int c = lane % LANES;
+#pragma unroll 2
+      for (int n = lane / LANES; n < 32; n += AT_ONCE) {
+        const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(row_at), n)) + c * 8;
+        const bool there = row - lane + n < k.rows;
+        const int rr = quarter * 32 + n;
+        uint8_t* dst = q_tile + (c >> 3) * P::BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+        if (a.vec) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(dst)), "l"(src), "r"(there ? 16 : 0)
+                       : "memory");
+        } else {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(dst)[e] = there ? u[e] : (uint16_t)0;
+        }
+      }
+    };
+    auto turn_queries = [&](int item) {
+      const int row = part_of_row * kTile + t;
+      if (row >= RT) return;
+      uint8_t* const q_row = smem + P::Q + part_of_row * P::ROWS + t * 128;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      float top = 0.0f;
+#pragma unroll 2
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4*>(q_row + (c >> 3) * P::BLOCK + (((c & 7) ^ (t & 7)) << 4));
+        const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
+                     f3 = Half2<T>::unpack(x.w);
+        top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                               fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y)))));
+      }
+      const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));
+      const float up = a.scale_log2 < 0.0f ? -pow2(e) : pow2(e);
+      factors[item & 1][row] = fabsf(a.scale_log2) * pow2(-e);
+#pragma unroll 2
+      for (int c = 0; c < D / 8; ++c) {
+        uint4* at = reinterpret_cast<uint4*>(q_row + (c >> 3) * P::BLOCK + (((c & 7) ^ (t & 7)) << 4));
+        const uint4 x = *at;
+        const float2 f0 = Half2<T>::unpack(x.x), f1 = Half2<T>::unpack(x.y), f2 = Half2<T>::unpack(x.z),
+                     f3 = Half2<T>::unpack(x.w);
+        uint4 w;  // channels in the order that codes unpack in
+        w.x = Half2<__half>::pack(f0.x * up, f2.x * up);
+        w.y = Half2<__half>::pack(f0.y * up, f2.y * up);
+        w.z = Half2<__half>::pack(f1.x * up, f3.x * up);
+        w.w = Half2<__half>::pack(f1.y * up, f3.y * up);
+        *at = w;
+      }
+      fence_smem();
+      bar_arrive(&q_full);
+    };
     tensor_memory();
+    look_up();
+    fetch_keys();
+    fetch_values();
+    begun = first;
+    slot_now = slot;
+    bool there = valid;
+    look_up();
     uint32_t value_top = 27;  // exponent field of the largest value so far
-    for (int j = 0; j < steps; ++j) {
-      const int stage = j % STAGES;
-      const uint32_t filled = (uint32_t)(j / STAGES) & 1;
+    int stage = 0;
+    uint32_t filled = 0;
+#pragma unroll 1
+    for (uint32_t j = 0; there; ++j) {
+      if (begun) {
+        value_top = 27;
+        if (items > 0) bar_wait(&q_empty, (items - 1) & 1, stalled);
+        __syncwarp();
+        copy_queries(queue[slot_now % kQueue]);
+        give_back(slot_now);
+        turn_queries(items);
+        ++items;
+      }
       // the largest key and value, over the step
       const uint32_t wk = __reduce_max_sync(0xffffffffu, reach(kp)), wv = __reduce_max_sync(0xffffffffu, reach(vp));
       if (lane == 0 && part_of_row == 0) {
@@ -694,13 +796,18 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       fence_smem();
       bar_arrive(&k_full[stage]);
       const uint32_t value_params = bad ? 0 : vp;  // a value that is not finite is left to its rows
-      fetch_keys(j + 1);
-      look_up(j + 2);
+      fetch_keys();
+      begun = first;
+      slot_now = slot;
+      there = valid;
+      look_up();
       bar_wait(&v_empty[stage], filled ^ 1, stalled);
       spread(vc, value_params, value_shift, smem + P::V + stage * P::ROWS);
       fence_smem();
       bar_arrive(&v_full[stage]);
       fetch_values();
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      filled ^= stage == 0;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::ISSUE_REGS));
@@ -710,7 +817,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     const uint32_t tensor = tensor_memory();
-    if (warp == kIssue && steps > 0) {
+    if (warp == kIssue) {
       // ---------------------------------------------------------------- products
       // The whole warp walks along, so that operands stay in uniform registers; one thread issues.
       const uint32_t base = smem_of(smem), into = __shfl_sync(0xffffffffu, tensor, 0);
@@ -742,48 +849,94 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         }
         __syncwarp();
       };
-      bar_wait(&q_full, 0, stalled);
-      bar_wait(&k_full[0], 0, stalled);
-      fence_after();
-#pragma unroll 1
-      for (int n = 0; n < min(2, halves); ++n)
-#pragma unroll
-        for (int tile = 0; tile < TILES; ++tile) scores(tile, 0, n);
-      if (one) commit(&k_empty[0]);
       int stage = 0;
-      uint32_t filled = 0;
+      uint32_t filled = 0, items = 0, done0 = 0, done1 = 0;
 #pragma unroll 1
-      for (int n = 0; n < halves; ++n) {
-        const int h = n & 1, next = stage + 1 == STAGES ? 0 : stage + 1;
-        const uint32_t phase = (n >> 1) & 1, next_filled = filled ^ (next == 0);
-        if (h == 0) bar_wait(&v_full[stage], filled, stalled);
+      for (int number = 0;; ++number) {
+        const Work& k = take(number);
+        const int steps = k.steps, halves = k.halves;
+        const bool some = k.some && !*stalled;
+        give_back(number);
+        if (!some) break;
+        if (steps <= 0) continue;
+        bar_wait(&q_full, items & 1, stalled);
+        bar_wait(&k_full[stage], filled, stalled);
+        fence_after();
+#pragma unroll 1
+        for (int n = 0; n < min(2, halves); ++n)
 #pragma unroll
-        for (int tile = 0; tile < TILES; ++tile) {
-          bar_wait(&p_full[tile][h], phase, stalled);
-          fence_after();
-          values(tile, stage, h, n > 0);
-          if (n + 2 < halves) {
-            if (h == 0 && tile == 0) {
-              bar_wait(&k_full[next], next_filled, stalled);
-              fence_after();
+          for (int tile = 0; tile < TILES; ++tile) scores(tile, stage, n);
+        if (one) {
+          commit(&k_empty[stage]);
+          if (halves <= 2) commit(&q_empty);
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int n = 0; n < halves; ++n) {
+          const int h = n & 1, next = stage + 1 == STAGES ? 0 : stage + 1;
+          const uint32_t phase = ((h ? done1 : done0) + (n >> 1)) & 1, next_filled = filled ^ (next == 0);
+          if (h == 0) bar_wait(&v_full[stage], filled, stalled);
+#pragma unroll
+          for (int tile = 0; tile < TILES; ++tile) {
+            bar_wait(&p_full[tile][h], phase, stalled);
+            fence_after();
+            values(tile, stage, h, n > 0);
+            if (n + 2 < halves) {
+              if (h == 0 && tile == 0) {
+                bar_wait(&k_full[next], next_filled, stalled);
+                fence_after();
+              }
+              scores(tile, next, h);
             }
-            scores(tile, next, h);
           }
-        }
-        if (h == 1) {
-          if (one) {
-            commit(&v_empty[stage]);
-            commit(&k_empty[next]);
-          }
+          if (one && n + 3 == halves) commit(&q_empty);  // no product reads these queries any more
           __syncwarp();
-          stage = next;
-          filled = next_filled;
+          if (h == 1 || n + 1 == halves) {  // the step's last half
+            if (one) {
+              commit(&v_empty[stage]);
+              if ((n >> 1) + 1 < steps) commit(&k_empty[next]);
+            }
+            __syncwarp();
+            stage = next;
+            filled = next_filled;
+          }
         }
+        if (one) commit(&o_full);
+        __syncwarp();
+        done0 += (halves + 1) >> 1;
+        done1 += halves >> 1;
+        ++items;
       }
-      if (one) commit(&o_full);
       // nothing is in flight when the tensor memory is given back, even after a wait that ran out
       volatile int late = 0;
-      bar_wait(&o_full, 0, &late);
+      if (items > 0) bar_wait(&o_full, (items - 1) & 1, &late);
+    } else if (warp == kIssue + 1) {
+      // ---------------------------------------------------------------- scheduling
+      // The first pieces are the blocks' by their numbers, the others whoever's is free: pieces of a
+      // causal prompt differ by the tokens that they see, the largest come first.
+      int number = 0, n = blockIdx.x;
+#pragma unroll 1
+      for (;;) {
+        Work w{};
+        if (n < work) w = work_at<RT>(a, split, n, lane);
+        if (n < work && !w.some) {
+          n = SPLIT ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
+          continue;
+        }
+        bar_wait(&w_empty[number % kQueue], number / kQueue & 1 ^ 1, stalled);
+        if (lane == 0) {
+          queue[number % kQueue] = w;
+          bar_arrive(&w_full[number % kQueue]);
+        }
+        __syncwarp();
+        if (!w.some) break;
+        // one that is taken earlier than it is needed may be one that another block would end sooner
+        bar_wait(&w_next, number & 1, stalled);
+        ++number;
+        n = SPLIT || *stalled ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
+      }
+      // every block has had its last number when the last of them comes here
+      if (!SPLIT && lane == 0 && arrive(split.arrivals + 1, gridDim.x)) split.arrivals[0] = 0;
     }
   }
   fence_before();
@@ -794,7 +947,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tensor_base));
   }
-  zero_rest();
+  zero_unowned<T>(a, D, blockIdx.x * (int64_t)(P::WARPS * 32) + threadIdx.x, (int64_t)gridDim.x * P::WARPS * 32);
 }
 
 // Row tiles times heads, at most: one tile that is not full for each sequence that has queries.
@@ -825,26 +978,24 @@ int splits_for(int64_t tiles, int64_t max_tokens) {
 template <int D, typename T>
 int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
   using P = Plan<D>;
-  static bool ready = false;
-  if (!ready) {
-    if (cudaFuncSetAttribute(attend_prompt_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) !=
-        cudaSuccess)
-      return TANS_E_CUDA;
-    ready = true;
-  }
   constexpr int RT = kTile * P::TILES;
   const int64_t tiles = most_tiles(RT, a.total_queries * a.group.d, std::min(a.batch, a.total_queries), a.pool.kv_heads);
-  if (tiles > 0x7fffffff) return TANS_E_TOO_LARGE;
+  if (tiles > 0x3fffffff) return TANS_E_TOO_LARGE;
   Split split{1, nullptr, nullptr, nullptr};
-  if (workspace) {
-    split.splits = splits_for(tiles, a.max_pages * a.pool.page_size);
-    split.arrivals = static_cast<int*>(workspace);
-    split.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + Join::kArrivalBytes);
-    split.parts = reinterpret_cast<float4*>(split.stats + tiles * split.splits * RT);
-  }
-  attend_prompt_kernel<D, T><<<(unsigned)(tiles * split.splits), P::WARPS * 32, P::BYTES, s>>>(a, split);
-  note_launch();
-  return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
+  split.splits = splits_for(tiles, a.max_pages * a.pool.page_size);
+  split.arrivals = static_cast<int*>(workspace);
+  split.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + Join::kArrivalBytes);
+  split.parts = reinterpret_cast<float4*>(split.stats + tiles * split.splits * RT);
+  const int work = (int)tiles * split.splits;
+  auto go = [&](auto* kernel, int blocks) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess)
+      return TANS_E_CUDA;
+    kernel<<<blocks, P::WARPS * 32, P::BYTES, s>>>(a, split, work);
+    note_launch();
+    return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
+  };
+  return split.splits > 1 ? go(&attend_prompt_kernel<D, T, true>, work)
+                          : go(&attend_prompt_kernel<D, T, false>, std::min(work, sm_count()));
 }
 
 }  // namespace
@@ -853,7 +1004,7 @@ size_t attend_prompt_workspace(int head_dim, int64_t total_rows, int64_t sequenc
   const int64_t rows = head_dim == 256 ? kTile : 2 * kTile;
   const int64_t tiles = most_tiles((int)rows, total_rows, sequences, kv_heads);
   const int splits = splits_for(tiles, max_tokens);
-  return splits == 1 ? 0 : align_up(Join::kArrivalBytes + (size_t)tiles * splits * rows * (8 + head_dim * 4));
+  return align_up(Join::kArrivalBytes + (splits == 1 ? 0 : (size_t)tiles * splits * rows * (8 + head_dim * 4)));
 }
 
 int launch_attend_prompt(const AttendArgs& a, int dtype, void* workspace, cudaStream_t s) {

@@ -851,6 +851,8 @@ std::optional<Tensor> kv4_append(const Tensor& codes, const Tensor& params, cons
                 "torch_ans_b200: `rotation` must be a contiguous float32 tensor (positions, rotary_dim) on the device of `codes`");
     rows = rotation->size(0);
     rotary = rotation->size(1);
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(rotation->data_ptr()) % 16 == 0,
+                "torch_ans_b200: `rotation` must be 16-byte aligned");
     TORCH_CHECK(rows >= 1 && rotary >= 16 && rotary <= p.head_dim && rotary % 16 == 0,
                 "torch_ans_b200: rotary_dim must be a multiple of 16 up to head_dim, not ", rotary);
   }

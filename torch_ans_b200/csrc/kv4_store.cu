@@ -42,148 +42,193 @@ struct AppendArgs {
   uint32_t* status;
 };
 
-// 8 consecutive elements of a row as floats
+// 8 consecutive elements of a row, as they are
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  if constexpr (VEC) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ uint4 load8(const T* p) {
+  if constexpr (VEC) return *reinterpret_cast<const uint4*>(p);
+  const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+  return make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16,
+                    u[6] | (uint32_t)u[7] << 16);
+}
+template <typename T>
+__device__ __forceinline__ void floats(const uint4& w, float (&x)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Half2<T>::unpack(u[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Half2<T>::load(p + i);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Half2<T>::unpack(u[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
   }
 }
 
-// Rotation and quantisation, head_dim / 8 lanes for each row (one token's head), 8 channels a lane.
-// The products and sums of the rotation are rounded one by one (no fused multiply-add), so the
-// codes do not depend on the compiler's choices.
-template <int D, typename T, bool VEC, bool INTERLEAVED>
+// Rotation and quantisation, head_dim / 8 lanes for each row (one token's head), 8 channels a lane; a
+// group of lanes takes ROWS rows of one token, so that the token's cosines and sines are read once for
+// all of them and the loads of the rows do not wait for one another.
+//
+// What it may not do without is bytes: 2 read and 2 written for a query's channel, 2 read and about 0.53
+// written for a key's or a value's.  16,381 tokens of 32 + 16 heads of 128 (355 MB): see the table of
+// measurements for the time.  The products and sums of the rotation are rounded one by one (no fused
+// multiply-add), so the codes do not depend on the compiler's choices.
+//
+// The quotient (x - offset) / scale is the correctly rounded one, so that ties (common: x has 8 or 11
+// bits, scale 8) go to the even code; it takes one division a row and, by Markstein's theorem, two fused
+// steps a channel: with y the correctly rounded 1 / scale and q0 = d y, q0 + (d - q0 scale) y rounds
+// correctly.
+template <int D, typename T, bool VEC, bool INTERLEAVED, int ROWS>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   constexpr int L = D / 8;
-  const int lane = threadIdx.x % L;
-  const int per_token = a.q_heads + 2 * a.pool.kv_heads;
-  const int64_t total = a.tokens * per_token;
-  int64_t row = blockIdx.x * (int64_t)(kThreads / L) + threadIdx.x / L;
-  const bool live = row < total;
-  if (!live) row = total - 1;  // keeps the warp's shuffles whole; writes nothing
-  const int64_t token = row / per_token;
-  const int r = (int)(row - token * per_token);
-  const int kind = r < a.q_heads ? 0 : (r < a.q_heads + a.pool.kv_heads ? 1 : 2);
-  const int head = kind == 0 ? r : (r - a.q_heads) % a.pool.kv_heads;
-  const T* src = kind == 0   ? static_cast<const T*>(a.q) + token * a.q_ts + head * a.q_hs
-                 : kind == 1 ? static_cast<const T*>(a.k) + token * a.k_ts + head * a.k_hs
-                             : static_cast<const T*>(a.v) + token * a.v_ts + head * a.v_hs;
-  const int d0 = lane * 8;
-  float x[8];
-  load8<T, VEC>(src + d0, x);
+  const int lane = threadIdx.x % L, d0 = lane * 8;
+  const int per_token = a.q_heads + 2 * a.pool.kv_heads, chunks = (per_token + ROWS - 1) / ROWS;
+  const int64_t group = blockIdx.x * (int64_t)(kThreads / L) + threadIdx.x / L;
+  const int64_t token = min(group / chunks, a.tokens - 1);  // groups past the end keep the warp's shuffles whole
+  const int r0 = (int)(group % chunks) * ROWS;
+  const int rows = group >= a.tokens * chunks ? 0 : min(ROWS, per_token - r0);
 
+  auto source = [&](int r) -> const T* {  // row r of the token: queries, keys, values
+    if (r < a.q_heads) return static_cast<const T*>(a.q) + token * a.q_ts + r * a.q_hs;
+    r -= a.q_heads;
+    if (r < a.pool.kv_heads) return static_cast<const T*>(a.k) + token * a.k_ts + r * a.k_hs;
+    return static_cast<const T*>(a.v) + token * a.v_ts + (r - a.pool.kv_heads) * a.v_hs;
+  };
+  uint4 raw[ROWS];
+#pragma unroll
+  for (int n = 0; n < ROWS; ++n) raw[n] = n < rows ? load8<T, VEC>(source(r0 + n) + d0) : make_uint4(0, 0, 0, 0);
+
+  const int64_t slot = r0 + rows > a.q_heads ? a.slots[token] : -1;
+  bool known = false;
+  float c[8], s[8];
+  const int half = a.rotary / 2;
+  const bool first = d0 < half;
   if (a.rotary > 0) {
     const int64_t pos = a.positions[token];
-    const bool known = pos >= 0 && pos < a.rotation_rows;
-    if (!known && a.status && lane == 0 && live) atomicOr(a.status, TANS_DEV_BAD_INDEX);
-    const bool turns = kind != 2 && known && d0 < a.rotary;
-    const int half = a.rotary / 2;
-    const float* cosines = a.rotation + (known ? pos : 0) * a.rotary;
+    known = pos >= 0 && pos < a.rotation_rows;
+    if (!known && a.status && lane == 0 && r0 == 0 && rows > 0) atomicOr(a.status, TANS_DEV_BAD_INDEX);
+    if (known && d0 < a.rotary) {
+      const float* cosines = a.rotation + pos * a.rotary + (INTERLEAVED ? d0 / 2 : (first ? d0 : d0 - half));
+#pragma unroll
+      for (int i = 0; i < (INTERLEAVED ? 4 : 8); i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(cosines + i), y = *reinterpret_cast<const float4*>(cosines + half + i);
+        c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
+        s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
+      }
+    }
+  }
+  const bool turns = known && d0 < a.rotary;
+  bool stores = slot >= 0;
+  if (slot >= a.pool.num_pages * a.pool.page_size) {
+    stores = false;
+    if (a.status && lane == 0) atomicOr(a.status, TANS_DEV_BAD_INDEX);
+  }
+  const int64_t page = stores ? slot / a.pool.page_size : 0;
+  const int in_page = stores ? (int)(slot - page * a.pool.page_size) : 0;
+
+#pragma unroll
+  for (int n = 0; n < ROWS; ++n) {
+    const int r = r0 + n;
+    const bool live = n < rows, query = r < a.q_heads, value = r >= a.q_heads + a.pool.kv_heads;
+    float x[8];
+    floats<T>(raw[n], x);
     if constexpr (INTERLEAVED) {
-      if (turns) {
+      if (turns && !value) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float c = cosines[d0 / 2 + i], s = cosines[half + d0 / 2 + i];
           const float u = x[2 * i], w = x[2 * i + 1];
-          x[2 * i] = __fsub_rn(__fmul_rn(u, c), __fmul_rn(w, s));
-          x[2 * i + 1] = __fadd_rn(__fmul_rn(w, c), __fmul_rn(u, s));
+          x[2 * i] = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(w, s[i]));
+          x[2 * i + 1] = __fadd_rn(__fmul_rn(w, c[i]), __fmul_rn(u, s[i]));
         }
       }
-    } else {
+    } else if (a.rotary > 0) {
       // the partner channels are half / 8 lanes away
-      const bool first = d0 < half;
       const int warp_lane = threadIdx.x & 31;
       const int partner = d0 < a.rotary ? (first ? warp_lane + half / 8 : warp_lane - half / 8) : warp_lane;
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
-      if (turns) {
-        const int i0 = first ? d0 : d0 - half;
+      uint4 w;
+      w.x = __shfl_sync(0xffffffffu, raw[n].x, partner);
+      w.y = __shfl_sync(0xffffffffu, raw[n].y, partner);
+      w.z = __shfl_sync(0xffffffffu, raw[n].z, partner);
+      w.w = __shfl_sync(0xffffffffu, raw[n].w, partner);
+      if (turns && !value) {
+        float y[8];
+        floats<T>(w, y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float c = cosines[i0 + i], s = cosines[half + i0 + i];
-          const float xc = __fmul_rn(x[i], c), ys = __fmul_rn(y[i], s);
+          const float xc = __fmul_rn(x[i], c[i]), ys = __fmul_rn(y[i], s[i]);
           x[i] = first ? __fsub_rn(xc, ys) : __fadd_rn(xc, ys);
         }
       }
     }
-  }
-
-  if (kind == 0 && live) {
-    uint4 w;
-    w.x = Half2<T>::pack(x[0], x[1]);
-    w.y = Half2<T>::pack(x[2], x[3]);
-    w.z = Half2<T>::pack(x[4], x[5]);
-    w.w = Half2<T>::pack(x[6], x[7]);
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (token * a.q_heads + head) * D + d0) = w;
-  }
-
-  // the row's range, then its codes
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
-  }
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (kind == 0 || !live) return;
-  const int64_t slot = a.slots[token];
-  if (slot < 0) return;
-  if (slot >= a.pool.num_pages * a.pool.page_size) {
-    if (a.status && lane == 0) atomicOr(a.status, TANS_DEV_BAD_INDEX);
-    return;
-  }
-  const float offset = __bfloat162float(__float2bfloat16_rn(lo));
-  // the product with the float nearest 1/15 is the quotient up to a unit in float's last place, 2^-15
-  // of one in bfloat16's
-  float scale = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, offset), 1.0f / 15.0f)));
-  if (scale < kTinyScale) scale = 0.0f;
-  const bool finite = isfinite(scale) && isfinite(offset);
-  uint32_t packed = 0;
-  if (finite && scale > 0.0f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], offset), scale)), 0.0f), 15.0f);
-      packed |= (uint32_t)c << (4 * i);
+    if (query && live) {
+      uint4 w;
+      w.x = Half2<T>::pack(x[0], x[1]);
+      w.y = Half2<T>::pack(x[2], x[3]);
+      w.z = Half2<T>::pack(x[4], x[5]);
+      w.w = Half2<T>::pack(x[6], x[7]);
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (token * a.q_heads + r) * D + d0) = w;
     }
-  }
-  const int64_t page = slot / a.pool.page_size;
-  const int64_t at = a.pool.row(page, kind - 1, head) + (slot - page * a.pool.page_size);
-  *reinterpret_cast<uint32_t*>(a.codes + at * (D / 2) + lane * 4) = packed;
-  if (lane == 0) {
-    a.params[at] = finite ? (__float_as_uint(scale) >> 16) | __float_as_uint(offset) : 0x7fff7fffu;
+    if (__all_sync(0xffffffffu, query || !live || !stores)) continue;
+
+    // the row's range, then its codes
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo = min_nan(lo, x[i]);
+      hi = max_nan(hi, x[i]);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (query || !live || !stores) continue;
+    const float offset = __bfloat162float(__float2bfloat16_rn(lo));
+    // the product with the float nearest 1/15 is the quotient up to a unit in float's last place, 2^-15
+    // of one in bfloat16's
+    float scale = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, offset), 1.0f / 15.0f)));
+    if (scale < kTinyScale) scale = 0.0f;
+    const bool finite = isfinite(scale) && isfinite(offset);
+    uint32_t packed = 0;
+    if (finite && scale > 0.0f) {
+      const float y = __frcp_rn(scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = __fsub_rn(x[i], offset), q0 = __fmul_rn(d, y);
+        const float q = __fmaf_rn(__fmaf_rn(-q0, scale, d), y, q0);
+        // adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and leaves it in the low bits
+        const uint32_t code = __float_as_uint(__fadd_rn(fminf(fmaxf(q, 0.0f), 15.0f), 12582912.0f)) & 15;
+        packed |= code << (4 * i);
+      }
+    }
+    const int kv = r - a.q_heads, side = value, head = value ? kv - a.pool.kv_heads : kv;
+    const int64_t at = a.pool.row(page, side, head) + in_page;
+    *reinterpret_cast<uint32_t*>(a.codes + at * (D / 2) + lane * 4) = packed;
+    if (lane == 0) a.params[at] = finite ? (__float_as_uint(scale) >> 16) | __float_as_uint(offset) : 0x7fff7fffu;
   }
 }
 
-template <int D, typename T>
-int launch_append(const AppendArgs& a, bool vec, bool interleaved, cudaStream_t s) {
-  const int64_t rows = a.tokens * (a.q_heads + 2 * (int64_t)a.pool.kv_heads);
-  const int64_t blocks = (rows + kThreads / (D / 8) - 1) / (kThreads / (D / 8));
+template <int D, typename T, int ROWS>
+int launch_rows(const AppendArgs& a, bool vec, bool interleaved, cudaStream_t s) {
+  const int64_t per_token = a.q_heads + 2 * (int64_t)a.pool.kv_heads;
+  const int64_t groups = a.tokens * ((per_token + ROWS - 1) / ROWS), per_block = kThreads / (D / 8);
+  const int64_t blocks = (groups + per_block - 1) / per_block;
   if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
   if (vec) {
-    if (interleaved) append_kernel<D, T, true, true><<<(unsigned)blocks, kThreads, 0, s>>>(a);
-    else append_kernel<D, T, true, false><<<(unsigned)blocks, kThreads, 0, s>>>(a);
+    if (interleaved) append_kernel<D, T, true, true, ROWS><<<(unsigned)blocks, kThreads, 0, s>>>(a);
+    else append_kernel<D, T, true, false, ROWS><<<(unsigned)blocks, kThreads, 0, s>>>(a);
   } else {
-    if (interleaved) append_kernel<D, T, false, true><<<(unsigned)blocks, kThreads, 0, s>>>(a);
-    else append_kernel<D, T, false, false><<<(unsigned)blocks, kThreads, 0, s>>>(a);
+    if (interleaved) append_kernel<D, T, false, true, ROWS><<<(unsigned)blocks, kThreads, 0, s>>>(a);
+    else append_kernel<D, T, false, false, ROWS><<<(unsigned)blocks, kThreads, 0, s>>>(a);
   }
   note_launch();
   return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
+}
+
+// One row for each group of lanes while that does not fill the SMs four times over (a call that waits
+// for its memory ends sooner with more of it in flight), else four.
+template <int D, typename T>
+int launch_append(const AppendArgs& a, bool vec, bool interleaved, cudaStream_t s) {
+  const int64_t rows = a.tokens * (a.q_heads + 2 * (int64_t)a.pool.kv_heads);
+  const int64_t resident = (int64_t)sm_count() * (2048 / (D / 8));
+  return rows <= 4 * resident ? launch_rows<D, T, 1>(a, vec, interleaved, s)
+                              : launch_rows<D, T, 4>(a, vec, interleaved, s);
 }
 
 // Values of the rows in `slots`: head_dim / 8 lanes for each row.
@@ -293,7 +338,8 @@ extern "C" int tans_kv4_append(uint8_t* codes, void* params, int64_t num_pages, 
   if (tokens == 0) return TANS_OK;
   if (!q) q_heads = 0;
   if (!k || !v || !slots || (q && (!q_out || q_heads < 1)) || (rotation && !positions)) return TANS_E_INVALID_ARGUMENT;
-  if ((reinterpret_cast<uintptr_t>(q_out) & 15) != 0) return TANS_E_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(rotation)) & 15) != 0)
+    return TANS_E_INVALID_ARGUMENT;  // they are read and written 16 bytes at a time
   cudaStream_t s = reinterpret_cast<cudaStream_t>(cuda_stream);
   const AppendArgs a{codes,
                      static_cast<uint32_t*>(params),

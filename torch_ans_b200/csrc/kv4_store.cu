@@ -42,28 +42,30 @@ struct AppendArgs {
   uint32_t* status;
 };
 
-// 8 consecutive elements of a row, as they are
+// 4 consecutive elements of a row, as they are, and as floats
 template <typename T, bool VEC>
-__device__ __forceinline__ uint4 load8(const T* p) {
-  if constexpr (VEC) return *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ uint2 load4(const T* p) {
+  if constexpr (VEC) return *reinterpret_cast<const uint2*>(p);
   const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
-  return make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16,
-                    u[6] | (uint32_t)u[7] << 16);
+  return make_uint2(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16);
 }
 template <typename T>
-__device__ __forceinline__ void floats(const uint4& w, float (&x)[8]) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Half2<T>::unpack(u[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ void floats(const uint2& w, float2 (&x)[2]) {
+  x[0] = Half2<T>::unpack(w.x);
+  x[1] = Half2<T>::unpack(w.y);
 }
 
-// Rotation and quantisation, head_dim / 8 lanes for each row (one token's head), 8 channels a lane; a
-// group of lanes takes ROWS rows of one token, so that the token's cosines and sines are read once for
-// all of them and the loads of the rows do not wait for one another.
+// (a, b) turned by an angle, every product and sum rounded by itself
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+  const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+  a = x;
+}
+
+// Rotation and quantisation, head_dim / 8 lanes for each row (one token's head), 8 channels a lane in two
+// fours: channels that turn together are in one lane (i and i + rotary / 2, or neighbours), so nothing is
+// exchanged for the rotation.  A group of lanes takes ROWS rows of one token, so that the token's cosines
+// and sines are read once for all of them and the loads of the rows do not wait for one another.
 //
 // What it may not do without is bytes: 2 read and 2 written for a query's channel, 2 read and about 0.53
 // written for a key's or a value's.  16,381 tokens of 32 + 16 heads of 128 (355 MB): see the table of
@@ -77,43 +79,47 @@ __device__ __forceinline__ void floats(const uint4& w, float (&x)[8]) {
 template <int D, typename T, bool VEC, bool INTERLEAVED, int ROWS>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   constexpr int L = D / 8;
-  const int lane = threadIdx.x % L, d0 = lane * 8;
+  const int lane = threadIdx.x % L, half = a.rotary / 2;
+  const bool in_rotary = lane * 8 < a.rotary;
+  const int d0 = !INTERLEAVED && in_rotary ? lane * 4 : lane * 8, d1 = !INTERLEAVED && in_rotary ? d0 + half : d0 + 4;
   const int per_token = a.q_heads + 2 * a.pool.kv_heads, chunks = (per_token + ROWS - 1) / ROWS;
   const int64_t group = blockIdx.x * (int64_t)(kThreads / L) + threadIdx.x / L;
   const int64_t token = min(group / chunks, a.tokens - 1);  // groups past the end keep the warp's shuffles whole
   const int r0 = (int)(group % chunks) * ROWS;
   const int rows = group >= a.tokens * chunks ? 0 : min(ROWS, per_token - r0);
 
-  auto source = [&](int r) -> const T* {  // row r of the token: queries, keys, values
-    if (r < a.q_heads) return static_cast<const T*>(a.q) + token * a.q_ts + r * a.q_hs;
-    r -= a.q_heads;
-    if (r < a.pool.kv_heads) return static_cast<const T*>(a.k) + token * a.k_ts + r * a.k_hs;
-    return static_cast<const T*>(a.v) + token * a.v_ts + (r - a.pool.kv_heads) * a.v_hs;
-  };
-  uint4 raw[ROWS];
+  const T* q_at = static_cast<const T*>(a.q) + token * a.q_ts;
+  const T* k_at = static_cast<const T*>(a.k) + token * a.k_ts - a.q_heads * a.k_hs;
+  const T* v_at = static_cast<const T*>(a.v) + token * a.v_ts - (a.q_heads + a.pool.kv_heads) * a.v_hs;
+  uint2 raw0[ROWS], raw1[ROWS];
 #pragma unroll
-  for (int n = 0; n < ROWS; ++n) raw[n] = n < rows ? load8<T, VEC>(source(r0 + n) + d0) : make_uint4(0, 0, 0, 0);
-
-  const int64_t slot = r0 + rows > a.q_heads ? a.slots[token] : -1;
-  bool known = false;
-  float c[8], s[8];
-  const int half = a.rotary / 2;
-  const bool first = d0 < half;
-  if (a.rotary > 0) {
-    const int64_t pos = a.positions[token];
-    known = pos >= 0 && pos < a.rotation_rows;
-    if (!known && a.status && lane == 0 && r0 == 0 && rows > 0) atomicOr(a.status, TANS_DEV_BAD_INDEX);
-    if (known && d0 < a.rotary) {
-      const float* cosines = a.rotation + pos * a.rotary + (INTERLEAVED ? d0 / 2 : (first ? d0 : d0 - half));
-#pragma unroll
-      for (int i = 0; i < (INTERLEAVED ? 4 : 8); i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(cosines + i), y = *reinterpret_cast<const float4*>(cosines + half + i);
-        c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
-        s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
-      }
+  for (int n = 0; n < ROWS; ++n) {  // rows of the token: queries, keys, values
+    const int r = r0 + n;
+    raw0[n] = raw1[n] = make_uint2(0, 0);
+    if (n < rows) {
+      const T* src = r < a.q_heads ? q_at + r * a.q_hs : (r < a.q_heads + a.pool.kv_heads ? k_at + r * a.k_hs : v_at + r * a.v_hs);
+      raw0[n] = load4<T, VEC>(src + d0);
+      raw1[n] = load4<T, VEC>(src + d1);
     }
   }
-  const bool turns = known && d0 < a.rotary;
+
+  const int64_t slot = r0 + rows > a.q_heads ? a.slots[token] : -1;
+  bool turns = false;
+  float2 c[2], s[2];  // of the lane's four angles
+  if (a.rotary > 0) {
+    const int64_t pos = a.positions[token];
+    const bool known = pos >= 0 && pos < a.rotation_rows;
+    if (!known && a.status && lane == 0 && r0 == 0 && rows > 0) atomicOr(a.status, TANS_DEV_BAD_INDEX);
+    turns = known && in_rotary;
+    if (turns) {
+      const float* cosines = a.rotation + pos * a.rotary + lane * 4;
+      const float4 x = *reinterpret_cast<const float4*>(cosines), y = *reinterpret_cast<const float4*>(cosines + half);
+      c[0] = make_float2(x.x, x.y);
+      c[1] = make_float2(x.z, x.w);
+      s[0] = make_float2(y.x, y.y);
+      s[1] = make_float2(y.z, y.w);
+    }
+  }
   bool stores = slot >= 0;
   if (slot >= a.pool.num_pages * a.pool.page_size) {
     stores = false;
@@ -126,45 +132,29 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   for (int n = 0; n < ROWS; ++n) {
     const int r = r0 + n;
     const bool live = n < rows, query = r < a.q_heads, value = r >= a.q_heads + a.pool.kv_heads;
-    float x[8];
-    floats<T>(raw[n], x);
-    if constexpr (INTERLEAVED) {
-      if (turns && !value) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = x[2 * i], w = x[2 * i + 1];
-          x[2 * i] = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(w, s[i]));
-          x[2 * i + 1] = __fadd_rn(__fmul_rn(w, c[i]), __fmul_rn(u, s[i]));
-        }
-      }
-    } else if (a.rotary > 0) {
-      // the partner channels are half / 8 lanes away
-      const int warp_lane = threadIdx.x & 31;
-      const int partner = d0 < a.rotary ? (first ? warp_lane + half / 8 : warp_lane - half / 8) : warp_lane;
-      uint4 w;
-      w.x = __shfl_sync(0xffffffffu, raw[n].x, partner);
-      w.y = __shfl_sync(0xffffffffu, raw[n].y, partner);
-      w.z = __shfl_sync(0xffffffffu, raw[n].z, partner);
-      w.w = __shfl_sync(0xffffffffu, raw[n].w, partner);
-      if (turns && !value) {
-        float y[8];
-        floats<T>(w, y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float xc = __fmul_rn(x[i], c[i]), ys = __fmul_rn(y[i], s[i]);
-          x[i] = first ? __fsub_rn(xc, ys) : __fadd_rn(xc, ys);
-        }
+    float2 u[2], w[2];  // the lane's fours
+    floats<T>(raw0[n], u);
+    floats<T>(raw1[n], w);
+    if (turns && !value) {
+      if constexpr (INTERLEAVED) {
+        turn(u[0].x, u[0].y, c[0].x, s[0].x);
+        turn(u[1].x, u[1].y, c[0].y, s[0].y);
+        turn(w[0].x, w[0].y, c[1].x, s[1].x);
+        turn(w[1].x, w[1].y, c[1].y, s[1].y);
+      } else {
+        turn(u[0].x, w[0].x, c[0].x, s[0].x);
+        turn(u[0].y, w[0].y, c[0].y, s[0].y);
+        turn(u[1].x, w[1].x, c[1].x, s[1].x);
+        turn(u[1].y, w[1].y, c[1].y, s[1].y);
       }
     }
     if (query && live) {
-      uint4 w;
-      w.x = Half2<T>::pack(x[0], x[1]);
-      w.y = Half2<T>::pack(x[2], x[3]);
-      w.z = Half2<T>::pack(x[4], x[5]);
-      w.w = Half2<T>::pack(x[6], x[7]);
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (token * a.q_heads + r) * D + d0) = w;
+      T* dst = static_cast<T*>(a.q_out) + (token * a.q_heads + r) * D;
+      *reinterpret_cast<uint2*>(dst + d0) = make_uint2(Half2<T>::pack(u[0].x, u[0].y), Half2<T>::pack(u[1].x, u[1].y));
+      *reinterpret_cast<uint2*>(dst + d1) = make_uint2(Half2<T>::pack(w[0].x, w[0].y), Half2<T>::pack(w[1].x, w[1].y));
     }
     if (__all_sync(0xffffffffu, query || !live || !stores)) continue;
+    const float x[8] = {u[0].x, u[0].y, u[1].x, u[1].y, w[0].x, w[0].y, w[1].x, w[1].y};
 
     // the row's range, then its codes
     float lo = x[0], hi = x[0];
@@ -199,7 +189,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     }
     const int kv = r - a.q_heads, side = value, head = value ? kv - a.pool.kv_heads : kv;
     const int64_t at = a.pool.row(page, side, head) + in_page;
-    *reinterpret_cast<uint32_t*>(a.codes + at * (D / 2) + lane * 4) = packed;
+    *reinterpret_cast<uint16_t*>(a.codes + at * (D / 2) + d0 / 2) = (uint16_t)packed;
+    *reinterpret_cast<uint16_t*>(a.codes + at * (D / 2) + d1 / 2) = (uint16_t)(packed >> 16);
     if (lane == 0) a.params[at] = finite ? (__float_as_uint(scale) >> 16) | __float_as_uint(offset) : 0x7fff7fffu;
   }
 }

@@ -120,22 +120,26 @@ __device__ __forceinline__ void join_parts(const Join& j, int first_place, int f
     weight[count + i][row] = st.y;
   }
   __syncthreads();
-  if (threadIdx.x < R) {
-    const int row = threadIdx.x;
+  for (int row = threadIdx.x >> 5; row < R; row += kWarps) {
+    const int lane = threadIdx.x & 31;
     float m = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < count; ++i) m = fmaxf(m, weight[i][row]);
+    for (int i = lane; i < count; i += 32) m = fmaxf(m, weight[i][row]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.0f : m;
-    for (int i = 0; i < count; ++i) {
+    for (int i = lane; i < count; i += 32) {
       const float w = ex2(weight[i][row] - base);
       weight[i][row] = w;
       sum += w * weight[count + i][row];
     }
-    total[row] = make_float2(m, sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) total[row] = make_float2(m, sum);
   }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < Sums<D, R>::N; ++e) sums.v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+#pragma unroll(Sums<D, R>::N == 1 ? 16 : 8)
   for (int i = 0; i < count; ++i) {
     const float4* part = reinterpret_cast<const float4*>(j.parts + (int64_t)place(i) * R * D);
 #pragma unroll
@@ -169,9 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
   // ---- this block's share of the work: the steps of every sequence, row tile and head, and a few
   // for each of these items' start and end
   auto steps_of = [&](const Sequence& s) { return (s.length + kStep - 1) / kStep + kItemSteps; };
-  auto units_of = [&](const Sequence& s) {
-    return (int64_t)((s.count * a.group.d + R - 1) / R) * heads * steps_of(s);
-  };
+  auto items_of = [&](const Sequence& s) { return (int64_t)((s.count * a.group.d + R - 1) / R) * heads; };
   auto block_scan = [&](int64_t v, int64_t& total) {  // sum of v over the threads before this one
     int64_t x = v;
 #pragma unroll
@@ -192,15 +194,18 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     return before + x - v;
   };
   const int batch = (int)a.batch;
-  int64_t all = 0, mine, before;
+  int64_t all = 0, items = 0, mine = 0, before = 0;
   Sequence seq{0, 0, 0};
   for (int b = 0; b < batch; b += kWarps * 32) {
     int64_t sum;
     mine = 0;
     if (b + (int)threadIdx.x < batch) {
       seq = sequence(a, b + threadIdx.x, blockIdx.x == 0);
-      mine = units_of(seq);
+      mine = items_of(seq);
     }
+    block_scan(mine, sum);
+    items += sum;
+    mine *= steps_of(seq);
     before = all + block_scan(mine, sum);
     all += sum;
   }
@@ -208,16 +213,32 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     if (blockIdx.x == 0 && threadIdx.x == 0) flag(a.status, TANS_DEV_BAD_VALUE);
     return;
   }
-  const int share = max(((int)all + (int)gridDim.x - 1) / (int)gridDim.x, kWarps + kItemSteps);
+  // With fewer items than half the blocks, each item has blocks of its own: as many as take `share` or
+  // less each, its steps spread evenly over them.  These are at most all / share + items blocks.  Else the
+  // blocks' shares follow one another across the items.  From here a sequence's extent is counted in
+  // blocks or in units of work.
+  const bool own = items < (int)gridDim.x / 2;
+  const int sharers = own ? (int)(gridDim.x - items) : (int)gridDim.x;
+  const int share = max(((int)all + sharers - 1) / sharers, kWarps + kItemSteps);
+  auto extent_of = [&](const Sequence& s) { return own ? (steps_of(s) + share - 1) / share : steps_of(s); };
+  if (own && batch <= kWarps * 32) {
+    mine = threadIdx.x < batch ? items_of(seq) * extent_of(seq) : 0;
+    before = block_scan(mine, all);
+  } else if (own) {
+    all = (int64_t)1 << 40;  // known when the end is reached
+  }
   auto zero_rest = [&]() {
     zero_unowned<T>(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32);
   };
-  if ((int64_t)blockIdx.x * share >= all) {
+  const int64_t start = (int64_t)blockIdx.x * (own ? 1 : share);
+  if (start >= all) {
     zero_rest();
     return;
   }
-  int u = blockIdx.x * share;
-  const int u_end = (int)min(all, (int64_t)u + share);
+  int u = (int)start;
+  const int u_end = (int)min(all, start + (own ? 1 : share));
+  if (threadIdx.x == 0) sh_found[0] = -1;
+  __syncthreads();
   int64_t done = 0;
   for (int b = 0; b < batch; b += kWarps * 32) {
     if (batch > kWarps * 32) {  // more sequences than threads: once more from the start
@@ -225,7 +246,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
       mine = 0;
       if (b + (int)threadIdx.x < batch) {
         seq = sequence(a, b + threadIdx.x, false);
-        mine = units_of(seq);
+        mine = items_of(seq) * extent_of(seq);
       }
       before = done + block_scan(mine, sum);
       done += sum;
@@ -240,6 +261,10 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
   __syncthreads();
   int b = sh_found[0], b_first = sh_found[1];
   seq = sh_sequence;
+  if (b < 0) {
+    zero_rest();
+    return;
+  }
 
   uint8_t* ring = smem + warp * kStages * S::BYTES;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
@@ -263,15 +288,16 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
   }
 
   while (u < u_end) {
-    while (u >= b_first + units_of(seq)) {  // sequences without queries have no units
-      b_first += (int)units_of(seq);
+    while (u >= b_first + items_of(seq) * extent_of(seq)) {  // sequences without queries have no extent
+      b_first += (int)(items_of(seq) * extent_of(seq));
       ++b;
       seq = sequence(a, b, false);
     }
-    const int units = steps_of(seq), steps = units - kItemSteps;
-    const int item = (u - b_first) / units, item_first = b_first + item * units;
-    const int unit1 = min(units, u_end - item_first);
-    const int step0 = max(0, u - item_first - kItemSteps), step1 = max(0, unit1 - kItemSteps);
+    const int extent = extent_of(seq), steps = steps_of(seq) - kItemSteps;
+    const int item = (u - b_first) / extent, item_first = b_first + item * extent;
+    const int u_next = min(item_first + extent, u_end);
+    const int step0 = own ? (int)((int64_t)(u - item_first) * steps / extent) : max(0, u - item_first - kItemSteps);
+    const int step1 = own ? (int)((int64_t)(u_next - item_first) * steps / extent) : max(0, u_next - item_first - kItemSteps);
     const int tile = a.kv_heads.div(item), head = item - tile * heads;
     const int row0 = tile * R, rows = min(R, seq.count * (int)a.group.d - row0);
 
@@ -646,10 +672,11 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     __syncthreads();  // the rings may be filled again
 
     // ---- whole here, or joined with the other blocks' parts
-    bool whole = u == item_first && unit1 == units;
+    bool whole = u == item_first && u_next == item_first + extent;
     if (!whole) {
       const Join& j = p.join;
-      const int c0 = item_first / share, c1 = (item_first + units - 1) / share;
+      const int c0 = own ? item_first : item_first / share;
+      const int c1 = own ? item_first + extent - 1 : (item_first + extent - 1) / share;
       auto leave = [&](int place) {
 #pragma unroll
         for (int e = 0; e < Part::N; ++e)
@@ -668,15 +695,15 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
       };
       const int me = blockIdx.x;
       leave(me * 2 + (me == c0));
-      const int f0 = max(c0, me / kFan * kFan), f1 = min(c1, me / kFan * kFan + kFan - 1);  // this block's group
+      const int f0 = c0 + (me - c0) / kFan * kFan, f1 = min(c1, f0 + kFan - 1);  // this block's group
       const int place = f0 * 2 + (f0 == c0);
       whole = f1 == f0 || last_of(0, place, f1 - f0 + 1);
       if (whole && f1 > f0) join_parts<D, R>(j, place, f0, f1 - f0 + 1, 1, sh_weight, sh_total, sums);
       if (whole && (f0 != c0 || f1 != c1)) {  // the groups
         if (f1 > f0) leave(place);
-        const int first_group = c0 / kFan, groups = c1 / kFan - first_group + 1;
+        const int groups = (c1 - c0) / kFan + 1;
         whole = last_of(1, c0 * 2 + 1, groups);
-        if (whole) join_parts<D, R>(j, c0 * 2 + 1, first_group * kFan, groups, kFan, sh_weight, sh_total, sums);
+        if (whole) join_parts<D, R>(j, c0 * 2 + 1, c0, groups, kFan, sh_weight, sh_total, sums);
       }
     }
     if (whole) {
@@ -697,7 +724,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
       }
       __syncthreads();  // the totals may be written again
     }
-    u = item_first + unit1;
+    u = u_next;
   }
   zero_rest();
 }

@@ -288,7 +288,7 @@ int tans_kv4_gather(const uint8_t* codes, const void* params, int64_t num_pages,
  *             TANS_KV4_ATTEND_COUNTS bytes are zero before the first call and are left zero by each
  *             call; calls that may overlap need workspaces of their own.  NULL allocates and clears
  *             one stream-ordered. */
-#define TANS_KV4_ATTEND_COUNTS 7680
+#define TANS_KV4_ATTEND_COUNTS 10240
 size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim, int64_t batch,
                                       int64_t max_pages, int page_size, int64_t max_queries);
 int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t total_queries, int q_heads,

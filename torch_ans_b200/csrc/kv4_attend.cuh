@@ -98,8 +98,8 @@ __device__ __forceinline__ float pow2(int x) { return __int_as_float((x + 127) <
 // before), and the last of them to arrive joins them, in the order of the blocks whatever the order
 // of arrival, so results repeat.  Over kFan blocks join in two levels.  The counts of arrivals are
 // zero between launches: the last arrival takes its count back.
-constexpr int kFan = 64;
-constexpr int kMostBlocks = 3 * 160;  // blocks that a workspace has places for
+constexpr int kFan = 32;
+constexpr int kMostBlocks = 4 * 160;  // blocks that a workspace has places for
 
 struct Join {
   int* arrivals;  // [2 levels][kMostBlocks][2]

@@ -34,7 +34,7 @@ namespace tans {
 namespace kv4 {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kStep = 32;   // tokens a warp takes at a time
 constexpr int kStages = 3;  // steps in flight for each warp, the one in use among them
 constexpr float kSlack = 8.0f;
@@ -156,7 +156,7 @@ __device__ __forceinline__ void join_parts(const Join& j, int first_place, int f
 }
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_rows_kernel(const RowsArgs p) {
+__global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_rows_kernel(const RowsArgs p) {
   const AttendArgs& a = p.a;
   using S = Stage<D>;
   constexpr int R = 8 * NT, KW = D / 32, VW = D / 64;  // rows of a tile; words of a key / value row's share of a lane
@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     }
     return before + x - v;
   };
+  constexpr int64_t kUnits = ((int64_t)1 << 40) - 1;
   const int batch = (int)a.batch;
   int64_t all = 0, items = 0, mine = 0, before = 0;
   Sequence seq{0, 0, 0};
@@ -201,13 +202,14 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     mine = 0;
     if (b + (int)threadIdx.x < batch) {
       seq = sequence(a, b + threadIdx.x, blockIdx.x == 0);
-      mine = items_of(seq);
+      // units and items in one sum: no sequence within memory reaches these bounds
+      mine = min(items_of(seq), (int64_t)1 << 20);
+      mine = min(items_of(seq) * steps_of(seq), (int64_t)1 << 31) | mine << 40;
     }
-    block_scan(mine, sum);
-    items += sum;
-    mine *= steps_of(seq);
-    before = all + block_scan(mine, sum);
-    all += sum;
+    before = all + (block_scan(mine, sum) & kUnits);
+    all += sum & kUnits;
+    items += sum >> 40;
+    mine &= kUnits;
   }
   if (all > 0x7f000000) {  // starts that cross one another: no call within memory has so much work
     if (blockIdx.x == 0 && threadIdx.x == 0) flag(a.status, TANS_DEV_BAD_VALUE);
@@ -301,6 +303,28 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     const int tile = a.kv_heads.div(item), head = item - tile * heads;
     const int row0 = tile * R, rows = min(R, seq.count * (int)a.group.d - row0);
 
+    // ---- this lane's quarters of the query rows, row g of each 8; they are turned to float16 below
+    uint4 raw[NT][D / 32];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) raw[n][c] = make_uint4(0, 0, 0, 0);
+      if (n * 8 + g < rows) {
+        const int r = row0 + n * 8 + g, i = a.group.div(r), h = head * a.group.d + (r - i * a.group.d);
+        const T* src = static_cast<const T*>(a.q) + (seq.start + i) * a.q_ts + h * a.q_hs + t * (D / 4);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          if (a.vec) {
+            raw[n][c] = *reinterpret_cast<const uint4*>(src + c * 8);
+          } else {
+            const uint16_t* u = reinterpret_cast<const uint16_t*>(src + c * 8);
+            raw[n][c] = make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16,
+                                   u[6] | (uint32_t)u[7] << 16);
+          }
+        }
+      }
+    }
+
     // ---- steps of this warp: step0 + warp, + kWarps, ...; kStages - 1 of them on their way
     uint32_t known = 0;  // two bits a step in flight, the newest lowest: the group's page is one of the pool
     const int64_t side_bytes = (int64_t)heads * page_size * S::ROW;  // from a page's keys to its values, and half a page
@@ -374,31 +398,16 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 2 : 1) attend_row
     int seen[NT][2];                 // tokens that the columns' queries see
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = row0 + n * 8 + g;
-      const bool live = n * 8 + g < rows;
       float x[D / 4];
-      if (live) {
-        const int i = a.group.div(r), h = head * a.group.d + (r - i * a.group.d);
-        const T* src = static_cast<const T*>(a.q) + (seq.start + i) * a.q_ts + h * a.q_hs + t * (D / 4);
-        if (a.vec) {
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(src + c * 8);
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+      for (int c = 0; c < D / 32; ++c) {
+        const uint32_t v[4] = {raw[n][c].x, raw[n][c].y, raw[n][c].z, raw[n][c].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = Half2<T>::unpack(v[e]);
-              x[c * 8 + 2 * e] = f.x;
-              x[c * 8 + 2 * e + 1] = f.y;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < D / 4; ++c) x[c] = Half2<T>::load(src + c);
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = Half2<T>::unpack(v[e]);
+          x[c * 8 + 2 * e] = f.x;
+          x[c * 8 + 2 * e + 1] = f.y;
         }
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 4; ++c) x[c] = 0.0f;
       }
       float top = 0.0f, sum = 0.0f;
 #pragma unroll

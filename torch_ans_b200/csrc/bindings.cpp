@@ -791,7 +791,7 @@ void kv4_codes_ok(const Tensor& codes) {
   const int64_t dim = 2 * codes.size(4);
   TORCH_CHECK(dim == 64 || dim == 128 || dim == 256, "torch_ans_b200: head_dim must be 64, 128 or 256, not ", dim);
   TORCH_CHECK(codes.size(3) >= 16 && codes.size(3) % 16 == 0 && codes.size(3) <= (1 << 20) && codes.size(2) >= 1 &&
-                  codes.size(2) <= 65535,
+                  codes.size(2) <= 65535 && codes.size(2) * codes.size(3) < (1 << 30),
               "torch_ans_b200: page_size must be a multiple of 16 and kv_heads at least 1");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "torch_ans_b200: `codes` must be 16-byte aligned");
 }

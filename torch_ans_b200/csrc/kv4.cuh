@@ -62,7 +62,7 @@ struct Half2<__half> {
 inline bool pool_ok(const void* codes, const void* params, int64_t num_pages, int kv_heads, int page_size,
                     int head_dim) {
   if (num_pages < 0 || kv_heads < 1 || kv_heads > 65535 || page_size < 16 || page_size > (1 << 20) ||
-      page_size % 16 != 0)
+      page_size % 16 != 0 || (int64_t)kv_heads * page_size >= ((int64_t)1 << 30))
     return false;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return false;
   if (num_pages > 0 && (!codes || !params)) return false;

@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
 
     // ---- steps of this warp: step0 + warp, + kWarps, ...; kStages - 1 of them on their way
     uint32_t known = 0;  // two bits a step in flight, the newest lowest: the group's page is one of the pool
-    const int64_t side_bytes = (int64_t)heads * page_size * S::ROW;  // from a page's keys to its values, and half a page
+    const uint32_t side_rows = (uint32_t)heads * page_size;  // from a page's keys to its values, and half a page (< 2^31)
     const uint8_t* head_codes = a.pool.codes + (int64_t)head * page_size * S::ROW + lane * 16;
     const uint32_t* head_params =
         a.pool.params + ((lane >= 4 ? heads : 0) + (int64_t)head) * page_size + (lane & 3) * 4;
@@ -362,9 +362,9 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           const bool there = (unsigned)page[h] < (unsigned)a.pool.num_pages;
           if (!there && lane == 0 && next * kStep + h * 16 < seq.length) flag(a.status, TANS_DEV_BAD_INDEX);
           if (there) bits |= 1u << h;
-          const int64_t pg = there ? page[h] : 0;
-          const uint8_t* ks = head_codes + pg * (2 * side_bytes) + h_first * S::ROW;
-          const uint8_t* vs = ks + side_bytes;
+          const uint64_t page_row = (uint64_t)(there ? page[h] : 0) * (2 * side_rows);
+          const uint8_t* ks = head_codes + (page_row + h_first) * S::ROW;
+          const uint8_t* vs = ks + (uint64_t)side_rows * S::ROW;
 #pragma unroll
           for (int i = 0; i < S::COPIES; ++i) {
             cp16(base + S::K + h * 16 * S::ROW + copy_at[i], ks + i * 512, there);
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           }
           if (lane < 8)  // keys' parameters, then values'
             cp16(base + S::KP + (lane >> 2) * kStep * 4 + h * 64 + (lane & 3) * 16,
-                 head_params + pg * (2 * (int64_t)heads * page_size) + h_first, there);
+                 head_params + page_row + h_first, there);
           h_first += 16;
           if (h_first == page_size) h_first = 0;
         }

@@ -342,6 +342,28 @@ def test_attend_is_reproducible_on_other_streams_and_in_graphs(C, count):
     del g
 
 
+@pytest.mark.parametrize("lengths,counts", [([700, 300], [700, 300]), ([9000], [300])])
+def test_attend_wait_that_runs_out_is_reported(C, monkeypatch, lengths, counts):
+    """Waits between a block's warps are bounded: one that runs out ends the call and flags TANS_DEV_STALLED, and the
+    next call on the same stream is right."""
+    pages, total = P.table(lengths, 16)
+    codes, params = P.pool(total, 2, 16, 128)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    starts = [sum(counts[:b]) for b in range(len(counts) + 1)]
+    q = torch.randn(starts[-1], 8, 128, device="cuda", generator=gen(1)).to(BF)
+    call = lambda: C.kv4_attend(q, codes, params, pages, torch.tensor(lengths, **i32),  # noqa: E731
+                                q_starts=torch.tensor(starts, **i32))
+    first = call()
+    torch.cuda.synchronize()
+    assert C.device_status() == 0
+    monkeypatch.setenv("TORCH_ANS_B200_WAIT_LIMIT", "0")
+    call()
+    torch.cuda.synchronize()  # returns: no warp is still waiting
+    assert C.device_status() & 64
+    monkeypatch.delenv("TORCH_ANS_B200_WAIT_LIMIT")
+    assert torch.equal(call(), first) and C.device_status() == 0
+
+
 @pytest.mark.parametrize("n,kv,page,dim,by_channel", [(1, 1, 16, 64, False), (5, 3, 48, 128, True), (9, 8, 64, 256, False)])
 def test_symbols(C, n, kv, page, dim, by_channel):
     codes, _ = P.pool(n + 4, kv, page, dim, n)

@@ -60,7 +60,27 @@ std::string status_bits_string(uint32_t bits) {
   if (bits & TANS_DEV_UNDERFLOW) s += " stream-underflow";
   if (bits & TANS_DEV_BAD_FREQ) s += " zero-frequency";
   if (bits & TANS_DEV_BAD_ESCAPE) s += " corrupt-escape";
+  if (bits & TANS_DEV_STALLED) s += " stalled";
   return s;
+}
+
+// Attention workspaces by device and stream (kv4_workspace); never freed: no CUDA calls at exit.
+struct Kept {
+  std::mutex mu;
+  std::map<std::pair<int, cudaStream_t>, Tensor> by_stream;
+};
+Kept& kept_workspaces() {
+  static Kept& k = *new Kept;
+  return k;
+}
+
+// A call that stalled may have left its workspace's counts as they were: the next one gets a new one.
+void after_stall(int device, int32_t bits) {
+  if (!(bits & (int32_t)TANS_DEV_STALLED)) return;
+  Kept& k = kept_workspaces();
+  std::lock_guard<std::mutex> g(k.mu);
+  for (auto it = k.by_stream.begin(); it != k.by_stream.end();)
+    it = it->first.first == device ? k.by_stream.erase(it) : std::next(it);
 }
 
 void after_op(const at::Device& dev) {
@@ -69,6 +89,7 @@ void after_op(const at::Device& dev) {
   const int32_t bits = w.item<int32_t>();  // synchronises the current stream
   if (bits != 0) {
     w.zero_();
+    after_stall(dev.index(), bits);
     throw std::runtime_error("torch_ans_b200: device reported:" + status_bits_string((uint32_t)bits));
   }
 }
@@ -899,20 +920,19 @@ Tensor kv4_workspace(const at::Device& dev, int64_t bytes) {
   const auto stream = at::cuda::getCurrentCUDAStream(dev.index());
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   TORCH_CHECK(cudaStreamIsCapturing(stream.stream(), &capture) == cudaSuccess, "torch_ans_b200: no capture status");
-  static std::mutex mu;
-  static auto& kept = *new std::map<std::pair<int, cudaStream_t>, Tensor>();  // never freed: no CUDA calls at exit
   const bool captured = capture != cudaStreamCaptureStatusNone;
-  Tensor ws;
+  Kept& k = kept_workspaces();
+  const std::pair<int, cudaStream_t> key{dev.index(), stream.stream()};
   if (!captured) {
-    std::lock_guard<std::mutex> g(mu);
-    auto it = kept.find({dev.index(), stream.stream()});
-    if (it != kept.end() && it->second.numel() >= bytes) return it->second;
+    std::lock_guard<std::mutex> g(k.mu);
+    auto it = k.by_stream.find(key);
+    if (it != k.by_stream.end() && it->second.numel() >= bytes) return it->second;
   }
-  ws = torch::empty({bytes}, opt);
+  Tensor ws = torch::empty({bytes}, opt);
   ws.narrow(0, 0, TANS_KV4_ATTEND_COUNTS).zero_();
   if (!captured) {
-    std::lock_guard<std::mutex> g(mu);
-    kept[{dev.index(), stream.stream()}] = ws;
+    std::lock_guard<std::mutex> g(k.mu);
+    k.by_stream[key] = ws;
   }
   return ws;
 }
@@ -1000,7 +1020,10 @@ int64_t device_status(std::optional<int64_t> device, bool reset) {
   const int64_t d = device.has_value() ? *device : (int64_t)c10::cuda::current_device();
   Tensor& w = status_word(at::Device(at::kCUDA, (c10::DeviceIndex)d));
   const int32_t v = w.item<int32_t>();
-  if (reset) w.zero_();
+  if (reset) {
+    w.zero_();
+    after_stall((int)d, v);
+  }
   return v;
 }
 

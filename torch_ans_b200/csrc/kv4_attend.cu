@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "kv4_attend.cuh"
+#include "launch.cuh"
 #include "rans_host.h"
 
 static_assert(tans::kv4::Join::kArrivalBytes == TANS_KV4_ATTEND_COUNTS, "the header names the size");
@@ -49,7 +50,8 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
   const AttendArgs a{Pool{codes, static_cast<const uint32_t*>(params), num_pages, kv_heads, page_size, head_dim},
                      q, q_token_stride, q_head_stride, total_queries, q_heads,
                      Divider::of(group), Divider::of(kv_heads), Divider::of(page_size), pages, batch, max_pages, lengths,
-                     q_starts, scale * 1.4426950408889634f, causal, vec, out, lse, dev_status};
+                     q_starts, scale * 1.4426950408889634f, causal, vec, out, lse, dev_status,
+                     tans::env_int("TORCH_ANS_B200_WAIT_LIMIT", 1 << 20)};
   const int64_t most = std::min(max_queries, total_queries);
   const size_t need = tans_kv4_attend_workspace_size(total_queries, q_heads, kv_heads, head_dim, batch, max_pages,
                                                      page_size, max_queries);

@@ -37,6 +37,7 @@ struct AttendArgs {
   void* out;
   float* lse;
   uint32_t* status;
+  int wait_limit;  // tries of a wait of one warp for another, a microsecond each at most
 };
 
 // One sequence: its tokens, its queries (first and number).

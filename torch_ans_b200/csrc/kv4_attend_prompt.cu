@@ -40,7 +40,7 @@ constexpr int kTile = 128;  // rows of a tile, tokens of a step
 constexpr int kHalf = 64;   // tokens of a half step
 constexpr float kSlack = 8.0f;
 constexpr int kInfos = 4;   // steps whose factors are kept: the unpacking warps run at most 2 ahead
-constexpr int kTries = 1 << 20;
+constexpr int kTries = 1 << 20;  // of the last wait
 
 template <int D>
 struct Plan {
@@ -89,7 +89,7 @@ __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
 }
 // A bounded wait.  One that runs out is recorded in `stalled`; waits after that return at once, so the
 // block comes to its end (with values that are not valid) and frees its tensor memory.
-__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatile int* stalled) {
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, int tries, volatile int* stalled) {
   const uint32_t at = smem_of(bar);
   uint32_t done;
   asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}\n"
@@ -97,7 +97,7 @@ __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatil
                : "r"(at), "r"(parity)
                : "memory");
   if (done) return;
-  for (int i = 0; i < kTries; ++i) {
+  for (int i = 0; i < tries; ++i) {
     asm volatile(
         "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n"
         : "=r"(done)
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     for (int64_t b = threadIdx.x; b < a.batch; b += P::WARPS * 32) sequence(a, b, true);
   // A group's next piece of work, and its return once it is read by the whole warp.
   auto take = [&](int number) -> const Work& {
-    bar_wait(&w_full[number % kQueue], number / kQueue & 1, stalled);
+    bar_wait(&w_full[number % kQueue], number / kQueue & 1, a.wait_limit, stalled);
     __syncwarp();
     return queue[number % kQueue];
   };
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     int shift = 0;
     uint32_t x[2][32];
     auto scores_of = [&](int n) {  // half step n's are there
-      bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, stalled);
+      bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, a.wait_limit, stalled);
       __syncwarp();
       fence_after();
     };
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
         l *= keep;
         if (n > 0) {  // O is not yet written before the first half step, and at rest after the last one's
-          bar_wait(&o_done[tile], (done0 + done1 + n - 1) & 1, stalled);
+          bar_wait(&o_done[tile], (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
           __syncwarp();
           fence_after();
           const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     const int64_t o = (int64_t)(k.seq.start + i) * a.q_heads + h;
     const int tile_head = k.tile_head, part = k.part, parts = SPLIT ? k.parts : 1;
     if (halves > 0) {
-      bar_wait(&o_full, items & 1, stalled);
+      bar_wait(&o_full, items & 1, a.wait_limit, stalled);
       __syncwarp();
       fence_after();
     }
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     for (uint32_t j = 0; there; ++j) {
       if (begun) {
         value_top = 27;
-        if (items > 0) bar_wait(&q_empty, (items - 1) & 1, stalled);
+        if (items > 0) bar_wait(&q_empty, (items - 1) & 1, a.wait_limit, stalled);
         __syncwarp();
         copy_queries(queue[slot_now % kQueue]);
         give_back(slot_now);
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         value_top = max(value_top, top_v[j & 1][w]);
       }
       const int key_shift = kReach - (int)key_top, value_shift = kReach - (int)value_top;
-      bar_wait(&k_empty[stage], filled ^ 1, stalled);
+      bar_wait(&k_empty[stage], filled ^ 1, a.wait_limit, stalled);
       Info& info = infos[j & (kInfos - 1)];
       if (lane == 0 && part_of_row == 0) {
         info.key_shift = key_shift;  // the same in all
@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       slot_now = slot;
       there = valid;
       look_up();
-      bar_wait(&v_empty[stage], filled ^ 1, stalled);
+      bar_wait(&v_empty[stage], filled ^ 1, a.wait_limit, stalled);
       spread(vc, value_params, value_shift, smem + P::V + stage * P::ROWS);
       fence_smem();
       bar_arrive(&v_full[stage]);
@@ -859,8 +859,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         give_back(number);
         if (!some) break;
         if (steps <= 0) continue;
-        bar_wait(&q_full, items & 1, stalled);
-        bar_wait(&k_full[stage], filled, stalled);
+        bar_wait(&q_full, items & 1, a.wait_limit, stalled);
+        bar_wait(&k_full[stage], filled, a.wait_limit, stalled);
         fence_after();
 #pragma unroll 1
         for (int n = 0; n < min(2, halves); ++n)
@@ -875,15 +875,15 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         for (int n = 0; n < halves; ++n) {
           const int h = n & 1, next = stage + 1 == STAGES ? 0 : stage + 1;
           const uint32_t phase = ((h ? done1 : done0) + (n >> 1)) & 1, next_filled = filled ^ (next == 0);
-          if (h == 0) bar_wait(&v_full[stage], filled, stalled);
+          if (h == 0) bar_wait(&v_full[stage], filled, a.wait_limit, stalled);
 #pragma unroll
           for (int tile = 0; tile < TILES; ++tile) {
-            bar_wait(&p_full[tile][h], phase, stalled);
+            bar_wait(&p_full[tile][h], phase, a.wait_limit, stalled);
             fence_after();
             values(tile, stage, h, n > 0);
             if (n + 2 < halves) {
               if (h == 0 && tile == 0) {
-                bar_wait(&k_full[next], next_filled, stalled);
+                bar_wait(&k_full[next], next_filled, a.wait_limit, stalled);
                 fence_after();
               }
               scores(tile, next, h);
@@ -909,7 +909,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       }
       // nothing is in flight when the tensor memory is given back, even after a wait that ran out
       volatile int late = 0;
-      if (items > 0) bar_wait(&o_full, (items - 1) & 1, &late);
+      if (items > 0) bar_wait(&o_full, (items - 1) & 1, kTries, &late);
     } else if (warp == kIssue + 1) {
       // ---------------------------------------------------------------- scheduling
       // The first pieces are the blocks' by their numbers, the others whoever's is free: pieces of a
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
           n = SPLIT ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
           continue;
         }
-        bar_wait(&w_empty[number % kQueue], number / kQueue & 1 ^ 1, stalled);
+        bar_wait(&w_empty[number % kQueue], number / kQueue & 1 ^ 1, a.wait_limit, stalled);
         if (lane == 0) {
           queue[number % kQueue] = w;
           bar_arrive(&w_full[number % kQueue]);
@@ -931,7 +931,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         __syncwarp();
         if (!w.some) break;
         // one that is taken earlier than it is needed may be one that another block would end sooner
-        bar_wait(&w_next, number & 1, stalled);
+        bar_wait(&w_next, number & 1, a.wait_limit, stalled);
         ++number;
         n = SPLIT || *stalled ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
       }

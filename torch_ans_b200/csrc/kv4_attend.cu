@@ -11,8 +11,13 @@
 static_assert(tans::kv4::Join::kArrivalBytes == TANS_KV4_ATTEND_COUNTS, "the header names the size");
 
 namespace {
-// rows of queries that share a key/value head
-bool few_rows(int64_t rows) { return rows <= 32; }
+// Whether the kernel that is bound by the cache's bytes takes the call: `rows` query rows at most share a
+// key/value head.  It reads the cache once for each 8 or 16 of them, the other unpacks it once for 128 or
+// 256.  Measured for head_dim 64, 128, 256: 16 contexts of 8,192 tokens with 4 heads, 32 rows 50, 60 and
+// 109 us against 72, 81 and 205, 64 rows 85, 98 and 200 us against 101, 114 and 205, 96 rows 111, 138 and
+// 290 us against 101, 115 and 258; 64 contexts of 700 tokens with 8 heads, 32 rows 44, 60 and 110 us
+// against 56, 66 and 117, 64 rows 74, 99 and 204 us against 56, 67 and 119.
+bool few_rows(int64_t rows) { return rows <= 48; }
 }  // namespace
 
 extern "C" size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim,

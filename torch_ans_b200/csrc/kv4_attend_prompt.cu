@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     const Work& k = take(number);  // read again where it is used: registers are dear here
     if (!k.some || *stalled) break;
     const int seen = row >= k.rows ? 0 : (a.causal ? min(k.seq.length, k.ahead + a.group.div(k.row0 + row)) : k.seq.length);
-    const int halves = k.halves;
+    const int halves = tile * kTile < k.rows ? k.halves : 0;  // a tile without rows has nothing to wait for
     int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
     float m = -INFINITY, l = 0.0f;
     bool poisoned = false;
@@ -588,13 +588,13 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     }
     if (live && a.lse && (parts == 1 || sh_last))
       a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-    if (halves > 0) {
-      done0 += (halves + 1) >> 1;
-      done1 += halves >> 1;
+    done0 += (halves + 1) >> 1;
+    done1 += halves >> 1;
+    if (k.halves > 0) {
       steps_done += k.steps;
       ++items;
-      fence_before();
     }
+    fence_before();
     if (SPLIT) break;
     give_back(number);
     }
@@ -850,11 +850,11 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         __syncwarp();
       };
       int stage = 0;
-      uint32_t filled = 0, items = 0, done0 = 0, done1 = 0;
+      uint32_t filled = 0, items = 0, done0[TILES] = {}, done1[TILES] = {};
 #pragma unroll 1
       for (int number = 0;; ++number) {
         const Work& k = take(number);
-        const int steps = k.steps, halves = k.halves;
+        const int steps = k.steps, halves = k.halves, tiles = (k.rows + kTile - 1) / kTile;
         const bool some = k.some && !*stalled;
         give_back(number);
         if (!some) break;
@@ -865,7 +865,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
 #pragma unroll 1
         for (int n = 0; n < min(2, halves); ++n)
 #pragma unroll
-          for (int tile = 0; tile < TILES; ++tile) scores(tile, stage, n);
+          for (int tile = 0; tile < TILES; ++tile)
+            if (tile < tiles) scores(tile, stage, n);
         if (one) {
           commit(&k_empty[stage]);
           if (halves <= 2) commit(&q_empty);
@@ -874,11 +875,12 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
 #pragma unroll 1
         for (int n = 0; n < halves; ++n) {
           const int h = n & 1, next = stage + 1 == STAGES ? 0 : stage + 1;
-          const uint32_t phase = ((h ? done1 : done0) + (n >> 1)) & 1, next_filled = filled ^ (next == 0);
+          const uint32_t next_filled = filled ^ (next == 0);
           if (h == 0) bar_wait(&v_full[stage], filled, a.wait_limit, stalled);
 #pragma unroll
           for (int tile = 0; tile < TILES; ++tile) {
-            bar_wait(&p_full[tile][h], phase, a.wait_limit, stalled);
+            if (tile >= tiles) continue;
+            bar_wait(&p_full[tile][h], ((h ? done1[tile] : done0[tile]) + (n >> 1)) & 1, a.wait_limit, stalled);
             fence_after();
             values(tile, stage, h, n > 0);
             if (n + 2 < halves) {
@@ -903,8 +905,12 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         }
         if (one) commit(&o_full);
         __syncwarp();
-        done0 += (halves + 1) >> 1;
-        done1 += halves >> 1;
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+          if (tile >= tiles) continue;
+          done0[tile] += (halves + 1) >> 1;
+          done1[tile] += halves >> 1;
+        }
         ++items;
       }
       // nothing is in flight when the tensor memory is given back, even after a wait that ran out

@@ -767,8 +767,13 @@ int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
 
 }  // namespace
 
+// Row tiles of 16 instead of 8.  The cache is read half as often, and a step costs about 1.3 times as much:
+// at 9 rows or more it pays (16 contexts of 8,192 tokens, 4 heads of 128, 16 rows: 37 against 50 us), but
+// not for head_dim 256, whose sums then do not fit the registers.
+static bool wide_tiles(int head_dim, int64_t max_rows) { return head_dim <= 128 && max_rows > 8; }
+
 size_t attend_rows_workspace(int head_dim, int64_t max_rows) {
-  const int64_t rows = max_rows <= 8 ? 8 : 16;
+  const int64_t rows = wide_tiles(head_dim, max_rows) ? 16 : 8;
   return align_up(Join::bytes(rows, head_dim));
 }
 
@@ -776,7 +781,10 @@ int launch_attend_rows(const AttendArgs& a, int dtype, int64_t max_rows, void* w
   auto by_rows = [&](auto d, auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int D = decltype(d)::value;
-    return max_rows <= 8 ? launch<D, 1, T>(a, workspace, s) : launch<D, 2, T>(a, workspace, s);
+    if constexpr (D <= 128) {
+      if (wide_tiles(D, max_rows)) return launch<D, 2, T>(a, workspace, s);
+    }
+    return launch<D, 1, T>(a, workspace, s);
   };
   auto by_dim = [&](auto* t) {
     return a.pool.head_dim == 64    ? by_rows(std::integral_constant<int, 64>{}, t)

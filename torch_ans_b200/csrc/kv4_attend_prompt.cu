@@ -73,9 +73,10 @@ struct Split {
 };
 constexpr int kLeastSteps = 4;  // that a block takes, if there are as many
 
-struct Info {  // of a step, from the unpacking warps to the softmax warps
-  int key_shift;     // keys are 2^key_shift times too large
-  int value_shift;   // values are 2^value_shift times too large
+struct alignas(16) Info {  // of a step, from the unpacking warps to the softmax warps
+  int key_shift;       // keys are 2^key_shift times too large
+  int value_shift;     // values are 2^value_shift times too large
+  uint8_t special[4];  // whether 32 tokens have one in the following
   uint32_t hidden[4], bad[4];  // tokens that no row sees, and those whose value is not finite
 };
 
@@ -381,6 +382,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     const int seen = row >= k.rows ? 0 : (a.causal ? min(k.seq.length, k.ahead + a.group.div(k.row0 + row)) : k.seq.length);
     const int halves = tile * kTile < k.rows ? k.halves : 0;  // a tile without rows has nothing to wait for
     int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
+    int least_left = __reduce_min_sync(0xffffffffu, left_all);  // that each of the warp's rows sees
     float m = -INFINITY, l = 0.0f;
     bool poisoned = false;
     int shift = 0;
@@ -403,12 +405,14 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       const int j = n >> 1, h = n & 1;
       const uint32_t at = s_at + h * kHalf, at_next = s_at + (h ^ 1) * kHalf;
       const Info& info = infos[(steps_done + j) & (kInfos - 1)];
-      const float f = scaled(factor, -info.key_shift);
-      const int now = info.value_shift;
-      const bool special = (info.hidden[2 * h] | info.hidden[2 * h + 1] | info.bad[2 * h] | info.bad[2 * h + 1]) != 0;
-      const int left = left_all;
+      const uint4 head = *reinterpret_cast<const uint4*>(&info);
+      const float f = scaled(factor, -(int)head.x);
+      const int now = (int)head.y;
+      const bool special = (head.z >> (16 * h) & 0xffff) != 0;
+      const int left = left_all;  // tokens of this half step that the row sees
+      const bool masked = least_left < kHalf || special;
       left_all -= kHalf;
-      const bool masked = __any_sync(0xffffffffu, left < kHalf) || special;
+      least_left -= kHalf;
       loaded();
       hold(x[0]);
       hold(x[1]);
@@ -789,6 +793,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       if (lane == 0 && part_of_row == 0) {
         info.key_shift = key_shift;  // the same in all
         info.value_shift = value_shift;
+        info.special[quarter] = (hidden | wrong) != 0;
         info.hidden[quarter] = hidden;
         info.bad[quarter] = wrong;
       }

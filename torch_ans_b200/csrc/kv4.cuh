@@ -16,6 +16,18 @@
 namespace tans {
 namespace kv4 {
 
+// Division by a number that the host knows: floor(n / d) for n < 2^31 is mulhi(2 n, m) >> l with
+// l = ceil(log2 d), m = ceil(2^(31 + l) / d) (Granlund and Montgomery).
+struct Divider {
+  uint32_t d, m, l;
+  static Divider of(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, (uint32_t)(((1ull << (31 + l)) + d - 1) / d), l};
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(__umulhi(2u * (uint32_t)n, m) >> l); }
+};
+
 struct Pool {
   const uint8_t* codes;
   const uint32_t* params;  // (scale, offset): low and high half

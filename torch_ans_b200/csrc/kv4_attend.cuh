@@ -8,18 +8,6 @@
 namespace tans {
 namespace kv4 {
 
-// Division by a number that the host knows: floor(n / d) for n < 2^31 is mulhi(2 n, m) >> l with
-// l = ceil(log2 d), m = ceil(2^(31 + l) / d) (Granlund and Montgomery).
-struct Divider {
-  uint32_t d, m, l;
-  static Divider of(uint32_t d) {
-    uint32_t l = 0;
-    while ((1ull << l) < d) ++l;
-    return {d, (uint32_t)(((1ull << (31 + l)) + d - 1) / d), l};
-  }
-  __device__ __forceinline__ int div(int n) const { return (int)(__umulhi(2u * (uint32_t)n, m) >> l); }
-};
-
 struct AttendArgs {
   Pool pool;
   const void* q;
@@ -99,7 +87,7 @@ __device__ __forceinline__ float pow2(int x) { return __int_as_float((x + 127) <
 // before), and the last of them to arrive joins them, in the order of the blocks whatever the order
 // of arrival, so results repeat.  Over kFan blocks join in two levels.  The counts of arrivals are
 // zero between launches: the last arrival takes its count back.
-constexpr int kFan = 32;
+constexpr int kFan = 16;
 constexpr int kMostBlocks = 4 * 160;  // blocks that a workspace has places for
 
 struct Join {

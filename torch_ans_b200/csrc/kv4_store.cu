@@ -25,6 +25,19 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// A slot's page.  Pools of 2^31 slots or more take the long division.
+struct PageOf {
+  Divider divider;
+  bool small;
+  int page_size;
+  static PageOf of(const Pool& p) {
+    return {Divider::of((uint32_t)p.page_size), p.num_pages < ((int64_t)1 << 31) / p.page_size, p.page_size};
+  }
+  __device__ __forceinline__ int64_t operator()(int64_t slot) const {
+    return small ? (int64_t)divider.div((int)slot) : slot / page_size;
+  }
+};
+
 struct AppendArgs {
   uint8_t* codes;
   uint32_t* params;
@@ -40,6 +53,8 @@ struct AppendArgs {
   int rotary;
   const int64_t* positions;
   uint32_t* status;
+  PageOf page_of;
+  Divider chunks;  // groups of rows of a token
 };
 
 // 4 consecutive elements of a row, as they are, and as floats
@@ -82,11 +97,11 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   const int lane = threadIdx.x % L, half = a.rotary / 2;
   const bool in_rotary = lane * 8 < a.rotary;
   const int d0 = !INTERLEAVED && in_rotary ? lane * 4 : lane * 8, d1 = !INTERLEAVED && in_rotary ? d0 + half : d0 + 4;
-  const int per_token = a.q_heads + 2 * a.pool.kv_heads, chunks = (per_token + ROWS - 1) / ROWS;
-  const int64_t group = blockIdx.x * (int64_t)(kThreads / L) + threadIdx.x / L;
-  const int64_t token = min(group / chunks, a.tokens - 1);  // groups past the end keep the warp's shuffles whole
-  const int r0 = (int)(group % chunks) * ROWS;
-  const int rows = group >= a.tokens * chunks ? 0 : min(ROWS, per_token - r0);
+  const int per_token = a.q_heads + 2 * a.pool.kv_heads;
+  const int group = blockIdx.x * (kThreads / L) + threadIdx.x / L, of = a.chunks.div(group);
+  const int64_t token = min((int64_t)of, a.tokens - 1);  // groups past the end keep the warp's shuffles whole
+  const int r0 = (group - of * (int)a.chunks.d) * ROWS;
+  const int rows = of >= a.tokens ? 0 : min(ROWS, per_token - r0);
 
   const T* q_at = static_cast<const T*>(a.q) + token * a.q_ts;
   const T* k_at = static_cast<const T*>(a.k) + token * a.k_ts - a.q_heads * a.k_hs;
@@ -125,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
     stores = false;
     if (a.status && lane == 0) atomicOr(a.status, TANS_DEV_BAD_INDEX);
   }
-  const int64_t page = stores ? slot / a.pool.page_size : 0;
+  const int64_t page = stores ? a.page_of(slot) : 0;
   const int in_page = stores ? (int)(slot - page * a.pool.page_size) : 0;
 
 #pragma unroll
@@ -196,11 +211,11 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
 }
 
 template <int D, typename T, int ROWS>
-int launch_rows(const AppendArgs& a, bool vec, bool interleaved, cudaStream_t s) {
-  const int64_t per_token = a.q_heads + 2 * (int64_t)a.pool.kv_heads;
-  const int64_t groups = a.tokens * ((per_token + ROWS - 1) / ROWS), per_block = kThreads / (D / 8);
-  const int64_t blocks = (groups + per_block - 1) / per_block;
-  if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
+int launch_rows(AppendArgs a, bool vec, bool interleaved, cudaStream_t s) {
+  const int64_t chunks = (a.q_heads + 2 * (int64_t)a.pool.kv_heads + ROWS - 1) / ROWS, per_block = kThreads / (D / 8);
+  const int64_t blocks = (a.tokens * chunks + per_block - 1) / per_block;
+  if (blocks > 0x7fffffff / per_block) return TANS_E_TOO_LARGE;  // groups are numbered in 31 bits
+  a.chunks = Divider::of((uint32_t)chunks);
   if (vec) {
     if (interleaved) append_kernel<D, T, true, true, ROWS><<<(unsigned)blocks, kThreads, 0, s>>>(a);
     else append_kernel<D, T, true, false, ROWS><<<(unsigned)blocks, kThreads, 0, s>>>(a);
@@ -224,22 +239,22 @@ int launch_append(const AppendArgs& a, bool vec, bool interleaved, cudaStream_t 
 
 // Values of the rows in `slots`: head_dim / 8 lanes for each row.
 template <int D, typename T>
-__global__ void __launch_bounds__(kThreads) gather_kernel(Pool pool, const int64_t* slots, int64_t tokens, T* k_out,
-                                                          T* v_out, uint32_t* status) {
+__global__ void __launch_bounds__(kThreads) gather_kernel(Pool pool, PageOf page_of, Divider per_token,
+                                                          const int64_t* slots, int64_t tokens, T* k_out, T* v_out,
+                                                          uint32_t* status) {
   constexpr int L = D / 8;
   const int lane = threadIdx.x % L;
-  const int per_token = 2 * pool.kv_heads;
-  const int64_t row = blockIdx.x * (int64_t)(kThreads / L) + threadIdx.x / L;
-  if (row >= tokens * per_token) return;
-  const int64_t token = row / per_token;
-  const int r = (int)(row - token * per_token);
+  const int row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  const int token = per_token.div(row);
+  if (token >= tokens) return;
+  const int r = row - token * (int)per_token.d;
   const int side = r >= pool.kv_heads, head = side ? r - pool.kv_heads : r;
   const int64_t slot = slots[token];
   uint4 w = make_uint4(0, 0, 0, 0);
   if (slot >= pool.num_pages * pool.page_size) {
     if (status && lane == 0) atomicOr(status, TANS_DEV_BAD_INDEX);
   } else if (slot >= 0) {
-    const int64_t page = slot / pool.page_size;
+    const int64_t page = page_of(slot);
     const int64_t at = pool.row(page, side, head) + (slot - page * pool.page_size);
     const uint32_t c = *reinterpret_cast<const uint32_t*>(pool.codes + at * (D / 2) + lane * 4);
     const uint32_t p = pool.params[at];
@@ -252,56 +267,48 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(Pool pool, const int64
     }
     w = make_uint4(u[0], u[1], u[2], u[3]);
   }
-  *reinterpret_cast<uint4*>((side ? v_out : k_out) + (token * pool.kv_heads + head) * D + lane * 8) = w;
+  *reinterpret_cast<uint4*>((side ? v_out : k_out) + ((int64_t)token * pool.kv_heads + head) * D + lane * 8) = w;
 }
 
-// Codes to symbols (and their tables' indexes): 4 codes a thread.
-__global__ void __launch_bounds__(kThreads) to_symbols_kernel(Pool pool, const int64_t* page_ids, int64_t n,
-                                                              int by_channel, int4* symbols, int4* indexes,
-                                                              uint32_t* status) {
-  const int64_t row_chunks = (int64_t)pool.page_size * pool.head_dim / 4;
-  const int64_t total = n * 2 * pool.kv_heads * row_chunks;
-  const int64_t e = blockIdx.x * (int64_t)kThreads + threadIdx.x;
-  if (e >= total) return;
-  const int64_t row = e / row_chunks, chunk = e - row * row_chunks;
-  const int sides = 2 * pool.kv_heads;
-  const int64_t i = row / sides;
-  const int side = (int)(row - i * sides);
-  const int64_t page = page_ids[i];
+// Codes to symbols (and their tables' indexes): 4 codes a thread, 16 bytes of each output at a time.  A row
+// of a page has a multiple of 1,024 codes (16 tokens of 64 channels at least), so a block's 256 threads are
+// in one row and only the block finds out where.  Bound by the 8 bytes written for each code.
+__global__ void __launch_bounds__(kThreads) to_symbols_kernel(Pool pool, const int64_t* page_ids, int by_channel,
+                                                              int4* symbols, int4* indexes, uint32_t* status) {
+  const unsigned row_blocks = (unsigned)(pool.page_size * (pool.head_dim / 4) / kThreads);
+  const unsigned row = blockIdx.x / row_blocks, sides = 2 * pool.kv_heads, i = row / sides, side = row - i * sides;
+  const unsigned chunk = (blockIdx.x - row * row_blocks) * kThreads + threadIdx.x;
+  const int64_t page = page_ids[i], e = blockIdx.x * (int64_t)kThreads + threadIdx.x;
   uint32_t c = 0;
   if (page < 0 || page >= pool.num_pages) {
     if (status && chunk == 0) atomicOr(status, TANS_DEV_BAD_INDEX);
   } else {
-    c = reinterpret_cast<const uint16_t*>(pool.codes)[(page * sides + side) * row_chunks + chunk];
+    c = reinterpret_cast<const uint16_t*>(pool.codes)[(page * sides + side) * (row_blocks * (int64_t)kThreads) + chunk];
   }
-  symbols[e] = make_int4(c & 15, (c >> 4) & 15, (c >> 8) & 15, c >> 12);
+  __stcs(symbols + e, make_int4(c & 15, (c >> 4) & 15, (c >> 8) & 15, c >> 12));
   if (indexes) {
-    const int t = by_channel ? side * pool.head_dim + (int)(chunk * 4 % pool.head_dim) : side;
-    indexes[e] = by_channel ? make_int4(t, t + 1, t + 2, t + 3) : make_int4(t, t, t, t);
+    const int t = by_channel ? side * pool.head_dim + (chunk * 4 & (pool.head_dim - 1)) : side;
+    __stcs(indexes + e, by_channel ? make_int4(t, t + 1, t + 2, t + 3) : make_int4(t, t, t, t));
   }
 }
 
-// Symbols to codes: 8 symbols a thread.
-__global__ void __launch_bounds__(kThreads) from_symbols_kernel(const int4* symbols, uint8_t* codes, Pool pool,
-                                                                const int64_t* page_ids, int64_t n, uint32_t* status) {
-  const int64_t row_chunks = (int64_t)pool.page_size * pool.head_dim / 8;
-  const int64_t total = n * 2 * pool.kv_heads * row_chunks;
-  const int64_t e = blockIdx.x * (int64_t)kThreads + threadIdx.x;
-  if (e >= total) return;
-  const int64_t row = e / row_chunks, chunk = e - row * row_chunks;
-  const int sides = 2 * pool.kv_heads;
-  const int64_t i = row / sides;
-  const int side = (int)(row - i * sides);
-  const int64_t page = page_ids[i];
+// Symbols to codes: 8 symbols a thread, a block in one row as above.  Bound by the 4 bytes read for each.
+constexpr int kBackThreads = 128;
+__global__ void __launch_bounds__(kBackThreads) from_symbols_kernel(const int4* symbols, uint8_t* codes, Pool pool,
+                                                                    const int64_t* page_ids, uint32_t* status) {
+  const unsigned row_blocks = (unsigned)(pool.page_size * (pool.head_dim / 8) / kBackThreads);
+  const unsigned row = blockIdx.x / row_blocks, sides = 2 * pool.kv_heads, i = row / sides, side = row - i * sides;
+  const unsigned chunk = (blockIdx.x - row * row_blocks) * kBackThreads + threadIdx.x;
+  const int64_t page = page_ids[i], e = blockIdx.x * (int64_t)kBackThreads + threadIdx.x;
+  const int4 a = __ldcs(symbols + 2 * e), b = __ldcs(symbols + 2 * e + 1);
   if (page < 0 || page >= pool.num_pages) {
     if (status && chunk == 0) atomicOr(status, TANS_DEV_BAD_INDEX);
     return;
   }
-  const int4 a = symbols[2 * e], b = symbols[2 * e + 1];
   if (((a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) & ~15) && status) atomicOr(status, TANS_DEV_BAD_VALUE);
   const uint32_t w = (uint32_t)(a.x & 15) | (a.y & 15) << 4 | (a.z & 15) << 8 | (a.w & 15) << 12 | (b.x & 15) << 16 |
                      (b.y & 15) << 20 | (b.z & 15) << 24 | (uint32_t)(b.w & 15) << 28;
-  reinterpret_cast<uint32_t*>(codes)[(page * sides + side) * row_chunks + chunk] = w;
+  reinterpret_cast<uint32_t*>(codes)[(page * sides + side) * (row_blocks * (int64_t)kBackThreads) + chunk] = w;
 }
 
 bool aligned16(const void* p, int64_t ts, int64_t hs) {
@@ -332,12 +339,13 @@ extern "C" int tans_kv4_append(uint8_t* codes, void* params, int64_t num_pages, 
   if (((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(rotation)) & 15) != 0)
     return TANS_E_INVALID_ARGUMENT;  // they are read and written 16 bytes at a time
   cudaStream_t s = reinterpret_cast<cudaStream_t>(cuda_stream);
-  const AppendArgs a{codes,
+  AppendArgs a{codes,
                      static_cast<uint32_t*>(params),
                      Pool{codes, static_cast<const uint32_t*>(params), num_pages, kv_heads, page_size, head_dim},
                      q, k, v,
                      q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
-                     q_out, q_heads, slots, tokens, rotation, rotation_rows, rotary_dim, positions, dev_status};
+                     q_out, q_heads, slots, tokens, rotation, rotation_rows, rotary_dim, positions, dev_status, {}, {}};
+  a.page_of = PageOf::of(a.pool);
   const bool vec = aligned16(k, k_token_stride, k_head_stride) && aligned16(v, v_token_stride, v_head_stride) &&
                    (!q || aligned16(q, q_token_stride, q_head_stride));
   const bool il = interleaved != 0;
@@ -365,11 +373,11 @@ extern "C" int tans_kv4_gather(const uint8_t* codes, const void* params, int64_t
   const Pool pool{codes, static_cast<const uint32_t*>(params), num_pages, kv_heads, page_size, head_dim};
   const int64_t per_block = kThreads / (head_dim / 8);
   const int64_t blocks = (tokens * 2 * kv_heads + per_block - 1) / per_block;
-  if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
+  if (blocks > 0x7fffffff / per_block) return TANS_E_TOO_LARGE;  // rows are numbered in 31 bits
   auto go = [&](auto d, auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     gather_kernel<decltype(d)::value, T><<<(unsigned)blocks, kThreads, 0, s>>>(
-        pool, slots, tokens, static_cast<T*>(k_out), static_cast<T*>(v_out), dev_status);
+        pool, PageOf::of(pool), Divider::of(2u * kv_heads), slots, tokens, static_cast<T*>(k_out), static_cast<T*>(v_out), dev_status);
   };
   auto by_dim = [&](auto* t) {
     if (head_dim == 64) go(std::integral_constant<int, 64>{}, t);
@@ -396,7 +404,7 @@ extern "C" int tans_kv4_to_symbols(const uint8_t* codes, int64_t num_pages, int 
   const int64_t blocks = (threads + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
   to_symbols_kernel<<<(unsigned)blocks, kThreads, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
-      pool, page_ids, n, by_channel, reinterpret_cast<int4*>(symbols), reinterpret_cast<int4*>(indexes), dev_status);
+      pool, page_ids, by_channel, reinterpret_cast<int4*>(symbols), reinterpret_cast<int4*>(indexes), dev_status);
   tans::note_launch();
   return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
 }
@@ -410,10 +418,10 @@ extern "C" int tans_kv4_from_symbols(const int32_t* symbols, uint8_t* codes, int
   if (!page_ids || !symbols || (reinterpret_cast<uintptr_t>(symbols) & 15) != 0) return TANS_E_INVALID_ARGUMENT;
   const Pool pool{codes, nullptr, num_pages, kv_heads, page_size, head_dim};
   const int64_t threads = n * 2 * kv_heads * ((int64_t)page_size * head_dim / 8);
-  const int64_t blocks = (threads + kThreads - 1) / kThreads;
+  const int64_t blocks = threads / kBackThreads;
   if (blocks > 0x7fffffff) return TANS_E_TOO_LARGE;
-  from_symbols_kernel<<<(unsigned)blocks, kThreads, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
-      reinterpret_cast<const int4*>(symbols), codes, pool, page_ids, n, dev_status);
+  from_symbols_kernel<<<(unsigned)blocks, kBackThreads, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
+      reinterpret_cast<const int4*>(symbols), codes, pool, page_ids, dev_status);
   tans::note_launch();
   return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
 }

@@ -23,6 +23,13 @@
 //
 // The running maximum follows the scores only when one passes it by over 8 (a weight under 2^9 still
 // fits float16), so most steps compare and go on.
+//
+// Measured: 48 contexts of 256 to 16,384 tokens (222k together, 32 query and 8 key/value heads of 128, 242
+// MB) 72 us, 3.4 TB/s: about 560 instructions a step, the ALU pipe half busy, and each item's start and end;
+// 3 contexts of about 127k tokens (16 and 2 heads, 103 MB) 43 us, of which the steps are about 20 (5 to 6
+// TB/s), the start 6 and the joins of 97 blocks an item 10; one context of 777 tokens 12 us, all latency.
+// Blocks of 4 warps, four on an SM, so that one's start and end run beside the others' steps: with 8 warps,
+// two on an SM, the ragged batch took 83 us and the long contexts 44.
 #include "kv4_attend.cuh"
 #include "launch.cuh"
 #include "rans_host.h"

@@ -38,6 +38,7 @@
 #include "rans_host.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace tans {
@@ -385,230 +386,230 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     int number = 0;
 #pragma unroll 1
     for (;; ++number) {
-    const Work& k = take(number);  // read again where it is used: registers are dear here
-    if (!k.some || *stalled) break;
-    const int seen = row >= k.rows ? 0 : (a.causal ? min(k.seq.length, k.ahead + a.group.div(k.row0 + row)) : k.seq.length);
-    const int halves = tile * kTile < k.rows ? k.halves : 0;  // a tile without rows has nothing to wait for
-    int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
-    int least_left = __reduce_min_sync(0xffffffffu, left_all);  // that each of the warp's rows sees
-    float m = -INFINITY, l = 0.0f;
-    bool poisoned = false;
-    int shift = 0;
-    uint32_t x[2][32];
-    auto scores_of = [&](int n) {  // half step n's are there
-      bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, a.wait_limit, stalled);
-      __syncwarp();
-      fence_after();
-    };
-    // scores are `factor` and the step's factor times the product, in powers of two
-    float factor = 0.0f;
-    if (halves > 0) {
-      scores_of(0);
-      factor = factors[items & 1][row];
-      load32(x[0], s_at);
-      load32(x[1], s_at + 32);
-    }
-#pragma unroll 1
-    for (int n = 0; n < halves; ++n) {
-      const int j = n >> 1, h = n & 1;
-      const uint32_t at = s_at + h * kHalf, at_next = s_at + (h ^ 1) * kHalf;
-      const Info& info = infos[(steps_done + j) & (kInfos - 1)];
-      const uint4 head = *reinterpret_cast<const uint4*>(&info);
-      const float f = scaled(factor, -(int)head.x);
-      const int now = (int)head.y;
-      const bool special = (head.z >> (16 * h) & 0xffff) != 0;
-      const int left = left_all;  // tokens of this half step that the row sees
-      const bool masked = least_left < kHalf || special;
-      left_all -= kHalf;
-      least_left -= kHalf;
-      loaded();
-      hold(x[0]);
-      hold(x[1]);
-      uint32_t visible[2];
-      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (masked) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int some = left - w * 32;
-          visible[w] = some >= 32 ? 0xffffffffu : (some <= 0 ? 0u : (1u << some) - 1);
-          if (special) {
-            visible[w] &= ~info.hidden[2 * h + w];
-            poisoned |= (visible[w] & info.bad[2 * h + w]) != 0;
-          }
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            tops[k & 3] = visible[w] >> k & 1 ? fmaxf(tops[k & 3], __uint_as_float(x[w][k])) : tops[k & 3];
-        }
-      } else {
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-          for (int k = 0; k < 32; k += 2)
-            tops[k / 2 & 3] = fmaxf(fmaxf(__uint_as_float(x[w][k]), __uint_as_float(x[w][k + 1])), tops[k / 2 & 3]);
-      }
-      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      top = top == -INFINITY ? top : top * f;
-      const bool moves = top > m + kSlack;
-      const float next = moves ? top : m;
-      if (__any_sync(0xffffffffu, moves || now != shift)) {
-        const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
-        l *= keep;
-        if (n > 0) {  // O is not yet written before the first half step, and at rest after the last one's
-          bar_wait(&o_done[tile], (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
-          __syncwarp();
-          fence_after();
-          const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
-#pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t y[16];
-            load16(y, o_at + c);
-            loaded();
-            hold(y);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * both);
-            store16(y, o_at + c);
-          }
-        }
-      }
-      m = next;
-      shift = now;
-      const float base = m == -INFINITY ? 0.0f : m;
-      float2 sum = make_float2(0.0f, 0.0f);
-      // Weights of 32 tokens, put over the scores; two at a time where the hardware has it.  The next
-      // scores take the registers of those that are done, so that they come while others are worked on.
-      auto weigh = [&](auto masked_) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t p[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float2 e = fma2(make_float2(__uint_as_float(x[w][2 * k]), __uint_as_float(x[w][2 * k + 1])),
-                            make_float2(f, f), make_float2(-base, -base));
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            if constexpr (decltype(masked_)::value) {
-              e.x = visible[w] >> (2 * k) & 1 ? e.x : 0.0f;
-              e.y = visible[w] >> (2 * k + 1) & 1 ? e.y : 0.0f;
-            }
-            sum = add2(sum, e);
-            p[k] = Half2<__half>::pack(e.x, e.y);
-          }
-          store16(p, at + w * 16);
-          if (n + 1 < halves) {
-            if (w == 0) scores_of(n + 1);
-            load32(x[w], at_next + w * 32);
-          }
-        }
+      const Work& k = take(number);  // read again where it is used: registers are dear here
+      if (!k.some || *stalled) break;
+      const int seen = row >= k.rows ? 0 : (a.causal ? min(k.seq.length, k.ahead + a.group.div(k.row0 + row)) : k.seq.length);
+      const int halves = tile * kTile < k.rows ? k.halves : 0;  // a tile without rows has nothing to wait for
+      int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
+      int least_left = __reduce_min_sync(0xffffffffu, left_all);  // that each of the warp's rows sees
+      float m = -INFINITY, l = 0.0f;
+      bool poisoned = false;
+      int shift = 0;
+      uint32_t x[2][32];
+      auto scores_of = [&](int n) {  // half step n's are there
+        bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, a.wait_limit, stalled);
+        __syncwarp();
+        fence_after();
       };
-      if (masked) weigh(std::true_type{});
-      else weigh(std::false_type{});
-      l += sum.x + sum.y;
-      stored();
-      fence_before();
-      bar_arrive(&p_full[tile][h]);
-    }
-    // ---- the rows' results
-    const bool live = row < k.rows;
-    const int i = a.group.div(k.row0 + (live ? row : 0)),
-              h = k.head * a.group.d + (k.row0 + (live ? row : 0) - i * a.group.d);
-    const int64_t o = (int64_t)(k.seq.start + i) * a.q_heads + h;
-    const int tile_head = k.tile_head, part = k.part, parts = SPLIT ? k.parts : 1;
-    if (halves > 0) {
-      bar_wait(&o_full, items & 1, a.wait_limit, stalled);
-      __syncwarp();
-      fence_after();
-    }
-    if (poisoned) l = __int_as_float(0x7fffffff);
-    // 8 channels of the row, unpacking's order undone
-    auto write8 = [&](int d, const float (&v)[8], float k) {
-      uint4 w;
-      w.x = Half2<T>::pack(v[0] * k, v[1] * k);
-      w.y = Half2<T>::pack(v[2] * k, v[3] * k);
-      w.z = Half2<T>::pack(v[4] * k, v[5] * k);
-      w.w = Half2<T>::pack(v[6] * k, v[7] * k);
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + d) = w;
-    };
-    const int64_t mine = (int64_t)tile_head * split.splits + part;
-    const float inv_l = l == 0.0f ? 0.0f : (SPLIT && parts > 1 ? 1.0f : 1.0f / l);
-    const float back0 = pow2((-shift) >> 1) * inv_l, back1 = pow2(-shift - ((-shift) >> 1));
-#pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
-      uint32_t x[32];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = 0;
+      // scores are `factor` and the step's factor times the product, in powers of two
+      float factor = 0.0f;
       if (halves > 0) {
-        load32(x, o_at + c);
-        loaded();
-        hold(x);
+        scores_of(0);
+        factor = factors[items & 1][row];
+        load32(x[0], s_at);
+        load32(x[1], s_at + 32);
       }
-      if (live) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = __uint_as_float(x[8 * g + 2 * e]) * back0;
-            v[e + 4] = __uint_as_float(x[8 * g + 2 * e + 1]) * back0;
-          }
-          if (!SPLIT || parts == 1) {
-            write8(c + g * 8, v, back1);
-          } else {
-            float4* to = split.parts + (mine * (D / 4) + c / 4 + g * 2) * RT + row;
-            to[0] = make_float4(v[0] * back1, v[1] * back1, v[2] * back1, v[3] * back1);
-            to[RT] = make_float4(v[4] * back1, v[5] * back1, v[6] * back1, v[7] * back1);
-          }
-        }
-      }
-    }
-    if (SPLIT && parts > 1) {
-      split.stats[mine * RT + row] = make_float2(m, l);
-      __threadfence();
-      asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
-      if (threadIdx.x == 0) sh_last = arrive(split.arrivals + tile_head, parts);
-      asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
-      if (sh_last) {
-        __threadfence();
-        const int64_t first = (int64_t)tile_head * split.splits;
-        m = -INFINITY;
-        for (int p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&split.stats[(first + p) * RT + row]).x);
-        const float base = m == -INFINITY ? 0.0f : m;
-        l = 0.0f;
-        for (int p = 0; p < parts; ++p) {
-          const float2 st = __ldcg(&split.stats[(first + p) * RT + row]);
-          l += ex2(st.x - base) * st.y;
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-        for (int d = 0; live && d < D; d += 16) {
-          float v[2][8] = {};
-          for (int p = 0; p < parts; ++p) {
-            const float w = ex2(__ldcg(&split.stats[(first + p) * RT + row]).x - base);
-            const float4* from = split.parts + ((first + p) * (D / 4) + d / 4) * RT + row;
+      for (int n = 0; n < halves; ++n) {
+        const int j = n >> 1, h = n & 1;
+        const uint32_t at = s_at + h * kHalf, at_next = s_at + (h ^ 1) * kHalf;
+        const Info& info = infos[(steps_done + j) & (kInfos - 1)];
+        const uint4 head = *reinterpret_cast<const uint4*>(&info);
+        const float f = scaled(factor, -(int)head.x);
+        const int now = (int)head.y;
+        const bool special = (head.z >> (16 * h) & 0xffff) != 0;
+        const int left = left_all;  // tokens of this half step that the row sees
+        const bool masked = least_left < kHalf || special;
+        left_all -= kHalf;
+        least_left -= kHalf;
+        loaded();
+        hold(x[0]);
+        hold(x[1]);
+        uint32_t visible[2];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (masked) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int some = left - w * 32;
+            visible[w] = some >= 32 ? 0xffffffffu : (some <= 0 ? 0u : (1u << some) - 1);
+            if (special) {
+              visible[w] &= ~info.hidden[2 * h + w];
+              poisoned |= (visible[w] & info.bad[2 * h + w]) != 0;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              tops[k & 3] = visible[w] >> k & 1 ? fmaxf(tops[k & 3], __uint_as_float(x[w][k])) : tops[k & 3];
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int k = 0; k < 32; k += 2)
+              tops[k / 2 & 3] = fmaxf(fmaxf(__uint_as_float(x[w][k]), __uint_as_float(x[w][k + 1])), tops[k / 2 & 3]);
+        }
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        top = top == -INFINITY ? top : top * f;
+        const bool moves = top > m + kSlack;
+        const float next = moves ? top : m;
+        if (__any_sync(0xffffffffu, moves || now != shift)) {
+          const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
+          l *= keep;
+          if (n > 0) {  // O is not yet written before the first half step, and at rest after the last one's
+            bar_wait(&o_done[tile], (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
+            __syncwarp();
+            fence_after();
+            const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t y[16];
+              load16(y, o_at + c);
+              loaded();
+              hold(y);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * both);
+              store16(y, o_at + c);
+            }
+          }
+        }
+        m = next;
+        shift = now;
+        const float base = m == -INFINITY ? 0.0f : m;
+        float2 sum = make_float2(0.0f, 0.0f);
+        // Weights of 32 tokens, put over the scores; two at a time where the hardware has it.  The next
+        // scores take the registers of those that are done, so that they come while others are worked on.
+        auto weigh = [&](auto masked_) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float2 e = fma2(make_float2(__uint_as_float(x[w][2 * k]), __uint_as_float(x[w][2 * k + 1])),
+                              make_float2(f, f), make_float2(-base, -base));
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              if constexpr (decltype(masked_)::value) {
+                e.x = visible[w] >> (2 * k) & 1 ? e.x : 0.0f;
+                e.y = visible[w] >> (2 * k + 1) & 1 ? e.y : 0.0f;
+              }
+              sum = add2(sum, e);
+              p[k] = Half2<__half>::pack(e.x, e.y);
+            }
+            store16(p, at + w * 16);
+            if (n + 1 < halves) {
+              if (w == 0) scores_of(n + 1);
+              load32(x[w], at_next + w * 32);
+            }
+          }
+        };
+        if (masked) weigh(std::true_type{});
+        else weigh(std::false_type{});
+        l += sum.x + sum.y;
+        stored();
+        fence_before();
+        bar_arrive(&p_full[tile][h]);
+      }
+      // ---- the rows' results
+      const bool live = row < k.rows;
+      const int i = a.group.div(k.row0 + (live ? row : 0)),
+                h = k.head * a.group.d + (k.row0 + (live ? row : 0) - i * a.group.d);
+      const int64_t o = (int64_t)(k.seq.start + i) * a.q_heads + h;
+      const int tile_head = k.tile_head, part = k.part, parts = SPLIT ? k.parts : 1;
+      if (halves > 0) {
+        bar_wait(&o_full, items & 1, a.wait_limit, stalled);
+        __syncwarp();
+        fence_after();
+      }
+      if (poisoned) l = __int_as_float(0x7fffffff);
+      // 8 channels of the row, unpacking's order undone
+      auto write8 = [&](int d, const float (&v)[8], float k) {
+        uint4 w;
+        w.x = Half2<T>::pack(v[0] * k, v[1] * k);
+        w.y = Half2<T>::pack(v[2] * k, v[3] * k);
+        w.z = Half2<T>::pack(v[4] * k, v[5] * k);
+        w.w = Half2<T>::pack(v[6] * k, v[7] * k);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + o * D + d) = w;
+      };
+      const int64_t mine = (int64_t)tile_head * split.splits + part;
+      const float inv_l = l == 0.0f ? 0.0f : (SPLIT && parts > 1 ? 1.0f : 1.0f / l);
+      const float back0 = pow2((-shift) >> 1) * inv_l, back1 = pow2(-shift - ((-shift) >> 1));
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = 0;
+        if (halves > 0) {
+          load32(x, o_at + c);
+          loaded();
+          hold(x);
+        }
+        if (live) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float v[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float4 x = __ldcg(from + e * RT);
-              v[e >> 1][(e & 1) * 4] += w * x.x;
-              v[e >> 1][(e & 1) * 4 + 1] += w * x.y;
-              v[e >> 1][(e & 1) * 4 + 2] += w * x.z;
-              v[e >> 1][(e & 1) * 4 + 3] += w * x.w;
+              v[e] = __uint_as_float(x[8 * g + 2 * e]) * back0;
+              v[e + 4] = __uint_as_float(x[8 * g + 2 * e + 1]) * back0;
+            }
+            if (!SPLIT || parts == 1) {
+              write8(c + g * 8, v, back1);
+            } else {
+              float4* to = split.parts + (mine * (D / 4) + c / 4 + g * 2) * RT + row;
+              to[0] = make_float4(v[0] * back1, v[1] * back1, v[2] * back1, v[3] * back1);
+              to[RT] = make_float4(v[4] * back1, v[5] * back1, v[6] * back1, v[7] * back1);
             }
           }
-          write8(d, v[0], inv);
-          write8(d + 8, v[1], inv);
         }
       }
-    }
-    if (live && a.lse && (parts == 1 || sh_last))
-      a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-    done0 += (halves + 1) >> 1;
-    done1 += halves >> 1;
-    if (k.halves > 0) {
-      steps_done += k.steps;
-      ++items;
-    }
-    fence_before();
-    if (SPLIT) break;
-    give_back(number);
+      if (SPLIT && parts > 1) {
+        split.stats[mine * RT + row] = make_float2(m, l);
+        __threadfence();
+        asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
+        if (threadIdx.x == 0) sh_last = arrive(split.arrivals + tile_head, parts);
+        asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
+        if (sh_last) {
+          __threadfence();
+          const int64_t first = (int64_t)tile_head * split.splits;
+          m = -INFINITY;
+          for (int p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(&split.stats[(first + p) * RT + row]).x);
+          const float base = m == -INFINITY ? 0.0f : m;
+          l = 0.0f;
+          for (int p = 0; p < parts; ++p) {
+            const float2 st = __ldcg(&split.stats[(first + p) * RT + row]);
+            l += ex2(st.x - base) * st.y;
+          }
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+          for (int d = 0; live && d < D; d += 16) {
+            float v[2][8] = {};
+            for (int p = 0; p < parts; ++p) {
+              const float w = ex2(__ldcg(&split.stats[(first + p) * RT + row]).x - base);
+              const float4* from = split.parts + ((first + p) * (D / 4) + d / 4) * RT + row;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float4 x = __ldcg(from + e * RT);
+                v[e >> 1][(e & 1) * 4] += w * x.x;
+                v[e >> 1][(e & 1) * 4 + 1] += w * x.y;
+                v[e >> 1][(e & 1) * 4 + 2] += w * x.z;
+                v[e >> 1][(e & 1) * 4 + 3] += w * x.w;
+              }
+            }
+            write8(d, v[0], inv);
+            write8(d + 8, v[1], inv);
+          }
+        }
+      }
+      if (live && a.lse && (parts == 1 || sh_last))
+        a.lse[o] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+      done0 += (halves + 1) >> 1;
+      done1 += halves >> 1;
+      if (k.halves > 0) {
+        steps_done += k.steps;
+        ++items;
+      }
+      fence_before();
+      if (SPLIT) break;
+      give_back(number);
     }
   } else if (warp < kIssue) {
     if constexpr (P::UNPACK_REGS > P::LAUNCH_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::UNPACK_REGS));
@@ -1006,15 +1007,22 @@ int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
   split.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + Join::kArrivalBytes);
   split.parts = reinterpret_cast<float4*>(split.stats + tiles * split.splits * RT);
   const int work = (int)tiles * split.splits;
-  auto go = [&](auto* kernel, int blocks) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess)
-      return TANS_E_CUDA;
+  auto go = [&](auto split_, int blocks) {
+    auto* kernel = &attend_prompt_kernel<D, T, decltype(split_)::value>;
+    static std::atomic<bool> ready[64];  // of this kernel, by device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TANS_E_CUDA;
+    if (!ready[dev].load(std::memory_order_relaxed)) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess)
+        return TANS_E_CUDA;
+      ready[dev].store(true, std::memory_order_relaxed);
+    }
     kernel<<<blocks, P::WARPS * 32, P::BYTES, s>>>(a, split, work);
     note_launch();
     return cudaGetLastError() == cudaSuccess ? TANS_OK : TANS_E_CUDA;
   };
-  return split.splits > 1 ? go(&attend_prompt_kernel<D, T, true>, work)
-                          : go(&attend_prompt_kernel<D, T, false>, std::min(work, sm_count()));
+  return split.splits > 1 ? go(std::true_type{}, work)
+                          : go(std::false_type{}, std::min(work, sm_count()));
 }
 
 }  // namespace

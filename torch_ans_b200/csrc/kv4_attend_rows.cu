@@ -35,6 +35,7 @@
 #include "rans_host.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace tans {
@@ -745,20 +746,23 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
   zero_rest();
 }
 
+// Blocks that an SM holds at once, found once for each device (a kernel's attributes are the device's).
 template <int D, int NT, typename T>
 int blocks_per_sm() {
-  static int known = 0;
-  if (known == 0) {
-    int n = 0;
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     constexpr int bytes = Shared<D, NT>::BYTES;
     if (cudaFuncSetAttribute(attend_rows_kernel<D, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
             cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_rows_kernel<D, NT, T>, kWarps * 32, bytes) !=
             cudaSuccess)
       return 0;
-    known = n;
+    known[dev].store(n, std::memory_order_relaxed);
   }
-  return known;
+  return n;
 }
 
 template <int D, int NT, typename T>

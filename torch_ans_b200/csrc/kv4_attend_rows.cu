@@ -12,24 +12,32 @@
 // byte permutes pair the tokens of a channel first).
 //
 // With a row's (s, o): q.k = s (q.c) + o sum(q), so scales and offsets never touch the codes: the
-// score takes two products and one sum, and the value's scale goes into the weight,
-//   sum p v = 2^E (sum w c - 7.5 sum w) + sum p (o + 7.5 s),  w = float16(p s 2^-E),
-// with E a running power of two over the largest s.  The 7.5 centres the codes (sum w is one more
-// row of ones in the second product), so a weight's rounding to float16 (2^-11) weighs on the code's
-// distance from the middle, not on the code: about half the error.  The sums of the softmax, the
-// offsets and all accumulators are float.  A query row is brought under 2^14 by a power of two and
-// rounded to float16, which loses nothing that bfloat16 or float16 holds above 2^-24 of the row's
-// largest.
+// score x (a power of two's exponent) takes two products and one sum, and the value's scale goes into
+// the weight,
+//   sum 2^x v = 2^Y (sum w c - 7.5 sum w) + sum 2^x (o + 7.5 s),  w = float16(2^(x - Y) s).
+// The 7.5 centres the codes (sum w is one more row of ones in the second product), so a weight's
+// rounding to float16 (2^-11) weighs on the code's distance from the middle, not on the code: about half
+// the error.  The sums of the softmax, the offsets and all accumulators are float.  A query row is
+// brought under 2^14 by a power of two and rounded to float16, which loses nothing that bfloat16 or
+// float16 holds above 2^-24 of the row's largest.
 //
-// The running maximum follows the scores only when one passes it by over 8 (a weight under 2^9 still
-// fits float16), so most steps compare and go on.
+// Y is each query row's own.  It follows the largest product of a weight and a value's size, max(s, |o +
+// 7.5 s|), among the tokens that the row sees, and leaves it at most 2^6 when it moves: what float16 cuts
+// off is 2^-31 of the largest product, whatever the sizes of the values and of those that do not count
+// (hidden tokens, or ones of no weight).  Weights 2^(x - R) are taken against R = Y, or the running
+// maximum m of x where that is less: then they are at most 2^8 and w = 2^(x - R) (s 2^(R - Y)); Y is kept
+// above m - 96, so where values are tiny the weights stay in float's range.  m and Y move only when a score
+// passes m by over 8, or when a lane's largest score and largest size (of four tokens) together pass Y by
+// 14 (w is then under 2^15): most steps compare and go on.
 //
 // Measured: 48 contexts of 256 to 16,384 tokens (222k together, 32 query and 8 key/value heads of 128, 242
-// MB) 72 us, 3.4 TB/s: about 560 instructions a step, the ALU pipe half busy, and each item's start and end;
-// 3 contexts of about 127k tokens (16 and 2 heads, 103 MB) 43 us, of which the steps are about 20 (5 to 6
+// MB) 74 us, 3.3 TB/s: about 570 instructions a step, the ALU pipe half busy, and each item's start and end;
+// 3 contexts of about 127k tokens (16 and 2 heads, 103 MB) 44 us, of which the steps are about 21 (5 to 6
 // TB/s), the start 6 and the joins of 97 blocks an item 10; one context of 777 tokens 12 us, all latency.
+// With one factor for all rows of a warp instead of a Y for each row these took 72 and 43 us, and a value 2^20
+// times larger than the others, of no weight or hidden, took a fifth of the answers away.
 // Blocks of 4 warps, four on an SM, so that one's start and end run beside the others' steps: with 8 warps,
-// two on an SM, the ragged batch took 83 us and the long contexts 44.
+// two on an SM, the ragged batch took 83 us and the long contexts 44 when these took 72 and 43.
 #include "kv4_attend.cuh"
 #include "launch.cuh"
 #include "rans_host.h"
@@ -45,7 +53,11 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStep = 32;   // tokens a warp takes at a time
 constexpr int kStages = 3;  // steps in flight for each warp, the one in use among them
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 8.0f;     // by which a score may pass the running maximum
+constexpr float kRoom = 14.0f;     // by which a product's size may pass Y: its weight is under 2^15
+constexpr float kDeepest = 96.0f;  // Y is at most so far under m: weights and their sums stay in float's range
+constexpr float kHighest = 122.0f; // and at most so far above it: a size of 2^128 at a weight of 2^8 leaves 2^14
+constexpr float kNone = -1e30f;    // Y before the first token
 constexpr int kItemSteps = 8;  // what an item's start and end cost a block, in steps
 constexpr int kMostParts = kMostBlocks / kFan > kFan ? kMostBlocks / kFan : kFan;  // that are joined at a time
 
@@ -86,6 +98,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
+}
+
+// the exponent of |v| as a float: 2^exponent <= |v| < 2^(exponent + 1); -127 for 0
+__device__ __forceinline__ float exponent(float v) {
+  return __uint_as_float(0x4b000000u | __float_as_uint(v) >> 23) - (8388608.0f + 127.0f);
 }
 
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -451,13 +468,15 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
     // every live row sees the tokens under `full`
     const int full = a.causal ? seq.length - seq.count + a.group.div(row0) + 1 : seq.length;
 
-    float m[NT][2], l[NT][2], off[NT][2], acc[NT][D / 16][4], ones[NT][4];
-    int E = 27;  // exponent field of the weights' common factor
+    // of columns 2t and 2t + 1: m and Y as above, the sums of the weights and of their offsets in 2^R, the
+    // products in 2^Y
+    float m[NT][2], Y[NT][2], l[NT][2], off[NT][2], acc[NT][D / 16][4], ones[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         m[n][c] = -INFINITY;
+        Y[n][c] = kNone;
         l[n][c] = off[n][c] = 0.0f;
       }
 #pragma unroll
@@ -516,7 +535,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
         bool in[4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-        uint32_t big = 0;
+        float big = 0.0f;  // the largest size
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // j: group j / 2, row g or g + 8
           const uint32_t kw = kp[8 * j], vw = vp[8 * j];
@@ -525,8 +544,8 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           ov[j] = fmaf(7.5f, sv[j], offset_of(vw));
           const int token = step * kStep + tok + 8 * j;
           in[j] = !masked || (token < seq.length && (bits >> (j >> 1) & 1));
-          const uint32_t field = (vw << 16) & 0x7f800000u;
-          big = max(big, in[j] && field != 0x7f800000u ? field : 0u);
+          const float size = fmaxf(fabsf(sv[j]), fabsf(ov[j]));
+          big = fmaxf(big, in[j] ? size : 0.0f);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -537,45 +556,55 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
               top[n][c] = fmaxf(top[n][c], x);
             }
         }
-        // follow the maximum and the largest scale
-        bool move = (int)(big >> 23) > E;
+        const float reach = exponent(big) - kRoom;
+        bool move = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) move |= top[n][0] > m[n][0] + kSlack || top[n][1] > m[n][1] + kSlack;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) move |= top[n][c] > m[n][c] + kSlack || top[n][c] + reach > Y[n][c];
         if (__any_sync(0xffffffffu, move)) {
-          const int field = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
-          const int now = min(252, max(E, field));
-          const float fall = E > now - 126 ? pow2(E - now) : 0.0f;
-          E = now;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float x = top[n][c];
+              float x = top[n][c], y = -INFINITY;
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-              const float top_now = x > m[n][c] + kSlack ? x : m[n][c];
-              const float keep = m[n][c] == -INFINITY ? 1.0f : ex2(m[n][c] - top_now);
-              m[n][c] = top_now;
-              l[n][c] *= keep;
-              off[n][c] *= keep;
-              const float both = keep * fall;
-              ones[n][c] *= both;
+              for (int j = 0; j < 4; ++j)  // a token that the row does not see is at -inf, whatever its size
+                y = fmaxf(y, s[j >> 1][n][(j & 1) * 2 + c] + exponent(fmaxf(fabsf(sv[j]), fabsf(ov[j]))));
 #pragma unroll
-              for (int i = 0; i < D / 16; ++i) {
-                acc[n][i][c] *= both;
-                acc[n][i][c + 2] *= both;
+              for (int o = 4; o < 32; o <<= 1) {
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
               }
+              const float m_now = x > m[n][c] + kSlack ? x : m[n][c];
+              float Y_now = y > Y[n][c] + kRoom ? y - (kRoom - kSlack) : Y[n][c];
+              if (m_now != -INFINITY) Y_now = fminf(fmaxf(Y_now, m_now - kDeepest), m_now + kHighest);
+              const float keep = ex2(fminf(m[n][c], Y[n][c]) - fminf(m_now, Y_now)), both = ex2(Y[n][c] - Y_now);
+              if (m[n][c] != -INFINITY) {  // nothing is kept before the first token
+                l[n][c] *= keep;
+                off[n][c] *= keep;
+                ones[n][c] *= both;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                  acc[n][i][c] *= both;
+                  acc[n][i][c + 2] *= both;
+                }
+              }
+              m[n][c] = m_now;
+              Y[n][c] = Y_now;
             }
         }
-        const float inv = pow2(126 - E);  // weights are under 2^8
-        float base[NT][2];
+        float base[NT][2], less[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) base[n][c] = m[n][c] == -INFINITY ? 0.0f : m[n][c];
+          for (int c = 0; c < 2; ++c) {
+            const float unit = fminf(m[n][c], Y[n][c]);
+            base[n][c] = m[n][c] == -INFINITY ? 0.0f : unit;
+            less[n][c] = ex2(unit - Y[n][c]);  // 1 unless values are larger than 2^6
+          }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float sc = sv[j] * inv;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float w[2];
@@ -585,7 +614,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
               const float e = ex2(x - base[n][c]);
               const bool hidden = masked && x == -INFINITY;
               l[n][c] += e;
-              w[c] = hidden ? 0.0f : e * sc;
+              w[c] = hidden ? 0.0f : e * (sv[j] * less[n][c]);
               off[n][c] = hidden ? off[n][c] : fmaf(e, ov[j], off[n][c]);
             }
             wf[j >> 1][n][j & 1] = transpose8(Half2<__half>::pack(w[0], w[1]));
@@ -639,7 +668,6 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
     // ---- join the warps: sums in shared memory (the rings' memory)
     __syncthreads();
     float* so = reinterpret_cast<float*>(smem);  // [warp][row][D + 4]
-    const float back = pow2(min(127, E - 126));  // the weights' common factor (E <= 252)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -650,6 +678,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           off[n][c] += __shfl_xor_sync(0xffffffffu, off[n][c], o);
         }
         const int row = n * 8 + 2 * t + c;
+        const float unit = fminf(m[n][c], Y[n][c]), back = m[n][c] == -INFINITY ? 0.0f : ex2(Y[n][c] - unit);
         float* dst = so + (warp * R + row) * (D + 4) + g * (D / 8);
         const float mid = 7.5f * ones[n][c];
 #pragma unroll
@@ -657,7 +686,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           dst[2 * i] = fmaf(fmaf(acc[n][i][c], 16777216.0f, -mid), back, off[n][c]);
           dst[2 * i + 1] = fmaf(fmaf(acc[n][i][c + 2], 1048576.0f, -mid), back, off[n][c]);
         }
-        if (g == 0) sh_stat[warp * R + row] = make_float2(m[n][c], l[n][c]);
+        if (g == 0) sh_stat[warp * R + row] = make_float2(unit, l[n][c]);
       }
     __syncthreads();
 

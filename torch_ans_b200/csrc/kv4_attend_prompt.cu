@@ -20,19 +20,27 @@
 // Where there are fewer such row tiles than SMs, several blocks share the tokens of each, leave their
 // sums in the workspace, and the last of them joins them in the order of the tokens.
 //
-// All operands are float16 brought into range by powers of two: a query row by its own, 128 keys by
-// theirs, values by one that only grows over the tokens (O is rescaled when it does, as when a
-// maximum moves).  So nothing that bfloat16 or float16 holds overflows, and the rounding is 2^-11 of
-// each value, key and weight; sums are float.  A maximum moves only when it is passed by over 8
-// (weights under 2^9), which rescales O rarely.
+// All operands are float16 brought into range by powers of two: a query row by its own, the keys and the
+// values of a step by one each.  A row of keys or values that is over 2^5 smaller than the step's largest
+// would come too near float16's least number: a step with such a row is "wide", and there each row has its
+// own factor, which the softmax warps put into its scores and weights (two 2^x a score instead of one).  So
+// the rounding is 2^-11 of each key, each row of values and each weight, whatever the sizes of other
+// tokens, of those that are hidden from a query too; sums are float.
 //
-// Measured: 4 packed prompts of 1,143 to 3,500 tokens (32 query and 8 key/value heads of 128, 166 GFLOP) 226
-// us, 733 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 161 us, 423 TFLOP/s.  A
-// half step takes about 2,000 cycles, in which the products are busy for 1,280 (head_dim 128), 2^x for 1,024
-// and the instructions' issue for 900 a scheduler: leaving out any one of them, or the unpacking, in a copy
-// took 2 to 4 % off (17 % for 2^x at head_dim 64), so it is the latency of all of them together.  Steps of 128
-// tokens whose softmax waits for its own products took 261 us where half steps took 243; without the blocks'
-// going on by themselves 243 against 233.
+// A query row's weights are 2^(x - m - d) for the score x, its running maximum m and a power of two d of
+// its own over the step's: it follows the largest product of a weight and a value's size that the row sees, and
+// leaves it at 2^6 when it moves, which it does (and O is rescaled) when a product passes it by 2^14.  The
+// sum of the softmax is 2^(x - m), which m follows when a score passes it by over 8.
+//
+// Measured: 4 packed prompts of 1,143 to 3,500 tokens (32 query and 8 key/value heads of 128, 166 GFLOP) 234
+// us, 709 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 165 us, 412 TFLOP/s.  With one power
+// of two for all values so far and none for single rows these took 228 and 161 us on the same GPU, and a value 2^16
+// times larger in a step, seen or not, left other queries' answers a fifth wrong.  A half step takes about 2,000
+// cycles, in which the products are busy for 1,280 (head_dim 128), 2^x for 1,024 and the instructions' issue
+// for 900 a scheduler: leaving out any one of them, or the unpacking, in a copy took 2 to 4 % off (17 % for 2^x
+// at head_dim 64), so it is the latency of all of them together.  Steps of 128 tokens whose softmax waits for
+// its own products took 261 us where half steps took 243; without the blocks' going on by themselves 243
+// against 233.
 #include "kv4_attend.cuh"
 #include "launch.cuh"
 #include "rans_host.h"
@@ -47,7 +55,8 @@ namespace {
 
 constexpr int kTile = 128;  // rows of a tile, tokens of a step
 constexpr int kHalf = 64;   // tokens of a half step
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 8.0f;  // by which a score may pass the running maximum
+constexpr float kRoom = 14.0f;  // largest exponent of a weight
 constexpr int kInfos = 4;   // steps whose factors are kept: the unpacking warps run at most 2 ahead
 constexpr int kTries = 1 << 20;  // of the last wait
 
@@ -83,9 +92,9 @@ struct Split {
 constexpr int kLeastSteps = 4;  // that a block takes, if there are as many
 
 struct alignas(16) Info {  // of a step, from the unpacking warps to the softmax warps
-  int key_shift;       // keys are 2^key_shift times too large
-  int value_shift;     // values are 2^value_shift times too large
-  uint8_t special[4];  // whether 32 tokens have one in the following
+  float key0, key1;    // the product of these undoes the keys' power of two (in a wide step each key has its own)
+  float value_shift;   // values are 2^value_shift times too large
+  uint8_t special[4];  // 1: 32 tokens have one in the following; 2: the step is wide
   uint32_t hidden[4], bad[4];  // tokens that no row sees, and those whose value is not finite
 };
 
@@ -204,6 +213,11 @@ __device__ __forceinline__ void store16(const uint32_t (&r)[16], uint32_t at) {
       TANS_W4(r, 4), TANS_W4(r, 8), TANS_W4(r, 12), "r"(at)
       : "memory");
 }
+__device__ __forceinline__ void store8(const uint32_t (&r)[8], uint32_t at) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::TANS_W4(r, 0), TANS_W4(r, 4),
+               "r"(at)
+               : "memory");
+}
 __device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 #define TANS_RW4(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3])
 // no use of these registers comes before this place (the wait that the loads into them need)
@@ -236,13 +250,103 @@ __device__ __forceinline__ float scaled(float v, int n) { return v * pow2(n >> 1
 __device__ __forceinline__ bool finite_row(uint32_t p) {
   return fabsf(scale_of(p)) < INFINITY && fabsf(offset_of(p)) < INFINITY;  // neither for NaN
 }
-// How far a row reaches, as an exponent field: 2^(kReach - field) brings its values under 2^14 and its
-// scale times 2^24 under 2^15.  0 for a row that is not finite.
-constexpr int kReach = 140;
-__device__ __forceinline__ uint32_t reach(uint32_t p) {
+// The size of a row's values as an exponent field, 0 for a row that is zero or not finite.  2^(kReach - size)
+// brings the values under 2^-7 and, since 7.5 scales are no more than the largest value, the scale times
+// 2^24 under 2^15.
+constexpr int kReach = 119, kLeast = 6;  // kLeast: smaller ones are taken for this
+constexpr int kSpread = 5;  // rows so much smaller are at 2^-13 still, where float16 rounds to 2^-25
+__device__ __forceinline__ int size_of(uint32_t p) {
   const float s = scale_of(p), o = offset_of(p), top = fmaxf(fabsf(o), fabsf(fmaf(15.0f, s, o)));
-  const uint32_t field = max(min(__float_as_uint(top) >> 23, 254u), (__float_as_uint(fabsf(s)) >> 23) + 23);
-  return finite_row(p) ? field : 0u;
+  return finite_row(p) ? min((int)(__float_as_uint(top) >> 23), 254) : 0;
+}
+
+// A row of queries: its running maximum m, its sum l of 2^(x - m), and d: weights are 2^(x - m - d) over the
+// step's power of two.
+struct Softmax {
+  float m = -INFINITY, l = 0.0f, d = 0.0f;
+
+  // m and d after the row's largest score and, as largest(m), its largest product against the new m.  O at o_at
+  // follows d; `done` says when it is at rest (null: nothing is there yet).
+  template <int D, typename Largest>
+  __device__ __forceinline__ void follow(float top, Largest largest, uint32_t o_at, uint64_t* done, uint32_t parity,
+                                         int tries, volatile int* stalled) {
+    const bool moves = top > m + kSlack;
+    const float next = moves ? top : m;
+    const float d_here = moves ? d - (next - m) : d;  // the same weights against the new maximum
+    const float size = largest(next);
+    l *= m == -INFINITY ? 1.0f : ex2(m - next);
+    m = next;
+    // whole, so that the weight of a token that outdoes all others is exact
+    d = size > d_here + kRoom ? ceilf(size) - (kRoom - kSlack) : ceilf(d_here);
+    if (done && __any_sync(0xffffffffu, d != d_here)) {
+      bar_wait(done, parity, tries, stalled);
+      __syncwarp();
+      fence_after();
+      const float keep = d != d_here ? ex2(d_here - d) : 1.0f;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t y[16];
+        load16(y, o_at + c);
+        loaded();
+        hold(y);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * keep);
+        store16(y, o_at + c);
+      }
+    }
+  }
+};
+
+// Half of a wide step: each key has its own power of two and each value its own (`own`: value's << 16 | key's).
+// Such steps are few, so the scores at `at` are read again for each use, 16 at a time.  A function of its own: within
+// the loop over the half steps this code made the others slower (the chunk below 168 us, 165 with the call).
+template <int D>
+__device__ __noinline__ Softmax wide_half(Softmax s, float factor, const uint32_t* own, uint32_t visible0, uint32_t visible1,
+                                          uint32_t at, uint32_t o_at, uint64_t* done, uint32_t parity, int tries,
+                                          volatile int* stalled) {
+  auto read = [&](int c, float (&v)[16], float (&shift)[16]) {
+    uint32_t y[16];
+    load16(y, at + c);
+    loaded();
+    hold(y);
+    const uint32_t in = (c & 32 ? visible1 : visible0) >> (c & 16);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int both = own[c + k], undo = -(int)(int16_t)both;
+      shift[k] = (float)(both >> 16);
+      v[k] = in >> k & 1 ? __uint_as_float(y[k]) * pow2(undo >> 1) * factor * pow2(undo - (undo >> 1)) : -INFINITY;
+    }
+  };
+  float v[16], shift[16], top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kHalf; c += 16) {
+    read(c, v, shift);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) top = fmaxf(top, v[k]);
+  }
+  s.follow<D>(top, [&](float next) {
+    float size = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < kHalf; c += 16) {
+      read(c, v, shift);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) size = fmaxf(size, v[k] - next - shift[k]);
+    }
+    return size;
+  }, o_at, done, parity, tries, stalled);
+  const float m = s.m == -INFINITY ? 0.0f : s.m;
+#pragma unroll 1
+  for (int c = 0; c < kHalf; c += 16) {  // the weights of 16 tokens lie where scores of no later ones are
+    read(c, v, shift);
+    uint32_t p[8];
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) {
+      s.l += ex2(v[k] - m) + ex2(v[k + 1] - m);
+      p[k / 2] = Half2<__half>::pack(ex2(v[k] - m - (s.d + shift[k])), ex2(v[k + 1] - m - (s.d + shift[k + 1])));
+    }
+    store8(p, at + c / 2);
+  }
+  return s;
 }
 
 // A block's piece of work: the rows of a row tile (or two) and head, and the steps of tokens it takes.
@@ -322,7 +426,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   __shared__ Info infos[kInfos];
   __shared__ Work queue[kQueue];
   __shared__ float factors[2][RT];  // of two pieces' rows
-  __shared__ uint32_t top_k[2][4], top_v[2][4];
+  __shared__ __align__(16) uint32_t range_k[2][4], range_v[2][4];  // of 32 tokens: largest size << 16 | smallest
+  __shared__ __align__(16) uint32_t own_shifts[kInfos][kTile];     // of a wide step's tokens: value's << 16 | key's
   volatile int* stalled = &stalled_;
   uint8_t* smem = raw + ((1024 - (smem_of(raw) & 1023)) & 1023);
   // the same in all of a warp's threads, which the compiler sees by the shuffle
@@ -392,9 +497,9 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       const int halves = tile * kTile < k.rows ? k.halves : 0;  // a tile without rows has nothing to wait for
       int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
       int least_left = __reduce_min_sync(0xffffffffu, left_all);  // that each of the warp's rows sees
-      float m = -INFINITY, l = 0.0f;
+      Softmax softmax;
+      float &m = softmax.m, &l = softmax.l, &d = softmax.d;
       bool poisoned = false;
-      int shift = 0;
       uint32_t x[2][32];
       auto scores_of = [&](int n) {  // half step n's are there
         bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, a.wait_limit, stalled);
@@ -415,9 +520,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         const uint32_t at = s_at + h * kHalf, at_next = s_at + (h ^ 1) * kHalf;
         const Info& info = infos[(steps_done + j) & (kInfos - 1)];
         const uint4 head = *reinterpret_cast<const uint4*>(&info);
-        const float f = scaled(factor, -(int)head.x);
-        const int now = (int)head.y;
-        const bool special = (head.z >> (16 * h) & 0xffff) != 0;
+        const float f = factor * __uint_as_float(head.x) * __uint_as_float(head.y), now = __uint_as_float(head.z);
+        const bool special = (head.w >> (16 * h) & 0xffff) != 0, wide = (head.w & 2) != 0;
         const int left = left_all;  // tokens of this half step that the row sees
         const bool masked = least_left < kHalf || special;
         left_all -= kHalf;
@@ -426,7 +530,6 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         hold(x[0]);
         hold(x[1]);
         uint32_t visible[2];
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if (masked) {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
@@ -436,10 +539,29 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
               visible[w] &= ~info.hidden[2 * h + w];
               poisoned |= (visible[w] & info.bad[2 * h + w]) != 0;
             }
+          }
+          if (wide) {
+            const uint32_t* const own = own_shifts[(steps_done + j) & (kInfos - 1)] + h * kHalf;
+            softmax = wide_half<D>(softmax, factor, own, visible[0], visible[1], at, o_at, n > 0 ? &o_done[tile] : nullptr,
+                                   (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
+            stored();
+            fence_before();
+            bar_arrive(&p_full[tile][h]);
+            if (n + 1 < halves) {
+              scores_of(n + 1);
+              load32(x[0], at_next);
+              load32(x[1], at_next + 32);
+            }
+            continue;
+          }
+        }
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (masked) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               tops[k & 3] = visible[w] >> k & 1 ? fmaxf(tops[k & 3], __uint_as_float(x[w][k])) : tops[k & 3];
-          }
         } else {
 #pragma unroll
           for (int w = 0; w < 2; ++w)
@@ -449,31 +571,13 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         }
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         top = top == -INFINITY ? top : top * f;
-        const bool moves = top > m + kSlack;
-        const float next = moves ? top : m;
-        if (__any_sync(0xffffffffu, moves || now != shift)) {
-          const float keep = m == -INFINITY ? 1.0f : ex2(m - next);
-          l *= keep;
-          if (n > 0) {  // O is not yet written before the first half step, and at rest after the last one's
-            bar_wait(&o_done[tile], (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
-            __syncwarp();
-            fence_after();
-            const float both = keep * (shift - now < 127 ? pow2(now - shift) : 0.0f);
-#pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t y[16];
-              load16(y, o_at + c);
-              loaded();
-              hold(y);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * both);
-              store16(y, o_at + c);
-            }
-          }
-        }
-        m = next;
-        shift = now;
-        const float base = m == -INFINITY ? 0.0f : m;
+        if (__any_sync(0xffffffffu, top > m + fminf(kSlack, d + now + kRoom)))
+          softmax.follow<D>(top, [&](float next) { return top - next - now; }, o_at, n > 0 ? &o_done[tile] : nullptr,
+                            (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
+        // Weights 2^(x - m - over); `over` stops at 60, where they are under 2^-52 (zeros in float16: values that
+        // are tiny beside the others'), so that the softmax's sum, which comes from them, stays in float's range.
+        const float over = fminf(d + now, 60.0f);
+        const float base = m + over;  // a row that has seen nothing yet: all of its weights are masked
         float2 sum = make_float2(0.0f, 0.0f);
         // Weights of 32 tokens, put over the scores; two at a time where the hardware has it.  The next
         // scores take the registers of those that are done, so that they come while others are worked on.
@@ -503,7 +607,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         };
         if (masked) weigh(std::true_type{});
         else weigh(std::false_type{});
-        l += sum.x + sum.y;
+        l = fmaf(sum.x + sum.y, ex2(over), l);
         stored();
         fence_before();
         bar_arrive(&p_full[tile][h]);
@@ -531,7 +635,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       };
       const int64_t mine = (int64_t)tile_head * split.splits + part;
       const float inv_l = l == 0.0f ? 0.0f : (SPLIT && parts > 1 ? 1.0f : 1.0f / l);
-      const float back0 = pow2((-shift) >> 1) * inv_l, back1 = pow2(-shift - ((-shift) >> 1));
+      const float back0 = ex2(floorf(0.5f * d)) * inv_l, back1 = ex2(d - floorf(0.5f * d));
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t x[32];
@@ -767,13 +871,11 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     slot_now = slot;
     bool there = valid;
     look_up();
-    uint32_t value_top = 27;  // exponent field of the largest value so far
     int stage = 0;
     uint32_t filled = 0;
 #pragma unroll 1
     for (uint32_t j = 0; there; ++j) {
       if (begun) {
-        value_top = 27;
         if (items > 0) bar_wait(&q_empty, (items - 1) & 1, a.wait_limit, stalled);
         __syncwarp();
         copy_queries(queue[slot_now % kQueue]);
@@ -781,31 +883,42 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         turn_queries(items);
         ++items;
       }
-      // the largest key and value, over the step
-      const uint32_t wk = __reduce_max_sync(0xffffffffu, reach(kp)), wv = __reduce_max_sync(0xffffffffu, reach(vp));
+      // the largest key and value, over the step, and the smallest of those that are not zero
+      const int key_size = size_of(kp), value_size = size_of(vp);
+      const int most_k = __reduce_max_sync(0xffffffffu, key_size), most_v = __reduce_max_sync(0xffffffffu, value_size),
+                least_k = __reduce_min_sync(0xffffffffu, key_size ? key_size : 255),
+                least_v = __reduce_min_sync(0xffffffffu, value_size ? value_size : 255);
       if (lane == 0 && part_of_row == 0) {
-        top_k[j & 1][quarter] = wk;
-        top_v[j & 1][quarter] = wv;
+        range_k[j & 1][quarter] = most_k << 16 | least_k;
+        range_v[j & 1][quarter] = most_v << 16 | least_v;
       }
       const bool bad = state == 1 && !finite_row(vp);
       const uint32_t hidden = __ballot_sync(0xffffffffu, state == 2), wrong = __ballot_sync(0xffffffffu, bad);
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      uint32_t key_top = 27;
+      int key_top = kLeast, value_top = kLeast, key_low = 255, value_low = 255;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        key_top = max(key_top, top_k[j & 1][w]);
-        value_top = max(value_top, top_v[j & 1][w]);
+        key_top = max(key_top, (int)(range_k[j & 1][w] >> 16));
+        key_low = min(key_low, (int)(range_k[j & 1][w] & 0xffff));
+        value_top = max(value_top, (int)(range_v[j & 1][w] >> 16));
+        value_low = min(value_low, (int)(range_v[j & 1][w] & 0xffff));
       }
-      const int key_shift = kReach - (int)key_top, value_shift = kReach - (int)value_top;
+      const bool wide = key_low + kSpread < key_top || value_low + kSpread < value_top;
+      const int key_shift = kReach - (wide ? max(key_size, kLeast) : key_top),
+                value_shift = kReach - (wide ? max(value_size, kLeast) : value_top);
       bar_wait(&k_empty[stage], filled ^ 1, a.wait_limit, stalled);
       Info& info = infos[j & (kInfos - 1)];
       if (lane == 0 && part_of_row == 0) {
-        info.key_shift = key_shift;  // the same in all
-        info.value_shift = value_shift;
-        info.special[quarter] = (hidden | wrong) != 0;
+        const int undo = key_top - kReach;  // the same in all
+        info.key0 = pow2(undo >> 1);
+        info.key1 = pow2(undo - (undo >> 1));
+        info.value_shift = (float)(kReach - value_top);
+        info.special[quarter] = ((hidden | wrong) != 0) | (wide ? 2 : 0);
         info.hidden[quarter] = hidden;
         info.bad[quarter] = wrong;
       }
+      if (wide && part_of_row == 0)
+        own_shifts[j & (kInfos - 1)][t] = (uint32_t)value_shift << 16 | (uint32_t)(key_shift & 0xffff);
       spread(kc, kp, key_shift, smem + P::K + stage * P::ROWS);
       fence_smem();
       bar_arrive(&k_full[stage]);

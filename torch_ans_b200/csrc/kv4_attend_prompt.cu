@@ -30,7 +30,9 @@
 // A query row's weights are 2^(x - m - d) for the score x, its running maximum m and a power of two d of
 // its own over the step's: it follows the largest product of a weight and a value's size that the row sees, and
 // leaves it at 2^6 when it moves, which it does (and O is rescaled) when a product passes it by 2^14.  The
-// sum of the softmax is 2^(x - m), which m follows when a score passes it by over 8.
+// sum of the softmax is 2^(x - m), which m follows when a score passes it by over 8.  Scores are fused into
+// x - (m + d); where |m| passes 2^10 they are rounded first and m is taken from them, token by token as in a
+// wide step: the product's rounding would otherwise be a factor of the weight, past float's range from 2^30.
 //
 // Measured: 4 packed prompts of 1,143 to 3,500 tokens (32 query and 8 key/value heads of 128, 166 GFLOP) 234
 // us, 709 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 165 us, 412 TFLOP/s.  With one power
@@ -57,6 +59,7 @@ constexpr int kTile = 128;  // rows of a tile, tokens of a step
 constexpr int kHalf = 64;   // tokens of a half step
 constexpr float kSlack = 8.0f;  // by which a score may pass the running maximum
 constexpr float kRoom = 14.0f;  // largest exponent of a weight
+constexpr float kFar = 1024.0f; // a maximum from here on is taken from the rounded scores: m + d would be rounded, too
 constexpr int kInfos = 4;   // steps whose factors are kept: the unpacking warps run at most 2 ahead
 constexpr int kTries = 1 << 20;  // of the last wait
 
@@ -297,11 +300,12 @@ struct Softmax {
   }
 };
 
-// Half of a wide step: each key has its own power of two and each value its own (`own`: value's << 16 | key's).
-// Such steps are few, so the scores at `at` are read again for each use, 16 at a time.  A function of its own: within
+// Half of a step token by token: each key has its own power of two and each value its own (`own`: value's << 16 |
+// key's), or, without `own`, scores are `factor` times the products and the values' power is the step's, `now`.  Such
+// steps are few, so the scores at `at` are read again for each use, 16 at a time.  A function of its own: within
 // the loop over the half steps this code made the others slower (the chunk below 168 us, 165 with the call).
 template <int D>
-__device__ __noinline__ Softmax wide_half(Softmax s, float factor, const uint32_t* own, uint32_t visible0, uint32_t visible1,
+__device__ __noinline__ Softmax by_token(Softmax s, float factor, float now, const uint32_t* own, uint32_t visible0, uint32_t visible1,
                                           uint32_t at, uint32_t o_at, uint64_t* done, uint32_t parity, int tries,
                                           volatile int* stalled) {
   auto read = [&](int c, float (&v)[16], float (&shift)[16]) {
@@ -312,8 +316,8 @@ __device__ __noinline__ Softmax wide_half(Softmax s, float factor, const uint32_
     const uint32_t in = (c & 32 ? visible1 : visible0) >> (c & 16);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-      const int both = own[c + k], undo = -(int)(int16_t)both;
-      shift[k] = (float)(both >> 16);
+      const int both = own ? own[c + k] : 0, undo = -(int)(int16_t)both;
+      shift[k] = own ? (float)(both >> 16) : now;
       v[k] = in >> k & 1 ? __uint_as_float(y[k]) * pow2(undo >> 1) * factor * pow2(undo - (undo >> 1)) : -INFINITY;
     }
   };
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       int least_left = __reduce_min_sync(0xffffffffu, left_all);  // that each of the warp's rows sees
       Softmax softmax;
       float &m = softmax.m, &l = softmax.l, &d = softmax.d;
-      bool poisoned = false;
+      bool poisoned = false, far = false;  // far: some |m| of the warp is over kFar
       uint32_t x[2][32];
       auto scores_of = [&](int n) {  // half step n's are there
         bar_wait(&s_full[tile][n & 1], ((n & 1 ? done1 : done0) + (n >> 1)) & 1, a.wait_limit, stalled);
@@ -523,13 +527,26 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         const float f = factor * __uint_as_float(head.x) * __uint_as_float(head.y), now = __uint_as_float(head.z);
         const bool special = (head.w >> (16 * h) & 0xffff) != 0, wide = (head.w & 2) != 0;
         const int left = left_all;  // tokens of this half step that the row sees
-        const bool masked = least_left < kHalf || special;
+        const bool masked = least_left < kHalf || special || far;
         left_all -= kHalf;
         least_left -= kHalf;
         loaded();
         hold(x[0]);
         hold(x[1]);
-        uint32_t visible[2];
+        auto token_by_token = [&](uint32_t visible0, uint32_t visible1) {
+          const uint32_t* const own = wide ? own_shifts[(steps_done + j) & (kInfos - 1)] + h * kHalf : nullptr;
+          softmax = by_token<D>(softmax, wide ? factor : f, now, own, visible0, visible1, at, o_at,
+                                n > 0 ? &o_done[tile] : nullptr, (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
+          stored();
+          fence_before();
+          bar_arrive(&p_full[tile][h]);
+          if (n + 1 < halves) {
+            scores_of(n + 1);
+            load32(x[0], at_next);
+            load32(x[1], at_next + 32);
+          }
+        };
+        uint32_t visible[2] = {0xffffffffu, 0xffffffffu};
         if (masked) {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
@@ -540,18 +557,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
               poisoned |= (visible[w] & info.bad[2 * h + w]) != 0;
             }
           }
-          if (wide) {
-            const uint32_t* const own = own_shifts[(steps_done + j) & (kInfos - 1)] + h * kHalf;
-            softmax = wide_half<D>(softmax, factor, own, visible[0], visible[1], at, o_at, n > 0 ? &o_done[tile] : nullptr,
-                                   (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
-            stored();
-            fence_before();
-            bar_arrive(&p_full[tile][h]);
-            if (n + 1 < halves) {
-              scores_of(n + 1);
-              load32(x[0], at_next);
-              load32(x[1], at_next + 32);
-            }
+          if (wide || far) {
+            token_by_token(visible[0], visible[1]);
             continue;
           }
         }
@@ -571,9 +578,15 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         }
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         top = top == -INFINITY ? top : top * f;
-        if (__any_sync(0xffffffffu, top > m + fminf(kSlack, d + now + kRoom)))
+        if (__any_sync(0xffffffffu, top > m + fminf(kSlack, d + now + kRoom))) {
           softmax.follow<D>(top, [&](float next) { return top - next - now; }, o_at, n > 0 ? &o_done[tile] : nullptr,
                             (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
+          far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > kFar);
+          if (far) {
+            token_by_token(visible[0], visible[1]);
+            continue;
+          }
+        }
         // Weights 2^(x - m - over); `over` stops at 60, where they are under 2^-52 (zeros in float16: values that
         // are tiny beside the others'), so that the softmax's sum, which comes from them, stays in float's range.
         const float over = fminf(d + now, 60.0f);
@@ -844,7 +857,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
                                fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y)))));
       }
-      const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));
+      const int e = 13 - max(-113, min(127, (int)(__float_as_uint(top) >> 23) - 127));
       const float up = a.scale_log2 < 0.0f ? -pow2(e) : pow2(e);
       factors[item & 1][row] = fabsf(a.scale_log2) * pow2(-e);
 #pragma unroll 2

@@ -28,13 +28,14 @@
 // maximum m of x where that is less: then they are at most 2^8 and w = 2^(x - R) (s 2^(R - Y)); Y is kept
 // above m - 96, so where values are tiny the weights stay in float's range.  m and Y move only when a score
 // passes m by over 8, or when a lane's largest score and largest size (of four tokens) together pass Y by
-// 14 (w is then under 2^15): most steps compare and go on.
+// 14 (w is then under 2^15): most steps compare and go on.  Where |m| passes 2^10 the column's scores get an
+// origin there, taken off before anything else is added to them, so that Y and R stay as exact as they are.
 //
 // Measured: 48 contexts of 256 to 16,384 tokens (222k together, 32 query and 8 key/value heads of 128, 242
 // MB) 74 us, 3.3 TB/s: about 570 instructions a step, the ALU pipe half busy, and each item's start and end;
-// 3 contexts of about 127k tokens (16 and 2 heads, 103 MB) 44 us, of which the steps are about 21 (5 to 6
+// 3 contexts of about 127k tokens (16 and 2 heads, 103 MB) 43 us, of which the steps are about 20 (5 to 6
 // TB/s), the start 6 and the joins of 97 blocks an item 10; one context of 777 tokens 12 us, all latency.
-// With one factor for all rows of a warp instead of a Y for each row these took 72 and 43 us, and a value 2^20
+// With one factor for all rows of a warp instead of a Y for each row the ragged batch took 72 us, and a value 2^20
 // times larger than the others, of no weight or hidden, took a fifth of the answers away.
 // Blocks of 4 warps, four on an SM, so that one's start and end run beside the others' steps: with 8 warps,
 // two on an SM, the ragged batch took 83 us and the long contexts 44 when these took 72 and 43.
@@ -58,6 +59,7 @@ constexpr float kRoom = 14.0f;     // by which a product's size may pass Y: its 
 constexpr float kDeepest = 96.0f;  // Y is at most so far under m: weights and their sums stay in float's range
 constexpr float kHighest = 122.0f; // and at most so far above it: a size of 2^128 at a weight of 2^8 leaves 2^14
 constexpr float kNone = -1e30f;    // Y before the first token
+constexpr float kFar = 1024.0f;    // |m| from which on scores have an origin
 constexpr int kItemSteps = 8;  // what an item's start and end cost a block, in steps
 constexpr int kMostParts = kMostBlocks / kFan > kFan ? kMostBlocks / kFan : kFan;  // that are joined at a time
 
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
   __shared__ int sh_found[2];
   __shared__ Sequence sh_sequence;
   __shared__ int sh_last;
-  __shared__ float2 sh_stat[kWarps * R], sh_total[R];
+  __shared__ float2 sh_stat[kWarps * R], sh_total[R], sh_origin[kWarps][R / 2];
   __shared__ float sh_weight[2 * kMostParts][R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int heads = a.pool.kv_heads, page_size = a.pool.page_size;
@@ -421,6 +423,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
     uint32_t qf[NT][KW][4];
     float fac[NT][2], shift[NT][2];  // of columns 2t and 2t + 1: score = (acc * s) * fac + o * shift
     int seen[NT][2];                 // tokens that the columns' queries see
+    uint32_t large[NT];              // bit 8 t + 4 c: a score lacks 2^24
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[D / 4];
@@ -434,18 +437,21 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           x[c * 8 + 2 * e + 1] = f.y;
         }
       }
-      float top = 0.0f, sum = 0.0f;
+      float top = 0.0f, sum = 0.0f;  // 2^-10 of the sum: it may pass float's range
 #pragma unroll
       for (int c = 0; c < D / 4; ++c) {
         top = fmaxf(top, fabsf(x[c]));
-        sum += x[c];
+        sum = fmaf(x[c], 0.0009765625f, sum);
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
-      const int e = 13 - max(-87, min(116, (int)(__float_as_uint(top) >> 23) - 127));  // the row times 2^e is under 2^14
+      const int e = 13 - max(-113, min(127, (int)(__float_as_uint(top) >> 23) - 127));  // the row times 2^e is under 2^14
+      // the score's factors, 2^(24 - e), may pass float's range for large queries: those lack 2^24 until the end
+      const bool over = e < -100;
+      large[n] = __ballot_sync(0xffffffffu, over);
       const float up = pow2(e), up16 = pow2(e - 4);
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
         qf[n][w][2] = Half2<__half>::pack(x[8 * w + 2] * up, x[8 * w + 6] * up);
         qf[n][w][3] = Half2<__half>::pack(x[8 * w + 3] * up16, x[8 * w + 7] * up16);
       }
-      const float f = a.scale_log2 * pow2(24 - e), sh = a.scale_log2 * sum;
+      const float f = a.scale_log2 * pow2(over ? -e : 24 - e), sh = a.scale_log2 * (over ? 0x1p-14f : 1024.0f) * sum;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         fac[n][c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
@@ -468,6 +474,15 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
     // every live row sees the tokens under `full`
     const int full = a.causal ? seq.length - seq.count + a.group.div(row0) + 1 : seq.length;
 
+    // Some scores lack 2^24, or have an origin: all steps go the longer way.
+    bool apart = false;
+    float2* const origin = sh_origin[warp];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      apart |= large[n] != 0;
+      if (g == 0) origin[n * 4 + t] = make_float2(0.0f, 0.0f);
+    }
+    __syncwarp();
     // of columns 2t and 2t + 1: m and Y as above, the sums of the weights and of their offsets in 2^R, the
     // products in 2^Y
     float m[NT][2], Y[NT][2], l[NT][2], off[NT][2], acc[NT][D / 16][4], ones[NT][4];
@@ -552,6 +567,10 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
             for (int c = 0; c < 2; ++c) {
               float& x = s[j >> 1][n][(j & 1) * 2 + c];
               x = fmaf(x * sk, fac[n][c], ok * shift[n][c]);
+              if (masked && apart) {
+                if (large[n] >> (8 * t + 4 * c) & 1) x *= 16777216.0f;
+                x -= c ? origin[n * 4 + t].y : origin[n * 4 + t].x;
+              }
               if (masked && !(in[j] && token < seen[n][c])) x = -INFINITY;
               top[n][c] = fmaxf(top[n][c], x);
             }
@@ -569,14 +588,27 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
             for (int c = 0; c < 2; ++c) {
               float x = top[n][c], y = -INFINITY;
 #pragma unroll
+              for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+              float m_now = x > m[n][c] + kSlack ? x : m[n][c];
+              const bool far = m_now != -INFINITY && fabsf(m_now) > kFar;
+              if (__any_sync(0xffffffffu, far)) {
+                float* const at = reinterpret_cast<float*>(origin) + (n * 4 + t) * 2 + c;
+                const float old = *at, now = old + (far ? m_now : 0.0f), from = now - old;
+                apart = true;
+                m_now -= from;
+                Y[n][c] = m[n][c] == -INFINITY ? kNone : Y[n][c] - from;
+                m[n][c] -= from;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j >> 1][n][(j & 1) * 2 + c] -= from;
+                __syncwarp();
+                if (g == 0) *at = now;
+                __syncwarp();
+              }
+#pragma unroll
               for (int j = 0; j < 4; ++j)  // a token that the row does not see is at -inf, whatever its size
                 y = fmaxf(y, s[j >> 1][n][(j & 1) * 2 + c] + exponent(fmaxf(fabsf(sv[j]), fabsf(ov[j]))));
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) {
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
-              }
-              const float m_now = x > m[n][c] + kSlack ? x : m[n][c];
+              for (int o = 4; o < 32; o <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
               float Y_now = y > Y[n][c] + kRoom ? y - (kRoom - kSlack) : Y[n][c];
               if (m_now != -INFINITY) Y_now = fminf(fmaxf(Y_now, m_now - kDeepest), m_now + kHighest);
               const float keep = ex2(fminf(m[n][c], Y[n][c]) - fminf(m_now, Y_now)), both = ex2(Y[n][c] - Y_now);
@@ -621,7 +653,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           }
         }
       };
-      if ((bits & 3u) == 3u && (step + 1) * kStep <= full) weigh(std::false_type{});
+      if ((bits & 3u) == 3u && (step + 1) * kStep <= full && !apart) weigh(std::false_type{});
       else weigh(std::true_type{});
 
       // ---- values
@@ -678,7 +710,12 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           off[n][c] += __shfl_xor_sync(0xffffffffu, off[n][c], o);
         }
         const int row = n * 8 + 2 * t + c;
-        const float unit = fminf(m[n][c], Y[n][c]), back = m[n][c] == -INFINITY ? 0.0f : ex2(Y[n][c] - unit);
+        // all in 2^m
+        const bool none = m[n][c] == -INFINITY;
+        const float back = none ? 0.0f : ex2(Y[n][c] - m[n][c]), low = none ? 1.0f : ex2(fminf(Y[n][c] - m[n][c], 0.0f));
+        const float2 from = origin[n * 4 + t];
+        l[n][c] *= low;
+        off[n][c] *= low;
         float* dst = so + (warp * R + row) * (D + 4) + g * (D / 8);
         const float mid = 7.5f * ones[n][c];
 #pragma unroll
@@ -686,7 +723,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
           dst[2 * i] = fmaf(fmaf(acc[n][i][c], 16777216.0f, -mid), back, off[n][c]);
           dst[2 * i + 1] = fmaf(fmaf(acc[n][i][c + 2], 1048576.0f, -mid), back, off[n][c]);
         }
-        if (g == 0) sh_stat[warp * R + row] = make_float2(unit, l[n][c]);
+        if (g == 0) sh_stat[warp * R + row] = make_float2(m[n][c] + (c ? from.y : from.x), l[n][c]);
       }
     __syncthreads();
 

@@ -34,6 +34,19 @@ _MAGIC = b"KV4\x01"
 _PRECISION = 16
 
 
+def _frequencies(counts: torch.Tensor) -> torch.Tensor:
+    """Tables of 16 frequencies, at least 1 each, that sum to 2^16, for counts (tables, 16) in 64 bits: what is left
+    of the sum when all are rounded down goes to the most frequent symbol.  (rans_pmf_to_quantized_cdf takes a
+    product in 32 bits, which a symbol of half the sum or more leaves.)"""
+    spare = (1 << _PRECISION) - 16
+    freqs = 1 + counts * spare // counts.sum(1, keepdim=True)
+    return freqs.scatter_add(1, counts.argmax(1, keepdim=True), (1 << _PRECISION) - freqs.sum(1, keepdim=True))
+
+
+def _cdfs(freqs: torch.Tensor) -> torch.Tensor:
+    return torch.nn.functional.pad(freqs.cumsum(1), (1, 0)).to(torch.int32)
+
+
 @dataclass
 class Step:
     """What the tokens that a call adds need on the device: one entry for each token (slots, positions) or
@@ -135,12 +148,12 @@ class PagedKVCache4:
         symbols, indexes = _C.kv4_to_symbols(self.codes, ids, by_channel=by_channel)
         tables = 2 * self.kv_heads * (self.head_dim if by_channel else 1)
         counts = torch.bincount((indexes * 16 + symbols).flatten(), minlength=tables * 16).view(tables, 16)
-        pmf = (counts + 1).float() / (counts + 1).sum(1, keepdim=True)
-        cdfs = _C.rans_pmf_to_quantized_cdf(pmf, _PRECISION)
+        freqs = _frequencies(counts)
+        cdfs = _cdfs(freqs)
         stream = _C.rans64_init_stream(symbols.shape[0], device=str(self.device))
         _C.rans64_push(stream, symbols, indexes, cdfs, *self._sizes(tables), freq_precision=_PRECISION,
                        bypass_coding=False)
-        freqs = cdfs.diff(dim=1).cpu().to(torch.uint16)  # 16 symbols of at least 1: under 2^16 each
+        freqs = freqs.cpu().to(torch.uint16)  # 16 symbols of at least 1: under 2^16 each
         params = self.params[ids].view(torch.int16).cpu()
         return b"".join([head, freqs.numpy().tobytes(), params.numpy().tobytes(), _C.stream_to_merged_bytes(stream, 4)])
 
@@ -170,7 +183,7 @@ class PagedKVCache4:
                 raise ValueError("the stored sequence is cut short")
             raw = torch.frombuffer(bytearray(data), dtype=torch.uint8)
             freqs = raw[at: at + sizes[0]].view(torch.uint16).to(torch.int32).view(tables, 16)
-            cdfs = torch.cat([torch.zeros(tables, 1, dtype=torch.int32), freqs.cumsum(1, dtype=torch.int32)], 1)
+            cdfs = _cdfs(freqs)
             if not bool((cdfs[:, -1] == 1 << _PRECISION).all()) or not bool((freqs > 0).all()):
                 raise ValueError("the stored sequence's tables are not valid")
             params = raw[at + sizes[0]: at + sum(sizes)].view(torch.int16).view(n, 2, kv_heads, page_size, 2)

@@ -138,7 +138,8 @@ class PagedKVCache4:
 
     def store(self, sequence, by_channel: bool = False) -> bytes:
         """A sequence as bytes: a header, the tables' frequencies, the rows' parameters, and the codes as the
-        container of one rANS stream for each page, side and head."""
+        container of one rANS stream for each page, side and head.  Rows of the last page after the sequence's end
+        are zeros: what was in that memory stays there."""
         pages = self._pages[sequence]
         ids = torch.tensor(pages, dtype=torch.int64, device=self.device)
         head = _HEADER.pack(_MAGIC, self._length[sequence], len(pages), self.kv_heads, self.page_size, self.head_dim,
@@ -146,6 +147,10 @@ class PagedKVCache4:
         if not pages:
             return head
         symbols, indexes = _C.kv4_to_symbols(self.codes, ids, by_channel=by_channel)
+        params = self.params[ids]
+        end = self._length[sequence] - (len(pages) - 1) * self.page_size
+        symbols.view(len(pages), -1, self.page_size, self.head_dim)[-1, :, end:] = 0
+        params[-1, :, :, end:] = 0
         tables = 2 * self.kv_heads * (self.head_dim if by_channel else 1)
         counts = torch.bincount((indexes * 16 + symbols).flatten(), minlength=tables * 16).view(tables, 16)
         freqs = _frequencies(counts)
@@ -154,7 +159,7 @@ class PagedKVCache4:
         _C.rans64_push(stream, symbols, indexes, cdfs, *self._sizes(tables), freq_precision=_PRECISION,
                        bypass_coding=False)
         freqs = freqs.cpu().to(torch.uint16)  # 16 symbols of at least 1: under 2^16 each
-        params = self.params[ids].view(torch.int16).cpu()
+        params = params.view(torch.int16).cpu()
         return b"".join([head, freqs.numpy().tobytes(), params.numpy().tobytes(), _C.stream_to_merged_bytes(stream, 4)])
 
     def load(self, data: bytes, sequence) -> None:

@@ -20,6 +20,7 @@ reference's format (``rans64_push`` / ``rans64_pop`` and the container of ``merg
 from __future__ import annotations
 
 import struct
+import zlib
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence
 
@@ -30,7 +31,9 @@ from . import _C
 __all__ = ["PagedKVCache4", "Step"]
 
 _HEADER = struct.Struct("<4sIIIIII")  # magic, length, pages, kv_heads, page_size, head_dim, tables by channel
-_MAGIC = b"KV4\x01"
+_MAGIC = b"KV4\x02"
+_MAGIC_1 = b"KV4\x01"  # the same without the checksum at the end
+_CRC = struct.Struct("<I")  # of all before it
 _PRECISION = 16
 
 
@@ -138,14 +141,14 @@ class PagedKVCache4:
 
     def store(self, sequence, by_channel: bool = False) -> bytes:
         """A sequence as bytes: a header, the tables' frequencies, the rows' parameters, and the codes as the
-        container of one rANS stream for each page, side and head.  Rows of the last page after the sequence's end
+        container of one rANS stream for each page, side and head, and a checksum of all that.  Rows of the last page after the sequence's end
         are zeros: what was in that memory stays there."""
         pages = self._pages[sequence]
         ids = torch.tensor(pages, dtype=torch.int64, device=self.device)
         head = _HEADER.pack(_MAGIC, self._length[sequence], len(pages), self.kv_heads, self.page_size, self.head_dim,
                             int(by_channel))
         if not pages:
-            return head
+            return head + _CRC.pack(zlib.crc32(head))
         symbols, indexes = _C.kv4_to_symbols(self.codes, ids, by_channel=by_channel)
         params = self.params[ids]
         end = self._length[sequence] - (len(pages) - 1) * self.page_size
@@ -160,47 +163,63 @@ class PagedKVCache4:
                        bypass_coding=False)
         freqs = freqs.cpu().to(torch.uint16)  # 16 symbols of at least 1: under 2^16 each
         params = params.view(torch.int16).cpu()
-        return b"".join([head, freqs.numpy().tobytes(), params.numpy().tobytes(), _C.stream_to_merged_bytes(stream, 4)])
+        data = b"".join([head, freqs.numpy().tobytes(), params.numpy().tobytes(), _C.stream_to_merged_bytes(stream, 4)])
+        return data + _CRC.pack(zlib.crc32(data))
 
     def load(self, data: bytes, sequence) -> None:
-        """Bring a stored sequence back under a new name."""
+        """Bring a stored sequence back under a new name.  Raises ValueError, and changes nothing, for bytes that are not
+        a whole stored sequence of this layout."""
         if sequence in self._pages:
             raise ValueError(f"sequence {sequence!r} is in the cache")
         if len(data) < _HEADER.size:
             raise ValueError("not a stored sequence")
         magic, length, n, kv_heads, page_size, head_dim, by_channel = _HEADER.unpack_from(data)
-        if magic != _MAGIC:
+        if magic not in (_MAGIC, _MAGIC_1):
             raise ValueError("not a stored sequence")
-        if (kv_heads, page_size, head_dim) != (self.kv_heads, self.page_size, self.head_dim) or n != -(-length // page_size):
+        body = len(data) - (_CRC.size if magic == _MAGIC else 0)
+        if (kv_heads, page_size, head_dim) != (self.kv_heads, self.page_size, self.head_dim) or \
+                n != -(-length // page_size) or by_channel > 1:
             raise ValueError("the stored sequence is of another cache layout")
         if n > len(self._free):
             raise RuntimeError(f"the cache has {len(self._free)} free pages, and {n} are needed")
-        if n:
+        if not n:
+            self._whole(data, _HEADER.size, body)
+        else:
             tables, rows = 2 * kv_heads * (head_dim if by_channel else 1), n * 2 * kv_heads
             at = _HEADER.size
             sizes = (tables * 16 * 2, rows * page_size * 2 * 2)
-            if len(data) < at + sum(sizes):
+            if body < at + sum(sizes):
                 raise ValueError("the stored sequence is cut short")
             end = at + sum(sizes)
             for _ in range(rows):  # the container's records: each as long as it says, the last ends the data
-                end += 4 + struct.unpack_from("<I", data, end)[0] if end + 4 <= len(data) else len(data)
-            if end != len(data):
-                raise ValueError("the stored sequence is cut short")
+                end += 4 + struct.unpack_from("<I", data, end)[0] if end + 4 <= body else body + 1
             raw = torch.frombuffer(bytearray(data), dtype=torch.uint8)
             freqs = raw[at: at + sizes[0]].view(torch.uint16).to(torch.int32).view(tables, 16)
             cdfs = _cdfs(freqs)
             if not bool((cdfs[:, -1] == 1 << _PRECISION).all()) or not bool((freqs > 0).all()):
                 raise ValueError("the stored sequence's tables are not valid")
+            self._whole(data, end, body)
             params = raw[at + sizes[0]: at + sum(sizes)].view(torch.int16).view(n, 2, kv_heads, page_size, 2)
-            stream = _C.merged_tensor_to_stream(raw[at + sum(sizes):].clone(), 4, device=str(self.device))
+            stream = _C.merged_tensor_to_stream(raw[at + sum(sizes): end].clone(), 4, device=str(self.device))
             ids = torch.tensor(self._free[-n:][::-1], dtype=torch.int64, device=self.device)
             _, indexes = _C.kv4_to_symbols(self.codes, ids, by_channel=bool(by_channel))
+            before = _C.device_status(self.device.index, reset=False)
             symbols = _C.rans64_pop(stream, indexes, cdfs.to(self.device), *self._sizes(tables),
                                     freq_precision=_PRECISION, bypass_coding=False)
+            if _C.device_status(self.device.index, reset=before == 0) & ~before:
+                raise ValueError("the stored sequence's streams are damaged")
             _C.kv4_from_symbols(symbols, self.codes, ids)
             self.params[ids] = params.to(self.device).view(torch.bfloat16)
         self._pages[sequence] = [self._free.pop() for _ in range(n)]
         self._length[sequence] = length
+
+    @staticmethod
+    def _whole(data: bytes, end: int, body: int) -> None:
+        """What the parts add up to is what is there, and the checksum (where there is one) is right."""
+        if end != body:
+            raise ValueError("the stored sequence is cut short")
+        if body < len(data) and zlib.crc32(memoryview(data)[:body]) != _CRC.unpack_from(data, body)[0]:
+            raise ValueError("the stored sequence is damaged")
 
     def _sizes(self, tables: int):
         full = dict(dtype=torch.int32, device=self.device)

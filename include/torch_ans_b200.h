@@ -234,9 +234,10 @@ int tans_cdf_fix_zero_freqs(int32_t* cdfs, int64_t rows, int64_t n, uint32_t* de
  *           in the low half of a byte; [:, 0] keys, [:, 1] values
  *   params  bfloat16 [num_pages, 2, kv_heads, page_size, 2]          (scale, offset) of each row
  * A code c stands for c * scale + offset.  A row x is stored with offset = bf16(min x),
- * scale = bf16((max x - offset) / 15) (0 when that is under 2^-100) and
- * c = round-half-even((x - offset) / scale) clamped to 0..15; a row that is not finite is stored
- * with NaN parameters and reads back as NaN.  A slot numbers a token's place: page * page_size +
+ * scale = bf16((max x - offset) * r), r the float nearest 1/15 and difference and product rounded to
+ * float (0 when the scale is under 2^-100), and c = round-half-even((x - offset) / scale) clamped to
+ * 0..15, the quotient rounded to float first; a row that is not finite is stored with NaN parameters
+ * and reads back as NaN.  A slot numbers a token's place: page * page_size +
  * place in the page.  head_dim is 64, 128 or 256, page_size a multiple of 16.  dtype (TANS_BF16 or
  * TANS_FP16) is that of queries, keys, values and outputs; their rows (one token's head) are
  * contiguous, strides are in elements. */
@@ -248,7 +249,8 @@ int tans_cdf_fix_zero_freqs(int32_t* cdfs, int64_t rows, int64_t n, uint32_t* de
  *   k, v      [tokens, kv_heads, head_dim]; q [tokens, q_heads, head_dim] or NULL
  *   q_out     [tokens, q_heads, head_dim], packed: the rotated queries (NULL without q)
  *   slots     int64[tokens]; a negative slot stores nothing, one past the pool is skipped and
- *             flags TANS_DEV_BAD_INDEX.  Two tokens with the same slot leave either's row.
+ *             flags TANS_DEV_BAD_INDEX.  Tokens with the same slot leave an unspecified mixture of
+ *             their rows: codes of one may lie beside another's scale and offset.
  *   rotation  float [rotation_rows, rotary_dim]: cosines of the rotary_dim / 2 angles, then their
  *             sines, one row per position; NULL = no rotation.  rotary_dim is a multiple of 16.
  *   positions int64[tokens], rows of `rotation`; one outside is not rotated and flags

@@ -283,7 +283,9 @@ int tans_kv4_gather(const uint8_t* codes, const void* params, int64_t num_pages,
  *             TANS_DEV_BAD_VALUE.
  *   q_starts  int32 [batch + 1], from 0 upwards; NULL: one query for each sequence.  Queries before
  *             the first start and after the last give zeros.  A sequence whose two starts are out of
- *             order or past the queries is skipped and flags TANS_DEV_BAD_VALUE.
+ *             order or past the queries is skipped and flags TANS_DEV_BAD_VALUE; queries that no
+ *             sequence answers are zeros (with -inf in lse), ones of several have one's answer or zeros.
+ *             Work past 2^36 tokens or so in one call answers nothing: all zeros, and the flag.
  *   max_queries  the caller's bound on one sequence's queries; it chooses the kernel only.
  *   lse       float [total_queries, q_heads] or NULL: log of the softmax's sum (-inf for none).
  *   workspace tans_kv4_attend_workspace_size() bytes, 256-byte aligned.  Its first

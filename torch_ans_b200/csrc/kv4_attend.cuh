@@ -28,9 +28,11 @@ struct AttendArgs {
   int wait_limit;  // tries of a wait of one warp for another, a microsecond each at most
 };
 
-// One sequence: its tokens, its queries (first and number).
+// One sequence: its tokens, its queries (first and number); not ok: its starts are out of order or past the
+// queries, and it has none.
 struct Sequence {
   int length, start, count;
+  bool ok;
 };
 
 __device__ __forceinline__ void flag(uint32_t* status, uint32_t bit) {
@@ -39,12 +41,13 @@ __device__ __forceinline__ void flag(uint32_t* status, uint32_t bit) {
 
 __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int64_t b, bool report) {
   Sequence s;
+  s.ok = true;
   if (a.q_starts) {
     const int lo = a.q_starts[b], hi = a.q_starts[b + 1];
-    const bool ok = lo >= 0 && hi >= lo && hi <= a.total_queries;
-    if (!ok && report) flag(a.status, TANS_DEV_BAD_VALUE);
-    s.start = ok ? lo : 0;
-    s.count = ok ? hi - lo : 0;
+    s.ok = lo >= 0 && hi >= lo && hi <= a.total_queries;
+    if (!s.ok && report) flag(a.status, TANS_DEV_BAD_VALUE);
+    s.start = s.ok ? lo : 0;
+    s.count = s.ok ? hi - lo : 0;
   } else {
     s.start = (int)b;
     s.count = 1;
@@ -70,6 +73,31 @@ __device__ __forceinline__ void zero_unowned(const AttendArgs& a, int dim, int64
     static_cast<T*>(a.out)[at * dim + e % dim] = Half2<T>::round(0.0f);
     if (a.lse && e % dim == 0) a.lse[at] = -INFINITY;
   }
+}
+
+// For starts that are not in order: queries that no sequence answers, one at a time by some threads, become
+// zeros.  `tiles` row tiles of `rows` rows are answered, in the order of the sequences.
+static __device__ __noinline__ void zero_unanswered(const int32_t* q_starts, int64_t batch, int64_t total_queries, int group,
+                                                    int64_t row_elements, uint16_t* out, float* lse, int q_heads,
+                                                    int64_t thread, int64_t threads, int rows, int64_t tiles) {
+  for (int64_t i = thread; i < total_queries; i += threads) {
+    bool answered = false;
+    int64_t before = 0;
+    for (int64_t b = 0; b < batch && !answered; ++b) {
+      const int lo = q_starts ? q_starts[b] : (int)b, hi = q_starts ? q_starts[b + 1] : (int)b + 1;
+      if (lo < 0 || hi < lo || hi > total_queries) continue;
+      before += ((int64_t)(hi - lo) * group + rows - 1) / rows;
+      answered = i >= lo && i < hi && before <= tiles;
+    }
+    if (answered) continue;
+    for (int64_t e = 0; e < row_elements; ++e) out[i * row_elements + e] = 0;
+    for (int h = 0; lse && h < q_heads; ++h) lse[i * q_heads + h] = -INFINITY;
+  }
+}
+__device__ __forceinline__ void zero_unanswered(const AttendArgs& a, int dim, int64_t thread, int64_t threads, int rows,
+                                                int64_t tiles) {
+  zero_unanswered(a.q_starts, a.batch, a.total_queries, a.group.d, (int64_t)a.q_heads * dim, static_cast<uint16_t*>(a.out),
+                  a.lse, a.q_heads, thread, threads, rows, tiles);
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -377,7 +377,7 @@ __device__ __forceinline__ Work work_at(const AttendArgs& a, const Split& split,
   int before = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < (int)a.batch && !w.some; b0 += 32) {
-    Sequence s{0, 0, 0};
+    Sequence s{0, 0, 0, true};
     int tiles = 0;
     if (b0 + lane < a.batch) {
       s = sequence(a, b0 + lane, false);
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       s_full[TILES][2], p_full[TILES][2], o_done[TILES], o_full, w_next, w_full[kQueue],
       w_empty[kQueue];
   __shared__ uint32_t tensor_base;
-  __shared__ int stalled_, sh_last;
+  __shared__ int stalled_, sh_last, sh_skipped;
   __shared__ Info infos[kInfos];
   __shared__ Work queue[kQueue];
   __shared__ float factors[2][RT];  // of two pieces' rows
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   const int heads = a.pool.kv_heads;
 
   if (threadIdx.x == 0) {
-    stalled_ = 0;
+    stalled_ = sh_skipped = 0;
     bar_init(&q_full, RT);
     bar_init(&q_empty, 1);
     for (int i = 0; i < STAGES; ++i) {
@@ -465,7 +465,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   }
   __syncthreads();
   if (blockIdx.x == 0)  // what is wrong with lengths and starts is reported once
-    for (int64_t b = threadIdx.x; b < a.batch; b += P::WARPS * 32) sequence(a, b, true);
+    for (int64_t b = threadIdx.x; b < a.batch; b += P::WARPS * 32)
+      if (!sequence(a, b, true).ok) sh_skipped = 1;
   // A group's next piece of work, and its return once it is read by the whole warp.
   auto take = [&](int number) -> const Work& {
     bar_wait(&w_full[number % kQueue], number / kQueue & 1, a.wait_limit, stalled);
@@ -1094,6 +1095,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tensor_base));
   }
   zero_unowned<T>(a, D, blockIdx.x * (int64_t)(P::WARPS * 32) + threadIdx.x, (int64_t)gridDim.x * P::WARPS * 32);
+  if (blockIdx.x == 0 && sh_skipped)
+    zero_unanswered(a, D, threadIdx.x, P::WARPS * 32, RT, work / (split.splits * heads));
 }
 
 // Row tiles times heads, at most: one tile that is not full for each sequence that has queries.

@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
   __shared__ int64_t sh_scan[kWarps];
   __shared__ int sh_found[2];
   __shared__ Sequence sh_sequence;
-  __shared__ int sh_last;
+  __shared__ int sh_last, sh_skipped;
   __shared__ float2 sh_stat[kWarps * R], sh_total[R], sh_origin[kWarps][R / 2];
   __shared__ float sh_weight[2 * kMostParts][R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -222,8 +222,9 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
   };
   constexpr int64_t kUnits = ((int64_t)1 << 40) - 1;
   const int batch = (int)a.batch;
+  if (threadIdx.x == 0) sh_skipped = 0;
   int64_t all = 0, items = 0, mine = 0, before = 0;
-  Sequence seq{0, 0, 0};
+  Sequence seq{0, 0, 0, true};
   for (int b = 0; b < batch; b += kWarps * 32) {
     int64_t sum;
     mine = 0;
@@ -234,12 +235,14 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
       mine = min(items_of(seq) * steps_of(seq), (int64_t)1 << 31) | mine << 40;
     }
     before = all + (block_scan(mine, sum) & kUnits);
+    if (!seq.ok) sh_skipped = 1;
     all += sum & kUnits;
     items += sum >> 40;
     mine &= kUnits;
   }
-  if (all > 0x7f000000) {  // starts that cross one another: no call within memory has so much work
+  if (all > 0x7f000000) {  // starts that cross one another, or 2^36 tokens together: nothing is answered
     if (blockIdx.x == 0 && threadIdx.x == 0) flag(a.status, TANS_DEV_BAD_VALUE);
+    zero_unanswered(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32, R, -1);
     return;
   }
   // With fewer items than half the blocks, each item has blocks of its own: as many as take `share` or
@@ -258,6 +261,10 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
   }
   auto zero_rest = [&]() {
     zero_unowned<T>(a, D, blockIdx.x * (int64_t)(kWarps * 32) + threadIdx.x, (int64_t)gridDim.x * kWarps * 32);
+    if (blockIdx.x == 0) {
+      __syncthreads();
+      if (sh_skipped) zero_unanswered(a, D, threadIdx.x, kWarps * 32, R, INT64_MAX);
+    }
   };
   const int64_t start = (int64_t)blockIdx.x * (own ? 1 : share);
   if (start >= all) {

@@ -110,7 +110,11 @@ __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(bar)) : "memory");
 }
 // A bounded wait.  One that runs out is recorded in `stalled`; waits after that return at once, so the
-// block comes to its end (with values that are not valid) and frees its tensor memory.
+// block comes to its end (with values that are not valid) and frees its tensor memory.  Warps leave their
+// loops early then, each as a whole (`stalled` is read by a vote where it decides); warps that meet at a named
+// barrier later on decide together, at that barrier (any_of), so that none waits there for one that has left.
+// What a wait was to protect is not written after one that ran out where others take addresses from it (the
+// queue).
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, int tries, volatile int* stalled) {
   const uint32_t at = smem_of(bar);
   uint32_t done;
@@ -129,6 +133,17 @@ __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, int tri
     if (*stalled) return;
   }
   *stalled = 1;
+}
+
+// A barrier of `threads` that tells all of them whether `one` is true for any.
+template <int BARRIER, int THREADS>
+__device__ __forceinline__ bool any_of(bool one) {
+  uint32_t any;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbar.red.or.pred p, %2, %3, q;\nselp.b32 %0, 1, 0, p;\n}\n"
+               : "=r"(any)
+               : "r"((uint32_t)one), "n"(BARRIER), "n"(THREADS)
+               : "memory");
+  return any != 0;
 }
 
 // true for one thread of the warp
@@ -439,7 +454,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   const int heads = a.pool.kv_heads;
 
   if (threadIdx.x == 0) {
-    stalled_ = sh_skipped = 0;
+    stalled_ = sh_skipped = sh_last = 0;
     bar_init(&q_full, RT);
     bar_init(&q_empty, 1);
     for (int i = 0; i < STAGES; ++i) {
@@ -497,7 +512,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
 #pragma unroll 1
     for (;; ++number) {
       const Work& k = take(number);  // read again where it is used: registers are dear here
-      if (!k.some || *stalled) break;
+      const bool none = !k.some || *stalled;
+      if (SPLIT ? any_of<2, RT>(none) : __any_sync(0xffffffffu, none) != 0) break;  // SPLIT: they all meet at the join
       const int seen = row >= k.rows ? 0 : (a.causal ? min(k.seq.length, k.ahead + a.group.div(k.row0 + row)) : k.seq.length);
       const int halves = tile * kTile < k.rows ? k.halves : 0;  // a tile without rows has nothing to wait for
       int left_all = seen - k.step0 * kTile;  // tokens of what is still to come that the row sees
@@ -749,7 +765,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       if (valid && first) {
         do {  // pieces in which nothing is seen are passed over
           const Work& k = take(number);
-          valid = k.some && !*stalled;
+          valid = !__any_sync(0xffffffffu, !k.some || *stalled);
           steps_left = k.steps;
           length = k.seq.length;
           in_head = k.head;
@@ -888,8 +904,8 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
     int stage = 0;
     uint32_t filled = 0;
 #pragma unroll 1
-    for (uint32_t j = 0; there; ++j) {
-      if (begun) {
+    for (uint32_t j = 0;; ++j) {
+      if (there && begun) {
         if (items > 0) bar_wait(&q_empty, (items - 1) & 1, a.wait_limit, stalled);
         __syncwarp();
         copy_queries(queue[slot_now % kQueue]);
@@ -908,7 +924,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       }
       const bool bad = state == 1 && !finite_row(vp);
       const uint32_t hidden = __ballot_sync(0xffffffffu, state == 2), wrong = __ballot_sync(0xffffffffu, bad);
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (any_of<1, 256>(!there || *stalled)) break;  // the ranges are there; or some warp has no more
       int key_top = kLeast, value_top = kLeast, key_low = 255, value_low = 255;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -996,7 +1012,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       for (int number = 0;; ++number) {
         const Work& k = take(number);
         const int steps = k.steps, halves = k.halves, tiles = (k.rows + kTile - 1) / kTile;
-        const bool some = k.some && !*stalled;
+        const bool some = !__any_sync(0xffffffffu, !k.some || *stalled);
         give_back(number);
         if (!some) break;
         if (steps <= 0) continue;
@@ -1071,6 +1087,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
           continue;
         }
         bar_wait(&w_empty[number % kQueue], number / kQueue & 1 ^ 1, a.wait_limit, stalled);
+        if (__any_sync(0xffffffffu, *stalled)) break;  // the place may be in use; nobody waits for it
         if (lane == 0) {
           queue[number % kQueue] = w;
           bar_arrive(&w_full[number % kQueue]);
@@ -1080,7 +1097,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         // one that is taken earlier than it is needed may be one that another block would end sooner
         bar_wait(&w_next, number & 1, a.wait_limit, stalled);
         ++number;
-        n = SPLIT || *stalled ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
+        n = SPLIT || __any_sync(0xffffffffu, *stalled) ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
       }
       // every block has had its last number when the last of them comes here
       if (!SPLIT && lane == 0 && arrive(split.arrivals + 1, gridDim.x)) split.arrivals[0] = 0;

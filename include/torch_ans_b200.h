@@ -290,9 +290,8 @@ int tans_kv4_gather(const uint8_t* codes, const void* params, int64_t num_pages,
  *   lse       float [total_queries, q_heads] or NULL: log of the softmax's sum (-inf for none).
  *   workspace tans_kv4_attend_workspace_size() bytes, 256-byte aligned.  Its first
  *             TANS_KV4_ATTEND_COUNTS bytes are zero before the first call and are left zero by each
- *             call that does not flag TANS_DEV_STALLED (clear them after one that does); calls that
- *             may overlap need workspaces of their own.  NULL allocates and clears one
- *             stream-ordered. */
+ *             call, one that flags TANS_DEV_STALLED included; calls that may overlap need
+ *             workspaces of their own.  NULL allocates and clears one stream-ordered. */
 #define TANS_KV4_ATTEND_COUNTS 10240
 size_t tans_kv4_attend_workspace_size(int64_t total_queries, int q_heads, int kv_heads, int head_dim, int64_t batch,
                                       int64_t max_pages, int page_size, int64_t max_queries);

@@ -74,22 +74,12 @@ Kept& kept_workspaces() {
   return k;
 }
 
-// A call that stalled may have left its workspace's counts as they were: the next one gets a new one.
-void after_stall(int device, int32_t bits) {
-  if (!(bits & (int32_t)TANS_DEV_STALLED)) return;
-  Kept& k = kept_workspaces();
-  std::lock_guard<std::mutex> g(k.mu);
-  for (auto it = k.by_stream.begin(); it != k.by_stream.end();)
-    it = it->first.first == device ? k.by_stream.erase(it) : std::next(it);
-}
-
 void after_op(const at::Device& dev) {
   if (!(g_force_check || sync_check_enabled())) return;
   Tensor& w = status_word(dev);
   const int32_t bits = w.item<int32_t>();  // synchronises the current stream
   if (bits != 0) {
     w.zero_();
-    after_stall(dev.index(), bits);
     throw std::runtime_error("torch_ans_b200: device reported:" + status_bits_string((uint32_t)bits));
   }
 }
@@ -1020,10 +1010,7 @@ int64_t device_status(std::optional<int64_t> device, bool reset) {
   const int64_t d = device.has_value() ? *device : (int64_t)c10::cuda::current_device();
   Tensor& w = status_word(at::Device(at::kCUDA, (c10::DeviceIndex)d));
   const int32_t v = w.item<int32_t>();
-  if (reset) {
-    w.zero_();
-    after_stall((int)d, v);
-  }
+  if (reset) w.zero_();
   return v;
 }
 

@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       w_empty[kQueue];
   __shared__ uint32_t tensor_base;
   __shared__ int stalled_, sh_last, sh_skipped;
+  __shared__ int owed_at, owed;  // SPLIT: the count at which this block is expected, and by how many; 0 when it was there
   __shared__ Info infos[kInfos];
   __shared__ Work queue[kQueue];
   __shared__ float factors[2][RT];  // of two pieces' rows
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   const int heads = a.pool.kv_heads;
 
   if (threadIdx.x == 0) {
-    stalled_ = sh_skipped = sh_last = 0;
+    stalled_ = sh_skipped = sh_last = owed = 0;
     bar_init(&q_full, RT);
     bar_init(&q_empty, 1);
     for (int i = 0; i < STAGES; ++i) {
@@ -699,7 +700,10 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         split.stats[mine * RT + row] = make_float2(m, l);
         __threadfence();
         asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
-        if (threadIdx.x == 0) sh_last = arrive(split.arrivals + tile_head, parts);
+        if (threadIdx.x == 0) {
+          sh_last = arrive(split.arrivals + tile_head, parts);
+          owed = 0;
+        }
         asm volatile("bar.sync 2, %0;" ::"n"(RT) : "memory");
         if (sh_last) {
           __threadfence();
@@ -1082,6 +1086,10 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       for (;;) {
         Work w{};
         if (n < work) w = work_at<RT>(a, split, n, lane);
+        if (SPLIT && w.some && w.parts > 1 && lane == 0) {
+          owed_at = w.tile_head;
+          owed = w.parts;
+        }
         if (n < work && !w.some) {
           n = SPLIT ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
           continue;
@@ -1106,6 +1114,9 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
   fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && stalled_) flag(a.status, TANS_DEV_STALLED);
+  // A block that stalled before its join arrives all the same: the counts are zero after every call.  (Its row
+  // tile may then be joined by nobody, or with what is not valid: the flag says so.)
+  if (SPLIT && threadIdx.x == 0 && owed > 0) arrive(split.arrivals + owed_at, owed);
   if (warp == kIssue) {
     __syncwarp();
     fence_after();

@@ -47,3 +47,22 @@ def test_calls_end_and_the_next_one_is_right(monkeypatch, lengths, counts, dim):
         status.zero_()
         assert torch.equal(call(), first) and status.item() == 0
     assert _C.device_status() == 0
+
+
+def test_a_long_piece_of_work_is_not_a_stall(monkeypatch):
+    """The warp that looks work up waits while a row tile's tokens are gone through, which takes as long as they are many:
+    524,288 here (one page again and again), some ten milliseconds, under a limit of less than one."""
+    from torch_ans_b200 import _C
+    _C.device_status()
+    page, heads, n = 1 << 14, 64, 700
+    codes, params = P.pool(1, 1, page, 64)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = torch.zeros(1, 32, **i32)
+    q = torch.randn(n, heads, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.bfloat16)
+    args = (q, codes, params, pages, torch.tensor([32 * page], **i32))
+    kw = dict(q_starts=torch.tensor([0, n], **i32), max_queries=n)
+    first = _C.kv4_attend(*args, **kw)
+    assert _C.device_status() == 0
+    monkeypatch.setenv("TORCH_ANS_B200_WAIT_LIMIT", "700")
+    assert torch.equal(_C.kv4_attend(*args, **kw), first)
+    assert _C.device_status() == 0

@@ -56,7 +56,7 @@ extern "C" int tans_kv4_attend(const void* q, int64_t q_token_stride, int64_t q_
                      q, q_token_stride, q_head_stride, total_queries, q_heads,
                      Divider::of(group), Divider::of(kv_heads), Divider::of(page_size), pages, batch, max_pages, lengths,
                      q_starts, scale * 1.4426950408889634f, causal, vec, out, lse, dev_status,
-                     tans::env_int("TORCH_ANS_B200_WAIT_LIMIT", 1 << 20)};
+                     std::min(tans::env_int("TORCH_ANS_B200_WAIT_LIMIT", 1 << 20), 1 << 30)};
   const int64_t most = std::min(max_queries, total_queries);
   const size_t need = tans_kv4_attend_workspace_size(total_queries, q_heads, kv_heads, head_dim, batch, max_pages,
                                                      page_size, max_queries);

@@ -1081,7 +1081,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       // ---------------------------------------------------------------- scheduling
       // The first pieces are the blocks' by their numbers, the others whoever's is free: pieces of a
       // causal prompt differ by the tokens that they see, the largest come first.
-      int number = 0, n = blockIdx.x;
+      int number = 0, n = blockIdx.x, steps = 0;  // of the piece before
 #pragma unroll 1
       for (;;) {
         Work w{};
@@ -1102,8 +1102,10 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         }
         __syncwarp();
         if (!w.some) break;
-        // one that is taken earlier than it is needed may be one that another block would end sooner
-        bar_wait(&w_next, number & 1, a.wait_limit, stalled);
+        // One that is taken earlier than it is needed may be one that another block would end sooner.  The one
+        // before it goes first: 16 tries more for each of its steps, which take two or three microseconds.
+        bar_wait(&w_next, number & 1, a.wait_limit + 16 * steps, stalled);
+        steps = w.steps;
         ++number;
         n = SPLIT || __any_sync(0xffffffffu, *stalled) ? work : gridDim.x + __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(split.arrivals, 1) : 0, 0);
       }

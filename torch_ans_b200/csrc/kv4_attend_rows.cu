@@ -182,8 +182,12 @@ __device__ __forceinline__ void join_parts(const Join& j, int first_place, int f
   }
 }
 
+// Blocks on an SM: four (two where registers allow no more), three for row tiles of 16 with head_dim 64, which
+// spilled with four (64 contexts of 700 tokens, 8 heads, 16 rows 29 us, was 34; 64 rows over 8,192 tokens 82, was 92).
+constexpr int blocks_of(int dim, int nt) { return dim * nt > 128 ? 2 : (nt == 2 ? 3 : 4); }
+
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_rows_kernel(const RowsArgs p) {
+__global__ void __launch_bounds__(kWarps * 32, blocks_of(D, NT)) attend_rows_kernel(const RowsArgs p) {
   const AttendArgs& a = p.a;
   using S = Stage<D>;
   constexpr int R = 8 * NT, KW = D / 32, VW = D / 64;  // rows of a tile; words of a key / value row's share of a lane
@@ -589,37 +593,62 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
 #pragma unroll
           for (int c = 0; c < 2; ++c) move |= top[n][c] > m[n][c] + kSlack || top[n][c] + reach > Y[n][c];
         if (__any_sync(0xffffffffu, move)) {
+          // the columns' reductions side by side: the largest scores, then the largest products
+          float now[NT][2], y[NT][2];
+          auto across = [&](float (&v)[NT][2]) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+              for (int i = 0; i < 2 * NT; ++i) v[i >> 1][i & 1] = fmaxf(v[i >> 1][i & 1], __shfl_xor_sync(0xffffffffu, v[i >> 1][i & 1], o));
+          };
+#pragma unroll
+          for (int i = 0; i < 2 * NT; ++i) now[i >> 1][i & 1] = top[i >> 1][i & 1];
+          across(now);
+          bool far = false;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float x = top[n][c], y = -INFINITY;
+              now[n][c] = now[n][c] > m[n][c] + kSlack ? now[n][c] : m[n][c];
+              far |= now[n][c] != -INFINITY && fabsf(now[n][c]) > kFar;
+            }
+          if (__any_sync(0xffffffffu, far)) {
+            apart = true;
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-              float m_now = x > m[n][c] + kSlack ? x : m[n][c];
-              const bool far = m_now != -INFINITY && fabsf(m_now) > kFar;
-              if (__any_sync(0xffffffffu, far)) {
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
                 float* const at = reinterpret_cast<float*>(origin) + (n * 4 + t) * 2 + c;
-                const float old = *at, now = old + (far ? m_now : 0.0f), from = now - old;
-                apart = true;
-                m_now -= from;
+                const bool moves = now[n][c] != -INFINITY && fabsf(now[n][c]) > kFar;
+                const float old = *at, to = old + (moves ? now[n][c] : 0.0f), from = to - old;
+                now[n][c] -= from;
                 Y[n][c] = m[n][c] == -INFINITY ? kNone : Y[n][c] - from;
                 m[n][c] -= from;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[j >> 1][n][(j & 1) * 2 + c] -= from;
                 __syncwarp();
-                if (g == 0) *at = now;
-                __syncwarp();
+                if (g == 0) *at = to;
               }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              y[n][c] = -INFINITY;
 #pragma unroll
               for (int j = 0; j < 4; ++j)  // a token that the row does not see is at -inf, whatever its size
-                y = fmaxf(y, s[j >> 1][n][(j & 1) * 2 + c] + exponent(fmaxf(fabsf(sv[j]), fabsf(ov[j]))));
+                y[n][c] = fmaxf(y[n][c], s[j >> 1][n][(j & 1) * 2 + c] + exponent(fmaxf(fabsf(sv[j]), fabsf(ov[j]))));
+            }
+          across(y);
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
-              float Y_now = y > Y[n][c] + kRoom ? y - (kRoom - kSlack) : Y[n][c];
-              if (m_now != -INFINITY) Y_now = fminf(fmaxf(Y_now, m_now - kDeepest), m_now + kHighest);
-              const float keep = ex2(fminf(m[n][c], Y[n][c]) - fminf(m_now, Y_now)), both = ex2(Y[n][c] - Y_now);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float Y_now = y[n][c] > Y[n][c] + kRoom ? y[n][c] - (kRoom - kSlack) : Y[n][c];
+              if (now[n][c] != -INFINITY) Y_now = fminf(fmaxf(Y_now, now[n][c] - kDeepest), now[n][c] + kHighest);
               if (m[n][c] != -INFINITY) {  // nothing is kept before the first token
+                const float keep = ex2(fminf(m[n][c], Y[n][c]) - fminf(now[n][c], Y_now)), both = ex2(Y[n][c] - Y_now);
                 l[n][c] *= keep;
                 off[n][c] *= keep;
                 ones[n][c] *= both;
@@ -629,7 +658,7 @@ __global__ void __launch_bounds__(kWarps * 32, D * NT <= 128 ? 4 : 2) attend_row
                   acc[n][i][c + 2] *= both;
                 }
               }
-              m[n][c] = m_now;
+              m[n][c] = now[n][c];
               Y[n][c] = Y_now;
             }
         }

@@ -21,11 +21,12 @@
 // sums in the workspace, and the last of them joins them in the order of the tokens.
 //
 // All operands are float16 brought into range by powers of two: a query row by its own, the keys and the
-// values of a step by one each.  A row of keys or values that is over 2^5 smaller than the step's largest
-// would come too near float16's least number: a step with such a row is "wide", and there each row has its
-// own factor, which the softmax warps put into its scores and weights (two 2^x a score instead of one).  So
-// the rounding is 2^-11 of each key, each row of values and each weight, whatever the sizes of other
-// tokens, of those that are hidden from a query too; sums are float.
+// values of a step by one each.  Rows that differ by over 2^5 need another conversion (1 % of the time if all steps
+// do); rows that differ by more than 2^20 (keys) or 2^12 (values) would lose bits of themselves or of the weights:
+// a step with such rows is "wide", and there each row has its own factor, which the softmax warps put into
+// its scores and weights, in some seven times the time.  So the rounding is 2^-11
+// of each key, each value and each weight, whatever the sizes of other tokens, of those that are hidden
+// from a query too; sums are float.
 //
 // A query row's weights are 2^(x - m - d) for the score x, its running maximum m and a power of two d of
 // its own over the step's: it follows the largest product of a weight and a value's size that the row sees, and
@@ -34,15 +35,16 @@
 // x - (m + d); where |m| passes 2^10 they are rounded first and m is taken from them, token by token as in a
 // wide step: the product's rounding would otherwise be a factor of the weight, past float's range from 2^30.
 //
-// Measured: 4 packed prompts of 1,143 to 3,500 tokens (32 query and 8 key/value heads of 128, 166 GFLOP) 234
-// us, 709 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 165 us, 412 TFLOP/s.  With one power
+// Measured: 4 packed prompts of 1,143 to 3,500 tokens (32 query and 8 key/value heads of 128, 166 GFLOP) 236
+// us, 703 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 166 us, 412 TFLOP/s.  With one power
 // of two for all values so far and none for single rows these took 228 and 161 us on the same GPU, and a value 2^16
-// times larger in a step, seen or not, left other queries' answers a fifth wrong.  A half step takes about 2,000
-// cycles, in which the products are busy for 1,280 (head_dim 128), 2^x for 1,024 and the instructions' issue
-// for 900 a scheduler: leaving out any one of them, or the unpacking, in a copy took 2 to 4 % off (17 % for 2^x
-// at head_dim 64), so it is the latency of all of them together.  Steps of 128 tokens whose softmax waits for
-// its own products took 261 us where half steps took 243; without the blocks' going on by themselves 243
-// against 233.
+// times larger in a step, seen or not, left other queries' answers a fifth wrong.  Such prompts with one row in
+// 16 2^8 times larger: 264 us where equal ones take 261; 2^14 times: 1,860 (every step wide); scores past 2^10: 1,210.
+// A half step takes about 2,000 cycles, in which the products are busy for 1,280 (head_dim 128), 2^x for 1,024
+// and the instructions' issue for 900 a scheduler: leaving out any one of them, or the unpacking, in a copy
+// took 2 to 4 % off (17 % for 2^x at head_dim 64), so it is the latency of all of them together.  Steps of 128
+// tokens whose softmax waits for its own products took 261 us where half steps took 243; without the blocks'
+// going on by themselves 243 against 233.
 #include "kv4_attend.cuh"
 #include "launch.cuh"
 #include "rans_host.h"
@@ -249,17 +251,23 @@ __device__ __forceinline__ void hold(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7, from s24 = s * 2^24 and s20 =
-// s * 2^20: the bits of c in the low four bits of a half are c * 2^-24, in the next four c * 2^-20.  The
-// product is exact, so a value is rounded once.
-__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s24, __half2 s20, __half2 o) {
+// 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7.  The bits of c in the low four bits
+// of a half are the subnormal c * 2^-24, in the next four c * 2^-20, and the factors are `low` = s * 2^24 and `high` =
+// s * 2^20.  FULL: with those of 1024 they are 1024 + c and 1024 + 16 c, the 1024 is taken off exactly, and the
+// factors are s and s / 16, which leaves float16's whole range to the rows' sizes.  The product is exact either
+// way, so a value is rounded once.
+template <bool FULL>
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 low, __half2 high, __half2 o) {
   auto value = [&](uint32_t c, __half2 s) {
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c), s, o);
+    if (FULL) c |= 0x64006400u;
+    __half2 v = *reinterpret_cast<const __half2*>(&c);
+    if (FULL) v = __hsub2(v, __float2half2_rn(1024.0f));
+    v = __hfma2(v, s, o);
     return *reinterpret_cast<const uint32_t*>(&v);
   };
   const uint32_t x = w >> 8;
-  return make_uint4(value(w & 0x000f000fu, s24), value(w & 0x00f000f0u, s20), value(x & 0x000f000fu, s24),
-                    value(x & 0x00f000f0u, s20));
+  return make_uint4(value(w & 0x000f000fu, low), value(w & 0x00f000f0u, high), value(x & 0x000f000fu, low),
+                    value(x & 0x00f000f0u, high));
 }
 
 // v * 2^n, n in -252 .. 254
@@ -269,13 +277,37 @@ __device__ __forceinline__ bool finite_row(uint32_t p) {
   return fabsf(scale_of(p)) < INFINITY && fabsf(offset_of(p)) < INFINITY;  // neither for NaN
 }
 // The size of a row's values as an exponent field, 0 for a row that is zero or not finite.  2^(kReach - size)
-// brings the values under 2^-7 and, since 7.5 scales are no more than the largest value, the scale times
-// 2^24 under 2^15.
-constexpr int kReach = 119, kLeast = 6;  // kLeast: smaller ones are taken for this
-constexpr int kSpread = 5;  // rows so much smaller are at 2^-13 still, where float16 rounds to 2^-25
+// brings the values under 2^-7 and, since 7.5 scales are no more than the largest value, the scale times 2^24
+// under 2^15; 2^(kFullReach - size) the values under 2^14.
+constexpr int kReach = 119, kFullReach = 140, kMostShift = 113;
+// Rows of a step that are so much smaller than its largest are at 2^-13 still, where float16 rounds to 2^-25, ...
+constexpr int kSpread = 5;
+// ... and with kFullReach, keys at 2^-7 and their scale / 16 at 2^-14, float16's least normal number.  Values: a
+// token that counts and is so much smaller than one that does not leaves the weights at 2^-6 instead of 2^6, and
+// what float16 cuts off a weight at 2^-19 of the largest.
+constexpr int kSpreadKeys = 20, kSpreadValues = 12;
 __device__ __forceinline__ int size_of(uint32_t p) {
   const float s = scale_of(p), o = offset_of(p), top = fmaxf(fabsf(o), fabsf(fmaf(15.0f, s, o)));
   return finite_row(p) ? min((int)(__float_as_uint(top) >> 23), 254) : 0;
+}
+
+// Half of token t's row, unpacked into its place among the tensor cores' rows, times 2^shift.
+template <int D, bool FULL>
+__device__ __forceinline__ void spread_row(const uint4 (&codes)[D / 64], uint32_t p, int shift, uint8_t* dst, int t,
+                                           int part_of_row) {
+  const float scale = scaled(scale_of(p), shift);
+  const __half2 low = __float2half2_rn(FULL ? scale : scale * 16777216.0f),
+                high = __float2half2_rn(scale * (FULL ? 0.0625f : 1048576.0f)), o = __float2half2_rn(scaled(offset_of(p), shift));
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    const uint32_t w[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int chunk = (part_of_row * (D / 64) + c) * 4 + k;
+      *reinterpret_cast<uint4*>(dst + (chunk >> 3) * Plan<D>::BLOCK + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) =
+          unpack8<FULL>(w[k], low, high, o);
+    }
+  }
 }
 
 // A row of queries: its running maximum m, its sum l of 2^(x - m), and d: weights are 2^(x - m - d) over the
@@ -822,20 +854,9 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         for (int c = 0; c < CODES; ++c) vc[c] = make_uint4(0, 0, 0, 0);
       }
     };
-    auto spread = [&](const uint4 (&codes)[CODES], uint32_t p, int shift, uint8_t* dst) {
-      const float scale = scaled(scale_of(p), shift);
-      const __half2 s24 = __float2half2_rn(scale * 16777216.0f), s20 = __float2half2_rn(scale * 1048576.0f),
-                    o = __float2half2_rn(scaled(offset_of(p), shift));
-#pragma unroll
-      for (int c = 0; c < CODES; ++c) {
-        const uint32_t w[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int chunk = (part_of_row * CODES + c) * 4 + k;
-          *reinterpret_cast<uint4*>(dst + (chunk >> 3) * P::BLOCK + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) =
-              unpack8(w[k], s24, s20, o);
-        }
-      }
+    auto spread = [&](bool full, const uint4 (&codes)[CODES], uint32_t p, int shift, uint8_t* dst) {
+      if (full) spread_row<D, true>(codes, p, shift, dst, t, part_of_row);
+      else spread_row<D, false>(codes, p, shift, dst, t, part_of_row);
     };
     // The queries of the piece whose first step is looked up.  A warp copies 32 rows as they are into
     // their places, LANES lanes a row; then each thread brings a row to float16 by its own power of two.
@@ -929,7 +950,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       const bool bad = state == 1 && !finite_row(vp);
       const uint32_t hidden = __ballot_sync(0xffffffffu, state == 2), wrong = __ballot_sync(0xffffffffu, bad);
       if (any_of<1, 256>(!there || *stalled)) break;  // the ranges are there; or some warp has no more
-      int key_top = kLeast, value_top = kLeast, key_low = 255, value_low = 255;
+      int key_top = 0, value_top = 0, key_low = 255, value_low = 255;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         key_top = max(key_top, (int)(range_k[j & 1][w] >> 16));
@@ -937,23 +958,24 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         value_top = max(value_top, (int)(range_v[j & 1][w] >> 16));
         value_low = min(value_low, (int)(range_v[j & 1][w] & 0xffff));
       }
-      const bool wide = key_low + kSpread < key_top || value_low + kSpread < value_top;
-      const int key_shift = kReach - (wide ? max(key_size, kLeast) : key_top),
-                value_shift = kReach - (wide ? max(value_size, kLeast) : value_top);
+      const bool wide = key_low + kSpreadKeys < key_top || value_low + kSpreadValues < value_top;
+      const bool full_k = !wide && key_low + kSpread < key_top, full_v = !wide && value_low + kSpread < value_top;
+      auto shift = [&](bool full, int size) { return min((full ? kFullReach : kReach) - size, kMostShift); };
+      const int key_shift = shift(full_k, wide ? key_size : key_top), value_shift = shift(full_v, wide ? value_size : value_top);
       bar_wait(&k_empty[stage], filled ^ 1, a.wait_limit, stalled);
       Info& info = infos[j & (kInfos - 1)];
       if (lane == 0 && part_of_row == 0) {
-        const int undo = key_top - kReach;  // the same in all
+        const int undo = -key_shift;  // the same in all, unless the step is wide
         info.key0 = pow2(undo >> 1);
         info.key1 = pow2(undo - (undo >> 1));
-        info.value_shift = (float)(kReach - value_top);
+        info.value_shift = (float)value_shift;
         info.special[quarter] = ((hidden | wrong) != 0) | (wide ? 2 : 0);
         info.hidden[quarter] = hidden;
         info.bad[quarter] = wrong;
       }
       if (wide && part_of_row == 0)
         own_shifts[j & (kInfos - 1)][t] = (uint32_t)value_shift << 16 | (uint32_t)(key_shift & 0xffff);
-      spread(kc, kp, key_shift, smem + P::K + stage * P::ROWS);
+      spread(full_k, kc, kp, key_shift, smem + P::K + stage * P::ROWS);
       fence_smem();
       bar_arrive(&k_full[stage]);
       const uint32_t value_params = bad ? 0 : vp;  // a value that is not finite is left to its rows
@@ -963,7 +985,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
       there = valid;
       look_up();
       bar_wait(&v_empty[stage], filled ^ 1, a.wait_limit, stalled);
-      spread(vc, value_params, value_shift, smem + P::V + stage * P::ROWS);
+      spread(full_v, vc, value_params, value_shift, smem + P::V + stage * P::ROWS);
       fence_smem();
       bar_arrive(&v_full[stage]);
       fetch_values();

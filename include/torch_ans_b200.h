@@ -286,7 +286,8 @@ int tans_kv4_gather(const uint8_t* codes, const void* params, int64_t num_pages,
  *             order or past the queries is skipped and flags TANS_DEV_BAD_VALUE; queries that no
  *             sequence answers are zeros (with -inf in lse), ones of several have one's answer or zeros.
  *             Work past 2^36 tokens or so in one call answers nothing: all zeros, and the flag.
- *   max_queries  the caller's bound on one sequence's queries; it chooses the kernel only.
+ *   max_queries  the caller's bound on one sequence's queries; it chooses the kernel only.  One far
+ *             above the real number may choose the kernel for many rows where the other takes half the time.
  *   lse       float [total_queries, q_heads] or NULL: log of the softmax's sum (-inf for none).
  *   workspace tans_kv4_attend_workspace_size() bytes, 256-byte aligned.  Its first
  *             TANS_KV4_ATTEND_COUNTS bytes are zero before the first call and are left zero by each

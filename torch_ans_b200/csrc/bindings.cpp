@@ -1107,7 +1107,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("kv4_attend", &kv4_attend, py::arg("q"), py::arg("codes"), py::arg("params"), py::arg("pages"),
         py::arg("lengths"), py::arg("q_starts") = py::none(), py::arg("max_queries") = py::none(),
         py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("lse") = py::none(),
-        "Attention of packed queries over a 4-bit paged cache: one token, a few or whole prompts for each sequence.");
+        "Attention of packed queries over a 4-bit paged cache: one token, a few or whole prompts for each sequence. "
+        "max_queries bounds one sequence's queries and chooses the kernel (default: all of them).");
   m.def("kv4_to_symbols", &kv4_to_symbols, py::arg("codes"), py::arg("page_ids"), py::arg("by_channel") = false,
         "Cache pages as coder streams: (symbols, indexes), one row for each page, side and head.");
   m.def("kv4_from_symbols", &kv4_from_symbols, py::arg("symbols"), py::arg("codes"), py::arg("page_ids"),

@@ -13,10 +13,12 @@ static_assert(tans::kv4::Join::kArrivalBytes == TANS_KV4_ATTEND_COUNTS, "the hea
 namespace {
 // Whether the kernel that is bound by the cache's bytes takes the call: `rows` query rows at most share a
 // key/value head.  It reads the cache once for each 8 or 16 of them, the other unpacks it once for 128 or
-// 256.  Measured for head_dim 64, 128, 256: 16 contexts of 8,192 tokens with 4 heads, 32 rows 50, 60 and
-// 109 us against 72, 81 and 205, 64 rows 85, 98 and 200 us against 101, 114 and 205, 96 rows 111, 138 and
-// 290 us against 101, 115 and 258; 64 contexts of 700 tokens with 8 heads, 32 rows 44, 60 and 110 us
-// against 56, 66 and 117, 64 rows 74, 99 and 204 us against 56, 67 and 119.
+// 256.  Measured for head_dim 64, 128, 256: 16 contexts of 8,192 tokens with 4 heads, 32 rows 52, 62 and
+// 113 us against 78, 88 and 212, 48 rows 70, 81 and 158 against 109, 125 and 213, 64 rows 83, 103 and 205
+// against 109, 125 and 213, 96 rows 115, 145 and 297 against 109, 127 and 270; 64 contexts of 700 tokens with 8
+// heads, 32 rows 45, 68 and 115 us against 63, 76 and 124, 48 rows 63, 88 and 167 against 64, 78 and 126, 64
+// rows 80, 110 and 212 against 64, 78 and 127.  Long contexts would take this kernel up to 64 rows and short ones up
+// to 32: the rule looks at the rows alone.
 bool few_rows(int64_t rows) { return rows <= 48; }
 }  // namespace
 

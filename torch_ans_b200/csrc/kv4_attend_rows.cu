@@ -881,8 +881,9 @@ int launch(const AttendArgs& a, void* workspace, cudaStream_t s) {
 }  // namespace
 
 // Row tiles of 16 instead of 8.  The cache is read half as often, and a step costs about 1.3 times as much:
-// at 9 rows or more it pays (16 contexts of 8,192 tokens, 4 heads of 128, 16 rows: 37 against 50 us), but
-// not for head_dim 256, whose sums then do not fit the registers.
+// at 9 rows or more it pays (16 contexts of 8,192 tokens, 4 heads of 128, 16 rows: 39 against 49 us, of 64: 33
+// against 37; 64 contexts of 700 tokens, 8 heads of 128: 43 both), but not for head_dim 256, whose sums then do
+// not fit the registers.
 static bool wide_tiles(int head_dim, int64_t max_rows) { return head_dim <= 128 && max_rows > 8; }
 
 size_t attend_rows_workspace(int head_dim, int64_t max_rows) {

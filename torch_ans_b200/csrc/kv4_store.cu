@@ -84,8 +84,9 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
 //
 // What it may not do without is bytes: 2 read and 2 written for a query's channel, 2 read and about 0.53
 // written for a key's or a value's.  16,381 tokens of 32 + 16 heads of 128 (355 MB) take 95 us, 3.7 TB/s:
-// the instructions (about 160 for two rows of a warp) keep it there.  With 2 rows a group 112 us, with 8
-// about 140 (too few groups at once).  The products and sums of the rotation are rounded one by one (no
+// warps wait for their loads (the largest stall) and for one another's turn, with 0.69 instructions a
+// scheduler and cycle (about 160 for two rows of a warp).  With 2 rows a group 112 us, with 8 about 140 (too
+// few groups at once).  The products and sums of the rotation are rounded one by one (no
 // fused multiply-add), so the codes do not depend on the compiler's choices.
 //
 // The quotient (x - offset) / scale is the correctly rounded one, so that ties (common: x has 8 or 11
@@ -239,7 +240,8 @@ int launch_append(const AppendArgs& a, bool vec, bool interleaved, cudaStream_t 
 }
 
 // Values of the rows in `slots`: head_dim / 8 lanes for each row.  16,381 tokens of 16 rows of 128 (85 MB,
-// four fifths of them written) take 26 us, 3.2 TB/s.
+// four fifths of them written) take 26 us, 3.2 TB/s: a lane's slot, codes and parameters are three loads in a row
+// with nothing else in flight (they are by far the largest stall).
 template <int D, typename T>
 __global__ void __launch_bounds__(kThreads) gather_kernel(Pool pool, PageOf page_of, Divider per_token,
                                                           const int64_t* slots, int64_t tokens, T* k_out, T* v_out,

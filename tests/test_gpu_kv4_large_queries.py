@@ -45,3 +45,19 @@ def test_large_scores_with_values_of_all_sizes(C, counts, dim, dtype, exponent):
     q, wanted = c.queries(counts, 4, dtype)
     out, bound = c.answers(q, wanted, counts)
     assert not c.wrong(c.attend(C, q, counts), out, bound).any() and C.device_status() == 0
+
+
+@pytest.mark.parametrize("exponent", [10, 14, 20, 40, 60])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [7, 3, 5]])
+def test_equal_large_scores_wherever_they_are(C, counts, dim, exponent):
+    """Blocks of 128 tokens, which many warps share: their equal scores stay equal beside others that are far away."""
+    c = Planted([353, 143, 1880], 32, 2, dim, 128, seed=dim + 1)
+    for b, n in enumerate(c.lengths):
+        c.resize(b, range(n), 0, exponent)
+    c.unlikely(2, [700, 1100, 1200])
+    c.resize(2, [700, 1100, 1200], 1, 16)
+    for first in (0, 5, 11):
+        q, wanted = c.queries(counts, 4, torch.bfloat16, beta={64: 26.0, 128: 36.0, 256: 50.0}[dim], first=first)
+        out, bound = c.answers(q, wanted, counts)
+        assert not c.wrong(c.attend(C, q, counts), out, bound).any() and C.device_status() == 0

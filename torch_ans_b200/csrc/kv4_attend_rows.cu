@@ -29,7 +29,8 @@
 // above m - 96, so where values are tiny the weights stay in float's range.  m and Y move only when a score
 // passes m by over 8, or when a lane's largest score and largest size (of four tokens) together pass Y by
 // 14 (w is then under 2^15): most steps compare and go on.  Where |m| passes 2^10 the column's scores get an
-// origin there, taken off before anything else is added to them, so that Y and R stay as exact as they are.
+// origin, their largest one itself, taken off before anything else is added to them: equal scores stay equal, in
+// whatever warp, and Y and R as exact as they are.
 //
 // Measured: 48 contexts of 256 to 16,384 tokens (222k together, 32 query and 8 key/value heads of 128, 242
 // MB) 74 us, 3.3 TB/s: about 570 instructions a step, the ALU pipe half busy, and each item's start and end;
@@ -578,20 +579,23 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, NT)) attend_rows_ker
             for (int c = 0; c < 2; ++c) {
               float& x = s[j >> 1][n][(j & 1) * 2 + c];
               x = fmaf(x * sk, fac[n][c], ok * shift[n][c]);
-              if (masked && apart) {
-                if (large[n] >> (8 * t + 4 * c) & 1) x *= 16777216.0f;
-                x -= c ? origin[n * 4 + t].y : origin[n * 4 + t].x;
-              }
+              if (masked && (large[n] >> (8 * t + 4 * c) & 1)) x *= 16777216.0f;
               if (masked && !(in[j] && token < seen[n][c])) x = -INFINITY;
               top[n][c] = fmaxf(top[n][c], x);
             }
         }
         const float reach = exponent(big) - kRoom;
+        // scores are as they are until their origin, which may move, is taken off below
+        float from[NT][2];
         bool move = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) move |= top[n][c] > m[n][c] + kSlack || top[n][c] + reach > Y[n][c];
+          for (int c = 0; c < 2; ++c) {
+            from[n][c] = !masked || !apart ? 0.0f : (c ? origin[n * 4 + t].y : origin[n * 4 + t].x);
+            const float x = top[n][c] - from[n][c];
+            move |= x > m[n][c] + kSlack || x + reach > Y[n][c];
+          }
         if (__any_sync(0xffffffffu, move)) {
           // the columns' reductions side by side: the largest scores, then the largest products
           float now[NT][2], y[NT][2];
@@ -604,30 +608,27 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, NT)) attend_rows_ker
 #pragma unroll
           for (int i = 0; i < 2 * NT; ++i) now[i >> 1][i & 1] = top[i >> 1][i & 1];
           across(now);
-          bool far = false;
+          bool far[NT][2], some_far = false;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              now[n][c] = now[n][c] > m[n][c] + kSlack ? now[n][c] : m[n][c];
-              far |= now[n][c] != -INFINITY && fabsf(now[n][c]) > kFar;
+              const float x = now[n][c] - from[n][c];
+              far[n][c] = x > m[n][c] + kSlack && fabsf(x) > kFar;
+              some_far |= far[n][c];
             }
-          if (__any_sync(0xffffffffu, far)) {
+          if (__any_sync(0xffffffffu, some_far)) {  // their origin becomes the largest score itself
             apart = true;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                float* const at = reinterpret_cast<float*>(origin) + (n * 4 + t) * 2 + c;
-                const bool moves = now[n][c] != -INFINITY && fabsf(now[n][c]) > kFar;
-                const float old = *at, to = old + (moves ? now[n][c] : 0.0f), from = to - old;
-                now[n][c] -= from;
-                Y[n][c] = m[n][c] == -INFINITY ? kNone : Y[n][c] - from;
-                m[n][c] -= from;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[j >> 1][n][(j & 1) * 2 + c] -= from;
-                __syncwarp();
-                if (g == 0) *at = to;
+                if (!far[n][c]) continue;
+                const float by = now[n][c] - from[n][c];
+                Y[n][c] = m[n][c] == -INFINITY ? kNone : Y[n][c] - by;
+                m[n][c] -= by;
+                from[n][c] = now[n][c];
+                if (g == 0) reinterpret_cast<float*>(origin)[(n * 4 + t) * 2 + c] = now[n][c];
               }
             __syncwarp();
           }
@@ -635,10 +636,12 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, NT)) attend_rows_ker
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+              now[n][c] -= from[n][c];
+              now[n][c] = now[n][c] > m[n][c] + kSlack ? now[n][c] : m[n][c];
               y[n][c] = -INFINITY;
 #pragma unroll
               for (int j = 0; j < 4; ++j)  // a token that the row does not see is at -inf, whatever its size
-                y[n][c] = fmaxf(y[n][c], s[j >> 1][n][(j & 1) * 2 + c] + exponent(fmaxf(fabsf(sv[j]), fabsf(ov[j]))));
+                y[n][c] = fmaxf(y[n][c], s[j >> 1][n][(j & 1) * 2 + c] - from[n][c] + exponent(fmaxf(fabsf(sv[j]), fabsf(ov[j]))));
             }
           across(y);
 #pragma unroll
@@ -661,6 +664,12 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, NT)) attend_rows_ker
               m[n][c] = now[n][c];
               Y[n][c] = Y_now;
             }
+        }
+        if (apart) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i >> 2][n][i & 3] -= from[n][i & 1];
         }
         float base[NT][2], less[NT][2];
 #pragma unroll

@@ -49,9 +49,10 @@ def test_large_scores_with_values_of_all_sizes(C, counts, dim, dtype, exponent):
 
 @pytest.mark.parametrize("exponent", [10, 14, 20, 40, 60])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("counts", [[1, 1, 1], [7, 3, 5]])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [7, 3, 5], [300, 143, 718]])
 def test_equal_large_scores_wherever_they_are(C, counts, dim, exponent):
-    """Blocks of 128 tokens, which many warps share: their equal scores stay equal beside others that are far away."""
+    """Blocks of 128 tokens, which many warps share: their equal scores stay equal beside others that are far away, and after steps
+    whose values differ by more than 2^12."""
     c = Planted([353, 143, 1880], 32, 2, dim, 128, seed=dim + 1)
     for b, n in enumerate(c.lengths):
         c.resize(b, range(n), 0, exponent)

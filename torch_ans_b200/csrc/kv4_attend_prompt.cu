@@ -587,6 +587,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
           const uint32_t* const own = wide ? own_shifts[(steps_done + j) & (kInfos - 1)] + h * kHalf : nullptr;
           softmax = by_token<D>(softmax, wide ? factor : f, now, own, visible0, visible1, at, o_at,
                                 n > 0 ? &o_done[tile] : nullptr, (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
+          far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > kFar);
           stored();
           fence_before();
           bar_arrive(&p_full[tile][h]);
@@ -631,8 +632,7 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         if (__any_sync(0xffffffffu, top > m + fminf(kSlack, d + now + kRoom))) {
           softmax.follow<D>(top, [&](float next) { return top - next - now; }, o_at, n > 0 ? &o_done[tile] : nullptr,
                             (done0 + done1 + n - 1) & 1, a.wait_limit, stalled);
-          far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > kFar);
-          if (far) {
+          if (__any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > kFar)) {
             token_by_token(visible[0], visible[1]);
             continue;
           }

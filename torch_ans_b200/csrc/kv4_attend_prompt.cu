@@ -22,7 +22,7 @@
 //
 // All operands are float16 brought into range by powers of two: a query row by its own, the keys and the
 // values of a step by one each.  Rows that differ by over 2^5 need another conversion (1 % of the time if all steps
-// do); rows that differ by more than 2^20 (keys) or 2^12 (values) would lose bits of themselves or of the weights:
+// do); rows that differ by more than 2^11 (keys) or 2^8 (values) would lose bits of themselves or of the weights:
 // a step with such rows is "wide", and there each row has its own factor, which the softmax warps put into
 // its scores and weights, in some seven times the time.  So the rounding is 2^-11
 // of each key, each value and each weight, whatever the sizes of other tokens, of those that are hidden
@@ -36,10 +36,10 @@
 // wide step: the product's rounding would otherwise be a factor of the weight, past float's range from 2^30.
 //
 // Measured: 4 packed prompts of 1,143 to 3,500 tokens (32 query and 8 key/value heads of 128, 166 GFLOP) 236
-// us, 703 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 166 us, 412 TFLOP/s.  With one power
+// us, 703 TFLOP/s; 511 queries over 32,749 tokens (16 and 4 heads of 64, 68 GFLOP) 169 us, 402 TFLOP/s.  With one power
 // of two for all values so far and none for single rows these took 228 and 161 us on the same GPU, and a value 2^16
 // times larger in a step, seen or not, left other queries' answers a fifth wrong.  Such prompts with one row in
-// 16 2^8 times larger: 264 us where equal ones take 261; 2^14 times: 1,860 (every step wide); scores past 2^10: 1,210.
+// 16 2^4 times larger: 263 us where others take 260; 2^14 times: 1,860 (every step wide); scores past 2^10: 1,210.
 // A half step takes about 2,000 cycles, in which the products are busy for 1,280 (head_dim 128), 2^x for 1,024
 // and the instructions' issue for 900 a scheduler: leaving out any one of them, or the unpacking, in a copy
 // took 2 to 4 % off (17 % for 2^x at head_dim 64), so it is the latency of all of them together.  Steps of 128
@@ -253,18 +253,17 @@ __device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.a
 
 // 8 codes as float16 values c * s + o, in the order 0, 4, 1, 5, 2, 6, 3, 7.  The bits of c in the low four bits
 // of a half are the subnormal c * 2^-24, in the next four c * 2^-20, and the factors are `low` = s * 2^24 and `high` =
-// s * 2^20.  FULL: with those of 1024 they are 1024 + c and 1024 + 16 c, the 1024 is taken off exactly, and the
-// factors are s and s / 16, which leaves float16's whole range to the rows' sizes.  The product is exact either
-// way, so a value is rounded once.
+// s * 2^20.  FULL: all are brought to bits 6 to 9, c * 2^-18, and the factor `low` is s * 2^18, which leaves 6 more
+// powers of two to the rows' sizes.  The product is exact either way, so a value is rounded once.
 template <bool FULL>
 __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 low, __half2 high, __half2 o) {
   auto value = [&](uint32_t c, __half2 s) {
-    if (FULL) c |= 0x64006400u;
-    __half2 v = *reinterpret_cast<const __half2*>(&c);
-    if (FULL) v = __hsub2(v, __float2half2_rn(1024.0f));
-    v = __hfma2(v, s, o);
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c), s, o);
     return *reinterpret_cast<const uint32_t*>(&v);
   };
+  if constexpr (FULL)
+    return make_uint4(value(w << 6 & 0x03c003c0u, low), value(w << 2 & 0x03c003c0u, low), value(w >> 2 & 0x03c003c0u, low),
+                      value(w >> 6 & 0x03c003c0u, low));
   const uint32_t x = w >> 8;
   return make_uint4(value(w & 0x000f000fu, low), value(w & 0x00f000f0u, high), value(x & 0x000f000fu, low),
                     value(x & 0x00f000f0u, high));
@@ -278,14 +277,14 @@ __device__ __forceinline__ bool finite_row(uint32_t p) {
 }
 // The size of a row's values as an exponent field, 0 for a row that is zero or not finite.  2^(kReach - size)
 // brings the values under 2^-7 and, since 7.5 scales are no more than the largest value, the scale times 2^24
-// under 2^15; 2^(kFullReach - size) the values under 2^14.
-constexpr int kReach = 119, kFullReach = 140, kMostShift = 113;
-// Rows of a step that are so much smaller than its largest are at 2^-13 still, where float16 rounds to 2^-25, ...
-constexpr int kSpread = 5;
-// ... and with kFullReach, keys at 2^-7 and their scale / 16 at 2^-14, float16's least normal number.  Values: a
-// token that counts and is so much smaller than one that does not leaves the weights at 2^-6 instead of 2^6, and
-// what float16 cuts off a weight at 2^-19 of the largest.
-constexpr int kSpreadKeys = 20, kSpreadValues = 12;
+// under 2^15.
+constexpr int kReach = 119, kMostShift = 113;
+// Rows of a step that are so much smaller than its largest are at 2^-13 still, where float16 rounds to 2^-25.  Keys
+// further apart, up to kSpreadKeys, and values up to kSpreadValues, are all made larger by what is missing, up to
+// 2^6 (keys) or 2^3 (values).  Values stop there because the weights of a step become as much smaller, and smaller
+// again by what a token that counts is smaller than one that does not: from 2^6 to 2^-5 at the most, where what float16
+// cuts off a weight is 2^-20 of the largest.
+constexpr int kSpread = 5, kSpreadKeys = 11, kSpreadValues = 8;
 __device__ __forceinline__ int size_of(uint32_t p) {
   const float s = scale_of(p), o = offset_of(p), top = fmaxf(fabsf(o), fabsf(fmaf(15.0f, s, o)));
   return finite_row(p) ? min((int)(__float_as_uint(top) >> 23), 254) : 0;
@@ -296,8 +295,8 @@ template <int D, bool FULL>
 __device__ __forceinline__ void spread_row(const uint4 (&codes)[D / 64], uint32_t p, int shift, uint8_t* dst, int t,
                                            int part_of_row) {
   const float scale = scaled(scale_of(p), shift);
-  const __half2 low = __float2half2_rn(FULL ? scale : scale * 16777216.0f),
-                high = __float2half2_rn(scale * (FULL ? 0.0625f : 1048576.0f)), o = __float2half2_rn(scaled(offset_of(p), shift));
+  const __half2 low = __float2half2_rn(scale * (FULL ? 262144.0f : 16777216.0f)), high = __float2half2_rn(scale * 1048576.0f),
+                o = __float2half2_rn(scaled(offset_of(p), shift));
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
     const uint32_t w[4] = {codes[c].x, codes[c].y, codes[c].z, codes[c].w};
@@ -959,9 +958,11 @@ __global__ void __launch_bounds__(Plan<D>::WARPS * 32, 1) attend_prompt_kernel(c
         value_low = min(value_low, (int)(range_v[j & 1][w] & 0xffff));
       }
       const bool wide = key_low + kSpreadKeys < key_top || value_low + kSpreadValues < value_top;
-      const bool full_k = !wide && key_low + kSpread < key_top, full_v = !wide && value_low + kSpread < value_top;
-      auto shift = [&](bool full, int size) { return min((full ? kFullReach : kReach) - size, kMostShift); };
-      const int key_shift = shift(full_k, wide ? key_size : key_top), value_shift = shift(full_v, wide ? value_size : value_top);
+      // what rows are too far apart for the ordinary conversion
+      const int more_k = wide ? 0 : max(0, key_top - key_low - kSpread), more_v = wide ? 0 : max(0, value_top - value_low - kSpread);
+      const bool full_k = more_k > 0, full_v = more_v > 0;
+      const int key_shift = min(kReach + more_k - (wide ? key_size : key_top), kMostShift),
+                value_shift = min(kReach + more_v - (wide ? value_size : value_top), kMostShift);
       bar_wait(&k_empty[stage], filled ^ 1, a.wait_limit, stalled);
       Info& info = infos[j & (kInfos - 1)];
       if (lane == 0 && part_of_row == 0) {

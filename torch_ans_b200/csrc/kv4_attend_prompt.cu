@@ -21,8 +21,8 @@
 // sums in the workspace, and the last of them joins them in the order of the tokens.
 //
 // All operands are float16 brought into range by powers of two: a query row by its own, the keys and the
-// values of a step by one each.  Rows that differ by over 2^5 need another conversion (1 % of the time if all steps
-// do); rows that differ by more than 2^11 (keys) or 2^8 (values) would lose bits of themselves or of the weights:
+// values of a step by one each.  Rows that differ by over 2^5 need another conversion (1 % more time if all steps
+// have such); rows that differ by more than 2^11 (keys) or 2^8 (values) would lose bits of themselves or of the weights:
 // a step with such rows is "wide", and there each row has its own factor, which the softmax warps put into
 // its scores and weights, in some seven times the time.  So the rounding is 2^-11
 // of each key, each value and each weight, whatever the sizes of other tokens, of those that are hidden

@@ -33,7 +33,7 @@
 // whatever warp, and Y and R as exact as they are.
 //
 // Measured: 48 contexts of 256 to 16,384 tokens (222k together, 32 query and 8 key/value heads of 128, 242
-// MB) 74 us, 3.3 TB/s: about 570 instructions a step, the ALU pipe half busy, and each item's start and end;
+// MB) 75 us, 3.2 TB/s: about 570 instructions a step, the ALU pipe half busy, and each item's start and end;
 // 3 contexts of about 127k tokens (16 and 2 heads, 103 MB) 43 us, of which the steps are about 20 (5 to 6
 // TB/s), the start 6 and the joins of 97 blocks an item 10; one context of 777 tokens 12 us, all latency.
 // With one factor for all rows of a warp instead of a Y for each row the ragged batch took 72 us, and a value 2^20
